@@ -7,6 +7,8 @@ artifact                       source                                      toolc
 =============================  ==========================================  =========
 ``libtk_gpu_probe.so``         ``csrc/tk_gpu_probe.hip`` (HBM/MFMA/memtest)  hipcc
 ``libtk_gemm.so``              ``csrc/tk_gemm_screen.hip`` (ABFT GEMM screen)  hipcc
+``libtk_loss.so``              ``csrc/tk_loss.hip`` (output-head losses)      hipcc
+``libtk_gemv.so``              ``csrc/tk_gemv_w4.hip`` (4-bit products)       hipcc
 ``libtk_rccl.so``              ``csrc/tk_rccl_probe.hip`` (N2, RCCL)          hipcc
 ``rccl-ready``                 same, ``-DTK_RCCL_MAIN``                     hipcc
 ``libtk_rccl_stub.so``         ``csrc/tk_rccl_stub.cpp`` (the ABI, no GPU)    g++
@@ -44,6 +46,9 @@ HIP_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-Wno-unused-result"
 RPATH = [f"-Wl,-rpath,{ROCM}/lib"]
 # VGPR-form MFMA accumulators: see the note at the top of csrc/tk_gpu_probe.hip
 MFMA_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+# no packed fp32 instructions: the compiler forms them from ordinary float code, and some of
+# their operand forms have given wrong results on this hardware
+SCALAR_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 @dataclass
@@ -119,6 +124,8 @@ def targets() -> List[Target]:
     probe = os.path.join(CSRC, "tk_gpu_probe.hip")
     rccl = os.path.join(CSRC, "tk_rccl_probe.hip")
     gemm = os.path.join(CSRC, "tk_gemm_screen.hip")
+    loss = os.path.join(CSRC, "tk_loss.hip")
+    gemv = os.path.join(CSRC, "tk_gemv_w4.hip")
     topo = os.path.join(CSRC, "tk_topo.cpp")
     stub = os.path.join(CSRC, "tk_rccl_stub.cpp")
     rccl_h = [os.path.join(CSRC, "tk_rccl_group.h"), os.path.join(CSRC, "tk_rccl_verify.h"),
@@ -132,6 +139,10 @@ def targets() -> List[Target]:
                [hipcc, *HIP_FLAGS, *MFMA_FLAGS, "-DTK_PROBE_MAIN", probe, gemm, "-o", out("gpu-burnin"), *RPATH]),
         Target("libtk_gemm.so", [gemm],
                [hipcc, *HIP_FLAGS, "-fPIC", "-shared", gemm, "-o", out("libtk_gemm.so"), *RPATH]),
+        Target("libtk_loss.so", [loss],
+               [hipcc, *HIP_FLAGS, *SCALAR_F32, "-fPIC", "-shared", loss, "-o", out("libtk_loss.so"), *RPATH]),
+        Target("libtk_gemv.so", [gemv],
+               [hipcc, *HIP_FLAGS, *SCALAR_F32, "-fPIC", "-shared", gemv, "-o", out("libtk_gemv.so"), *RPATH]),
         Target("libtk_rccl.so", [rccl, *rccl_h],
                [hipcc, *HIP_FLAGS, "-fPIC", "-shared", rccl, "-o", out("libtk_rccl.so"), f"-L{ROCM}/lib",
                 "-lrccl", *RPATH]),

@@ -1,0 +1,152 @@
+"""Python front-end of the 4-bit matrix-vector products (``csrc/tk_gemv_w4.hip``).
+
+``gemv_w4(x, codes, scales, zeros)`` multiplies 1 to 64 rows of ``x`` -- one token, or a
+decode batch -- with a weight of 4-bit codes and a scale (and a zero) per group of columns,
+``w[n][k] = scales[n][k // group] * (codes[n][k] - zeros[n][k // group])``.  Like
+``gemm.gemm_bt`` it takes torch tensors on the GPU and queues its work on torch's current
+stream of that device.  ``quantize_w4``, ``pack_w4`` and ``dequantize_w4`` make such weights
+and undo them, on any device.
+"""
+
+import ctypes
+from typing import Any, Optional, Tuple
+
+from .native import load
+
+MAX_ROWS = 64
+MAX_OUT = 1 << 24
+MAX_IN = 1 << 20
+SYMMETRIC_ZERO = 8  # the zero of weights without zeros
+
+
+class GemvError(RuntimeError):
+    pass
+
+
+_loaded = None
+
+
+def _lib():
+    global _loaded
+    if _loaded is None:
+        lib = load("libtk_gemv.so")
+        lib.tkv_last_error.restype = ctypes.c_char_p
+        i, ll, p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
+        lib.tkv_gemv_w4.argtypes = [i, i, p, ll, p, p, p, p, ll, i, i, i, i, p]
+        _loaded = lib
+    return _loaded
+
+
+def _check_weight(codes, scales, zeros) -> Tuple[int, int, int]:
+    """``(n, k, group)`` of a packed weight."""
+    import torch
+
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0]:
+        raise GemvError(f"wants codes uint8 [N, K/2] and scales [N, K/group], not {codes.dtype} {list(codes.shape)} "
+                        f"and {list(scales.shape)}")
+    n, k, groups = codes.shape[0], codes.shape[1] * 2, scales.shape[1]
+    if not groups or not k or k % groups or (k // groups) % 32:
+        raise GemvError(f"{groups} groups do not divide {k} columns into groups of a multiple of 32")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise GemvError(f"wants zeros uint8 {list(scales.shape)}, not {zeros.dtype} {list(zeros.shape)}")
+    return n, k, k // groups
+
+
+def gemv_w4(x, codes, scales, zeros=None, *, out=None):
+    """``x @ w.T`` for ``x [..., K]`` of at most 64 rows, bf16 or fp16, of any strides.
+
+    ``codes`` is uint8 ``[N, K/2]``, two codes to a byte, the lower half first; ``scales``
+    ``[N, K/group]`` has ``x``'s type, ``zeros`` (uint8, the same shape) may be left out for
+    symmetric weights, whose zero is 8.  The weight's tensors are contiguous; ``group`` is a
+    multiple of 32.  Sums are fp32 and rounded once.  The result (``out``, if given: contiguous,
+    ``[..., N]``) has ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that
+    wants one is refused."""
+    import torch
+
+    from .native import require_torch_first
+
+    require_torch_first()
+    if x.dtype not in (torch.bfloat16, torch.float16) or scales.dtype != x.dtype:
+        raise GemvError(f"gemv_w4 wants x and scales both bf16 or both fp16, not {x.dtype} and {scales.dtype}")
+    n, k, group = _check_weight(codes, scales, zeros)
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise GemvError(f"x {list(x.shape)} does not go with {k} columns")
+    if n > MAX_OUT or k > MAX_IN:
+        raise GemvError(f"a weight of {n} x {k} (at most {MAX_OUT} x {MAX_IN})")
+    weight = (codes, scales) if zeros is None else (codes, scales, zeros)
+    if not x.is_cuda or any(t.device != x.device for t in weight):
+        raise GemvError("gemv_w4 wants CUDA tensors on one device")
+    if not all(t.is_contiguous() for t in weight) or codes.data_ptr() % 16:
+        raise GemvError("gemv_w4 wants a contiguous weight, its codes 16-byte aligned")
+    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad):
+        raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
+    m = x.numel() // k
+    if m > MAX_ROWS:
+        raise GemvError(f"{m} rows of x (at most {MAX_ROWS}): dequantize_w4 and a matrix product serve more")
+    shape = (*x.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+        raise GemvError(f"out must be contiguous {x.dtype} {list(shape)} on x's device")
+    if m == 0 or n == 0:
+        return out
+    x = x.reshape(m, k)
+    if x.stride(1) != 1 or x.stride(0) < k or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    rc = _lib().tkv_gemv_w4(x.device.index, x.dtype == torch.float16, x.data_ptr(), x.stride(0), codes.data_ptr(),
+                            scales.data_ptr(), None if zeros is None else zeros.data_ptr(), out.data_ptr(), n, m, n, k,
+                            group, torch.cuda.current_stream(x.device).cuda_stream)
+    if rc != 0:
+        raise GemvError(_lib().tkv_last_error().decode())
+    return out
+
+
+def pack_w4(codes):
+    """Codes 0 to 15, uint8 ``[N, K]``, as ``[N, K/2]``: two to a byte, the lower half first."""
+    import torch
+
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] % 2:
+        raise GemvError(f"pack_w4 wants uint8 [N, K] with an even K, not {codes.dtype} {list(codes.shape)}")
+    if codes.numel() and int(codes.max()) > 15:
+        raise GemvError("pack_w4 wants codes 0 to 15")
+    return codes[:, 0::2] | (codes[:, 1::2] << 4)
+
+
+def quantize_w4(w, group: int = 128, symmetric: bool = True) -> Tuple[Any, Any, Optional[Any]]:
+    """``(codes, scales, zeros)`` of a bf16 or fp16 weight ``[N, K]``, each value to the code
+    nearest to it; ``zeros`` is None for a symmetric weight.  A symmetric group's scale is its
+    largest magnitude / 7; else scale and zero span the group's values (and 0) with 15 steps."""
+    import torch
+
+    if w.dtype not in (torch.bfloat16, torch.float16) or w.dim() != 2:
+        raise GemvError(f"quantize_w4 wants bf16 or fp16 [N, K], not {w.dtype} {list(w.shape)}")
+    n, k = w.shape
+    if group < 32 or group % 32 or k < group or k % group:
+        raise GemvError(f"a group of {group} must be a multiple of 32 that divides {k} columns")
+    v = w.detach().float().reshape(n, k // group, group)
+    if not bool(torch.isfinite(v).all()):
+        raise GemvError("quantize_w4 wants finite weights")
+    if symmetric:
+        scales = (v.abs().amax(2) / 7).to(w.dtype)
+        zeros = None
+    else:
+        lo, hi = v.amin(2).clamp_max(0), v.amax(2).clamp_min(0)
+        scales = ((hi - lo) / 15).to(w.dtype)
+    # codes go by the rounded scale; a scale of 0 (a group of zeros, or too small for the type) has code = zero
+    step = scales.float()
+    inv = torch.where(step > 0, 1 / step, 0.0)
+    if not symmetric:
+        zeros = (-lo * inv).round().clamp(0, 15).to(torch.uint8)
+    zero = float(SYMMETRIC_ZERO) if zeros is None else zeros.float()[:, :, None]
+    codes = (v * inv[:, :, None] + zero).round().clamp(0, 15).to(torch.uint8)
+    return pack_w4(codes.reshape(n, k)), scales, zeros
+
+
+def dequantize_w4(codes, scales, zeros=None):
+    """The weight ``[N, K]`` in fp32."""
+    import torch
+
+    n, k, group = _check_weight(codes, scales, zeros)
+    c = torch.stack((codes & 15, codes >> 4), 2).reshape(n, k // group, group).float()
+    zero = float(SYMMETRIC_ZERO) if zeros is None else zeros.float()[:, :, None]
+    return ((c - zero) * scales.float()[:, :, None]).reshape(n, k)

@@ -19,7 +19,7 @@ _cache: Dict[str, ctypes.CDLL] = {}
 # Whether the first HIP library was loaded before torch: torch bundles its own
 # libamdhip64 / librccl under the same sonames as /opt/rocm's, and the one loaded first
 # serves the whole process; torch imported afterwards would run on the other build.
-_HIP_LIBS = {"libtk_gpu_probe.so", "libtk_gemm.so", "libtk_rccl.so"}
+_HIP_LIBS = {"libtk_gpu_probe.so", "libtk_gemm.so", "libtk_loss.so", "libtk_gemv.so", "libtk_rccl.so"}
 _hip_before_torch = None
 
 
