@@ -130,3 +130,21 @@ def test_quantized_values_are_the_nearest(dt, symmetric):
     assert bool(((back - w.float()).abs() <= most * step + 1e-30).all())
     assert bool((back[4] == 0).all())
 
+
+@pytest.mark.parametrize("argv", [["loss", "--tokens", "0"], ["loss", "--dtype", "fp8"], ["gemv", "--rows", "0"],
+                                  ["gemv", "--group", "x"]])
+def test_screen_commands_check_their_counts(argv, capsys):
+    from triton_kubernetes_amd.ops import cli
+
+    with pytest.raises(SystemExit) as exc:
+        cli.main(argv)
+    assert exc.value.code == 2
+
+
+@pytest.mark.parametrize("argv", [["loss"], ["gemv"]])
+def test_screen_commands_without_a_gpu(argv, capsys, monkeypatch):
+    from triton_kubernetes_amd.ops import cli
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    assert cli.main(argv) == 2
+    assert "tk-gpu: no GPU" in capsys.readouterr().err

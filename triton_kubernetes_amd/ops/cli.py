@@ -10,6 +10,8 @@
     python -m triton_kubernetes_amd.ops.cli hbm|mfma [...] [--clock]
     python -m triton_kubernetes_amd.ops.cli rccl-slim [--source DIR] [--root DIR] [--no-verify]
     python -m triton_kubernetes_amd.ops.cli gemm [--size N] [--reps R] [--schedule staggered|single-barrier] [--dtype bf16|fp8]
+    python -m triton_kubernetes_amd.ops.cli loss [--tokens N] [--vocab V] [--hidden D] [--reps R] [--dtype bf16|fp16]
+    python -m triton_kubernetes_amd.ops.cli gemv [--rows M] [--out N] [--inp K] [--group G] [--reps R] [--dtype bf16|fp16]
 
 Every command prints one JSON document (``metrics``: Prometheus text); the exit status is
 non-zero when the GPU(s) fail the gate.
@@ -27,12 +29,14 @@ def main(argv: Sequence[str] = ()) -> int:
     line on stderr and exit 2, not a traceback."""
     from ..errors import TKError
     from .gemm import GemmError
+    from .gemv import GemvError
+    from .loss import LossError
     from .native import NativeUnavailable
     from .probe import ProbeError
 
     try:
         return _main(argv)
-    except (TKError, GemmError, NativeUnavailable, ProbeError, ValueError) as exc:
+    except (TKError, GemmError, GemvError, LossError, NativeUnavailable, ProbeError, ValueError) as exc:
         print(f"tk-gpu: {exc}", file=sys.stderr)
         return 2
 
@@ -113,6 +117,21 @@ def _main(argv: Sequence[str]) -> int:
                    help="GEMM main loop (single-barrier: the earlier loop, for A/B; bf16 only)")
     g.add_argument("--dtype", default="bf16", choices=["bf16", "fp8"],
                    help="operands: bf16, or fp8 e4m3 through the block-scaled MFMA")
+    ls = sub.add_parser("loss", help="a training step's output head (loss and gradients), checked (needs PyTorch)")
+    ls.add_argument("--device", type=_num(0), default=0)
+    ls.add_argument("--tokens", type=_num(1), default=4096)
+    ls.add_argument("--vocab", type=_num(1), default=32768)
+    ls.add_argument("--hidden", type=_num(1), default=4096)
+    ls.add_argument("--reps", type=_num(1), default=3)
+    ls.add_argument("--dtype", default="bf16", choices=["bf16", "fp16"])
+    gv = sub.add_parser("gemv", help="a token's product with a 4-bit weight, checked (needs PyTorch)")
+    gv.add_argument("--device", type=_num(0), default=0)
+    gv.add_argument("--rows", type=_num(1), default=1, help="tokens at once, at most 64")
+    gv.add_argument("--out", type=_num(1), default=16384)
+    gv.add_argument("--inp", type=_num(1), default=16384, help="a multiple of the group")
+    gv.add_argument("--group", type=_num(1), default=128, help="columns of a scale, a multiple of 32")
+    gv.add_argument("--reps", type=_num(1), default=20)
+    gv.add_argument("--dtype", default="bf16", choices=["bf16", "fp16"])
     m.add_argument("--clock", action="store_true",
                    help="also report the in-kernel clock and FLOP/clk/SIMD (stamped diagnostic launch)")
     args = ap.parse_args(list(argv) or sys.argv[1:])
@@ -201,6 +220,15 @@ def _main(argv: Sequence[str]) -> int:
         gemm.set_schedule(args.schedule)
         res = gemm.screen(args.device, args.size, args.size, args.size, args.reps, dtype=args.dtype)
         print(json.dumps(dict(res.to_json(), schedule=args.schedule if args.dtype == "bf16" else "staggered")))
+        return 0 if res.ok else 1
+    if args.cmd in ("loss", "gemv"):
+        from . import head_screen
+
+        if args.cmd == "loss":
+            res = head_screen.loss_screen(args.device, args.tokens, args.vocab, args.hidden, args.reps, args.dtype)
+        else:
+            res = head_screen.gemv_screen(args.device, args.rows, args.out, args.inp, args.group, args.reps, args.dtype)
+        print(json.dumps(res.to_json()))
         return 0 if res.ok else 1
     return 2
 
