@@ -124,6 +124,23 @@ __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// 16 bytes a lane from a buffer (offset `voff`, zeros past its end) to LDS at `lds` + 16 lane.
+// In asm, because the compiler would wait for every copy in flight before each
+// ds_read_b64_tr_b16 (2.25 instead of 1.83 ms for k_dx and k_dw at 8192 x 4096 x 32768); product() does the
+// waiting.  The copy has no register output; it reads its operands when it is issued.
+__device__ __forceinline__ void copy16(u32x4 buffer, unsigned voff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff),
+               "s"(buffer)
+               : "memory", "m0");
+}
+__device__ __forceinline__ u32x4 buffer_of(const char* base, unsigned bytes) {
+  const unsigned long long b = reinterpret_cast<unsigned long long>(base);
+  // (the readfirstlanes are no instructions where the values are scalar already: they only
+  // make the compiler keep the descriptor in scalar registers)
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)b), hi = __builtin_amdgcn_readfirstlane((unsigned)(b >> 32));
+  return u32x4{lo, hi & 0xffffu, (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+
 // One 256-wide panel of an operand.  ALONG: a row of the panel lies along K (128 rows of 128
 // bytes are a half-tile); else K is the matrix's row index (64 rows of 128 columns), and the
 // fragments are transposed on their way out of LDS.
@@ -135,29 +152,26 @@ struct Panel;
 template <>
 struct Panel<true> {
   const char* base;
-  long long bytes;  // from base to the end of the last valid row
-  int ld, kbytes;   // row stride, valid bytes of a row
-  unsigned voff;
-  int chunk;
+  unsigned ld, kbytes;  // row stride, valid bytes of a row
+  unsigned bytes;       // from base to the end of the last valid row (at most 256 rows: below 2^31)
+  unsigned voff, chunk;
 
   __device__ __forceinline__ Panel(const void* m, long long ldb, int row0, int rows, int k0, int k, int tid) {
     base = static_cast<const char*>(m) + (long long)row0 * ldb + (long long)k0 * 2;
-    ld = (int)ldb;
+    ld = (unsigned)ldb;
     kbytes = k * 2;
-    bytes = (long long)(min(rows - row0, TILE) - 1) * ldb + kbytes;
+    bytes = (min(rows - row0, TILE) - 1) * ld + kbytes;
     const int r = tid >> 3;
     chunk = ((tid & 7) ^ ((r >> 1) & 7)) * 16;
     voff = r * ld + chunk;
   }
-  __device__ __forceinline__ void stage(int t, int h, char* dst, int tid) const {
-    const unsigned v = t * (KT * 2) + chunk < kbytes ? voff : FAR;  // past the row's end: zeros
+  // the two copies of a thread for half-tile h of step t, to LDS at dst (of this wave)
+  __device__ __forceinline__ void stage(int t, int h, unsigned dst) const {
+    const unsigned k = t * (KT * 2), v = k + chunk < kbytes ? voff : FAR;  // past the row's end: zeros
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const long long at = (long long)(h * 128 + i * 64) * ld + t * (KT * 2);
-      const long long left = max(0LL, bytes - at);
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + at), 0, (int)left, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (__attribute__((address_space(3))) void*)(dst + (i * THREADS + (tid & ~63)) * 16), 16, v, 0, 0, 0);
+      const unsigned at = (h * 128 + i * 64) * ld + k;
+      copy16(buffer_of(base + at, bytes > at ? bytes - at : 0), v, dst + i * THREADS * 16);
     }
   }
   // the 16 rows at r0 of a half-tile, K chunk kk of 32
@@ -165,7 +179,6 @@ struct Panel<true> {
     const int r = r0 + (lane & 15), c = kk * 4 + (lane >> 4);
     return *reinterpret_cast<const u32x4*>(img + r * 128 + ((c ^ ((r >> 1) & 7)) * 16));
   }
-  static constexpr int READS = 1;  // LDS instructions per fragment
 };
 
 // K down the rows: LDS image [64 k][8 units of 32 bytes], unit u of row k at u ^ f(k), f(k) =
@@ -175,29 +188,26 @@ struct Panel<true> {
 template <>
 struct Panel<false> {
   const char* base;
-  long long krows;
-  int ld, width;
+  int krows;
+  unsigned ld, width;  // row stride, valid bytes of a row from base on
   unsigned voff;
 
   __device__ __forceinline__ Panel(const void* m, long long ldb, int col0, int cols, int k0, int k, int tid) {
     base = static_cast<const char*>(m) + (long long)k0 * ldb + (long long)col0 * 2;
-    ld = (int)ldb;
+    ld = (unsigned)ldb;
     krows = k;
     width = (cols - col0) * 2;
     const int r = tid >> 4, c = tid & 15;
     const int f = (r & 3) | ((r >> 1) & 4);
     voff = r * ld + ((((c >> 1) ^ f) << 1) | (c & 1)) * 16;
   }
-  __device__ __forceinline__ void stage(int t, int h, char* dst, int tid) const {
+  __device__ __forceinline__ void stage(int t, int h, unsigned dst) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const long long rows = min(krows - t * KT - i * 32, 64LL);
-      const long long left = max(0LL, (rows - 1) * ld + width - h * 256);
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<char*>(base + (long long)(t * KT + i * 32) * ld + h * 256), 0, rows > 0 ? (int)left : 0,
-          0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (__attribute__((address_space(3))) void*)(dst + (i * THREADS + (tid & ~63)) * 16), 16, voff, 0, 0, 0);
+      const int k = t * KT + i * 32, rows = min(krows - k, 32);
+      const unsigned end = rows > 0 ? (rows - 1) * ld + width : 0;  // 32 rows of at most 2^25 bytes
+      copy16(buffer_of(base + (unsigned long long)(unsigned)k * ld + h * 256, end > h * 256u ? end - h * 256u : 0), voff,
+             dst + i * THREADS * 16);
     }
   }
   __device__ __forceinline__ static u32x4 frag(const char* img, int c0, int kk, int lane) {
@@ -209,7 +219,6 @@ struct Panel<false> {
     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * 256)));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
-  static constexpr int READS = 2;
 };
 
 typedef f32x4 Acc[2][2][4][2];  // [mh][nh][i][j]
@@ -235,10 +244,13 @@ __device__ __forceinline__ void product(Acc& acc, char* smem, const Panel<AA>& p
         for (int j = 0; j < 2; ++j) acc[mh][nh][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (nk <= 0) return;
 
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem +
+                        __builtin_amdgcn_readfirstlane(wid) * 64 * 16;
   auto slot = [&](int t, int h) { return smem + ((t & 1) * 4 + h) * HBYTES; };
   auto stage = [&](int t, int h) {  // h: 0 A0, 1 A1, 2 B0, 3 B1
-    if (h < 2) pa.stage(t, h, slot(t, h), tid);
-    else pb.stage(t, h - 2, slot(t, h), tid);
+    const unsigned dst = lds0 + ((t & 1) * 4 + h) * HBYTES;
+    if (h < 2) pa.stage(t, h, dst);
+    else pb.stage(t, h - 2, dst);
   };
   u32x4 a[4][2], b[2][2][2];
   auto read_a = [&](int t, int mh) {
