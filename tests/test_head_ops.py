@@ -90,7 +90,7 @@ def test_gemv_refuses_inputs():
     (1, 4, 64, 64, 32, 4, 4096, 4096), (1, 4, 64, 64, 68, 4, 4096, 4096), (1, 4, 64, 64, 64, 4, 4098, 4096),
     (1, 4, 64, 64, 64, 4, 4096, 4104), (1, 4, 64, 64, 64, 3, 4096, 4096)])
 def test_the_gemv_c_entry_checks_before_the_gpu(m, n, k, group, ldx, ldy, x, codes):
-    assert gemv._lib().tkv_gemv_w4(0, 0, x, ldx, codes, 4096, None, 4096, ldy, m, n, k, group, None) == -1
+    assert gemv._lib().tkv_gemv_w4(0, 0, x, ldx, codes, 4096, None, 4096, ldy, m, n, k, group, 1, None, None) == -1
     assert gemv._lib().tkv_last_error()
 
 
@@ -148,3 +148,13 @@ def test_screen_commands_without_a_gpu(argv, capsys, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
     assert cli.main(argv) == 2
     assert "tk-gpu: no GPU" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("m", [1, 2, 16, 17, 64])
+@pytest.mark.parametrize("n,k", [(1, 32), (100, 4096), (4096, 4128), (131072, 4096), (16, 1 << 20)])
+def test_gemv_splits_leave_no_part_empty(m, n, k):
+    parts = gemv.splits(m, n, k)
+    chunks = -(-k // 128)
+    per = -(-(-(-chunks // parts)) // 2) * 2  # as the launch divides them
+    assert 1 <= parts <= 64 and (parts - 1) * per < chunks <= parts * per
+    assert m > 1 or parts == 1

@@ -142,7 +142,7 @@ def targets() -> List[Target]:
         Target("libtk_loss.so", [loss],
                [hipcc, *HIP_FLAGS, *SCALAR_F32, "-fPIC", "-shared", loss, "-o", out("libtk_loss.so"), *RPATH]),
         Target("libtk_gemv.so", [gemv],
-               [hipcc, *HIP_FLAGS, *SCALAR_F32, "-fPIC", "-shared", gemv, "-o", out("libtk_gemv.so"), *RPATH]),
+               [hipcc, *HIP_FLAGS, *MFMA_FLAGS, *SCALAR_F32, "-fPIC", "-shared", gemv, "-o", out("libtk_gemv.so"), *RPATH]),
         Target("libtk_rccl.so", [rccl, *rccl_h],
                [hipcc, *HIP_FLAGS, "-fPIC", "-shared", rccl, "-o", out("libtk_rccl.so"), f"-L{ROCM}/lib",
                 "-lrccl", *RPATH]),

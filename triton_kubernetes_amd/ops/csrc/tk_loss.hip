@@ -119,9 +119,11 @@ __device__ __forceinline__ void tile_of(int b, int nwg, int tiles_m, int tiles_n
 }
 
 __device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");  // the barrier alone does not hold the compiler's LDS reads back
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
 }
 
 // 16 bytes a lane from a buffer (offset `voff`, zeros past its end) to LDS at `lds` + 16 lane.
