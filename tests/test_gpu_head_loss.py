@@ -51,11 +51,14 @@ SIZES = [(1, 8, 1), (1, 64, 300), (2, 72, 256), (5, 72, 257), (48, 512, 1000), (
          (300, 77, 1030), (64, 8, 70001), (513, 128, 513), (1, 4096, 2000)]
 
 
+@pytest.mark.parametrize("tiles", [0, 7], ids=["large", "small"])
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
 @pytest.mark.parametrize("n,d,v", SIZES)
-def test_cross_entropy(n, d, v, dt):
+def test_cross_entropy(n, d, v, dt, tiles, monkeypatch):
+    from triton_kubernetes_amd.ops import loss
     from triton_kubernetes_amd.ops.loss import linear_cross_entropy
 
+    monkeypatch.setattr(loss, "small_products", lambda *a: tiles)
     gen = _gen(n, d, v)
     x, w, t = _inputs(n, d, v, dt, gen)
     for reduction in ("none", "mean"):
@@ -66,9 +69,12 @@ def test_cross_entropy(n, d, v, dt):
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
 @pytest.mark.parametrize("n,d,v,k,temp", [(1, 64, 300, 1, 1.0), (7, 72, 257, 5, 2.0), (130, 264, 1111, 64, 0.7),
                                           (40, 77, 5003, 130, 2.0), (300, 512, 999, 33, 1.0)])
-def test_distill(n, d, v, k, temp, dt):
+@pytest.mark.parametrize("tiles", [0, 7], ids=["large", "small"])
+def test_distill(n, d, v, k, temp, dt, tiles, monkeypatch):
+    from triton_kubernetes_amd.ops import loss
     from triton_kubernetes_amd.ops.loss import linear_distill
 
+    monkeypatch.setattr(loss, "small_products", lambda *a: tiles)
     gen = _gen(n, d, v, k)
     x, w, _ = _inputs(n, d, v, dt, gen)
     ids = torch.randint(0, v, (n, k), device="cuda", generator=gen)  # the same id twice among them
@@ -225,8 +231,9 @@ def test_pieces_and_splits(monkeypatch):
     gen = _gen(13)
     x, w, t = _inputs(n, d, v, torch.float16, gen)
     call = lambda x, w: loss.linear_cross_entropy(x, w, t, reduction="none")  # noqa: E731
-    for parts in (1, 2, 7):
-        monkeypatch.setattr(loss, "splits", lambda *a, parts=parts: parts)
+    for groups, tiles in ((1, 0), (30, 7), (14, 0), (4096, 2), (4096, 5)):
+        monkeypatch.setattr(loss, "fill", lambda small, groups=groups: groups)
+        monkeypatch.setattr(loss, "small_products", lambda *a, tiles=tiles: tiles)
         _against(call, x, w, *ref.targets_of(t, -100, n, v), gen=gen)
 
 

@@ -1,8 +1,6 @@
 """The output head's operators without a GPU: what they refuse, the rules that size their
 workspaces, the C entries' own checks, and the 4-bit weight format."""
 
-import ctypes
-
 import pytest
 import torch
 
@@ -36,14 +34,27 @@ def test_pieces_cover_the_vocabulary_within_the_workspace(n, v):
     assert piece == loss.TILE or piece * n * 2 <= loss.DL_BYTES
     count = -(-v // piece)
     assert (count - 1) * piece < v  # no empty piece
-    for d in (8, 77, 4096, 65536):
-        parts = loss.splits(n, d, piece)
-        assert 1 <= parts <= 512 and (parts == 1 or parts * n * 4 * d <= loss.DX_BYTES)
+
+
+FIELDS = ("n", "d", "v", "k", "ldx", "ldw", "ldg", "ignore", "piece", "fill", "dev", "f16", "distill", "reduction",
+          "temperature", "want", "small", "x", "w", "ids", "teacher", "grad", "loss", "kept", "room", "wc", "dx", "dw",
+          "stream")
 
 
 def _args(**fields):
-    base = dict(n=4, d=8, v=16, k=1, ldx=8, ldw=8, reduction=2, temperature=1.0, piece=256, splits=1, w=4096)
-    return loss._Args(**{**base, **fields})
+    base = dict(n=4, d=8, v=16, k=1, ldx=8, ldw=8, reduction=2, temperature=1.0, piece=256, fill=256, w=4096)
+    return loss._ARGS.pack(*({**dict.fromkeys(FIELDS, 0), **base, **fields}[f] for f in FIELDS))
+
+
+@pytest.mark.parametrize("n,d,k", [(1, 1, 1), (7, 72, 1), (333, 1288, 100), (8192, 4096, 64)])
+def test_buffers_have_the_sizes_that_the_kernels_take(n, d, k):
+    lib = loss._lib()
+    for distill in (0, 1):
+        assert lib.tkl_kept_bytes(_args(n=n, d=d, k=k, distill=distill)) == loss.kept_bytes(n, d, n * k * distill)
+        for want, groups, small, piece in ((3, 256, 0, 512), (1, 512, 2, 4096), (2, 256, 0, 256), (1, 1, 0, 32768),
+                                           (3, 4096, 7, 256)):
+            args = _args(n=n, d=d, k=k, want=want, piece=piece, fill=groups, small=small, distill=distill)
+            assert lib.tkl_room_bytes(args) == loss.room_bytes(n, d, piece, groups, bool(small & 2), want, distill)
 
 
 @pytest.mark.parametrize("fields,message", [
@@ -56,13 +67,13 @@ def _args(**fields):
 def test_the_c_entries_check_before_the_gpu(fields, message):
     lib = loss._lib()
     for call in (lib.tkl_forward, lib.tkl_backward):
-        assert call(ctypes.byref(_args(**fields))) == -1
+        assert call(_args(**fields)) == -1
         assert message in lib.tkl_last_error().decode()
 
 
-@pytest.mark.parametrize("fields", [dict(piece=0), dict(piece=255), dict(piece=1 << 25), dict(splits=0), dict(splits=1025)])
+@pytest.mark.parametrize("fields", [dict(piece=0), dict(piece=255), dict(piece=1 << 25), dict(fill=0), dict(fill=4097)])
 def test_the_c_backward_checks_its_pieces(fields):
-    assert loss._lib().tkl_backward(ctypes.byref(_args(**fields))) == -1
+    assert loss._lib().tkl_backward(_args(**fields)) == -1
 
 
 def test_gemv_refuses_inputs():
@@ -158,3 +169,9 @@ def test_gemv_splits_leave_no_part_empty(m, n, k):
     per = -(-(-(-chunks // parts)) // 2) * 2  # as the launch divides them
     assert 1 <= parts <= 64 and (parts - 1) * per < chunks <= parts * per
     assert m > 1 or parts == 1
+
+
+def test_tile_rules_at_their_corners():
+    assert loss.small_products(1, 512, 1000) == 7 and loss.small_products(1024, 512, 1000) == 7
+    assert loss.small_products(64, 4096, 131072) == 3 and loss.small_products(65, 4096, 131072) == 0
+    assert loss.small_products(8192, 4096, 131072) == 0

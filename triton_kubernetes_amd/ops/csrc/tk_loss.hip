@@ -10,13 +10,20 @@
 //
 // Cross entropy is K = 1, p = 1, T = 1; distillation takes p from a teacher's top logits.
 //
-// Forward: one matrix product whose epilogue reduces every tile of 256 vocabulary entries to
-// a running maximum and sum per token (k_logits<LSE>), a dot product per target (k_dots), and
-// a join over the tiles (k_loss).
+// Forward: one matrix product whose epilogue reduces every tile of the vocabulary to a maximum
+// and a sum per token (k_logits<LSE>), a dot product per target, and a join over the tiles
+// (k_loss, which also forms a cross entropy's dot products; k_dots those of a teacher's lists).
 // Backward, in pieces of the vocabulary: the logits of the piece are computed again, and the
-// epilogue turns them into their 16-bit derivative dl (k_logits<DL>; the sparse targets are
+// epilogue turns them into their 16-bit derivative dl (k_logits<DL>; a teacher's targets are
 // put in by k_fix); then dX += dl W and dW = dl^T X, two matrix products that read dl while
 // the last-level cache still holds it.
+//
+// dl is rounded to 16 bits, which costs each product about as much as the rounding of its result.
+// Most of a row's derivative is at its target, though, and few numbers' roundings do not average
+// out: up to FEW_ROWS packed rows, what the largest ones lose (`lost`, RESIDUALS a row) is added
+// to dX and dW in fp32.  (48 tokens, bf16: error 1.0 instead of 1.25 times that of rounding the
+// exact gradients; one token alone can have twice as much.  For 4096 tokens it would be 1.0
+// instead of 1.18 times, and cost k_dw a tenth.)
 //
 // Rows without a target (masked tokens) are left out before any product: k_gather packs the
 // others into Xc, so that whatever the masked rows hold (infinities, NaN) reaches nothing and
@@ -49,32 +56,50 @@ static int set_err(const char* what, hipError_t e) {
   return (int)e == 0 ? -1 : (int)e;
 }
 
-// One call's tensors and sizes (ops/loss.py:_Args holds the same fields in the same order).
+// One call's tensors and sizes (ops/loss.py packs the same fields in the same order).
 struct tkl_args {
   long long n, d, v, k;        // tokens, width, vocabulary, targets per token
   long long ldx, ldw, ldg;     // row strides of x and w, stride of the upstream gradient (elements)
   long long ignore;            // cross entropy: the target that means "no loss"
-  long long piece, splits;     // backward: vocabulary entries per piece, splits of the dX product
+  long long piece, fill;       // backward: vocabulary entries per piece, workgroups that fill the chip with dX
   int dev, f16, distill, reduction;  // reduction 0 none, 1 sum, 2 mean
   float temperature;
   int want;                    // backward: 1 dX, 2 dW, 3 both
+  int small;                   // products in small tiles: 1 the logits, 2 dX, 4 dW
   const void *x, *w, *ids, *teacher, *grad;
-  void *loss, *xc, *lse, *zk, *p, *rowloss, *rowmap, *posof, *count;  // kept from forward to backward
-  void *flag;                  // distillation: whether a row has a target
-  void *part;                  // forward: tile maxima and sums
+  void *loss, *kept;           // kept: from forward to backward (struct Kept)
+  void *room;                  // forward: the tiles' maxima and sums; backward: dl, sums of dX, factors
   void *wc;                    // a padded copy of w, where w's rows are not 16-byte aligned
-  void *dl, *dxpart, *factor;  // backward workspaces
   void *dx, *dw;
   void* stream;
 };
 
 namespace {
 
-constexpr int THREADS = 512;  // of the matrix products: 8 waves, one 256x256 tile
-constexpr int TILE = 256;
 constexpr int KT = 64;  // K elements of a step (128 bytes of a row)
-constexpr int HBYTES = 128 * KT * 2;
-constexpr int LDS = 8 * HBYTES;
+constexpr int MAX_TARGETS = 1024;
+constexpr int RESIDUALS = 4;  // entries of a teacher's list whose rounding is made good; 1 of a cross entropy
+constexpr float LARGE = 0.125f;  // |q - p| from which it is: at most 16 of a row
+constexpr int FEW_ROWS = 512;
+
+// The two tilings of the matrix products.  A fragment is 16 x 16; a lane of a wave holds rows
+// row(mf) + (lane / 16) * 4 + 0..3 and column col(nf) + lane % 16 of fragment (mf, nf).
+struct Big {  // 8 waves, the schedule of product<Big>
+  static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2, LDS = 8 * 128 * KT * 2;
+  static __device__ __forceinline__ int wave_m(int wid) { return wid >> 2; }
+  static __device__ __forceinline__ int row(int mf, int wid) { return (mf >> 2) * 128 + (wid >> 2) * 64 + (mf & 3) * 16; }
+  static __device__ __forceinline__ int col(int nf, int wid) { return (nf >> 1) * 128 + (wid & 3) * 32 + (nf & 1) * 16; }
+  static __device__ __forceinline__ bool owns(int col, int wid) { return (col >> 5 & 3) == (wid & 3); }
+};
+struct Small {  // 4 waves, three steps in LDS: for few tokens, two workgroups to a compute unit
+  static constexpr int BM = 128, BN = 64, THREADS = 256, MF = 2, NF = 4, WAVES_M = 4, STEPS = 3,
+                       LDS = STEPS * (BM + BN) * KT * 2;
+  static __device__ __forceinline__ int wave_m(int wid) { return wid; }
+  static __device__ __forceinline__ int row(int mf, int wid) { return wid * 32 + mf * 16; }
+  static __device__ __forceinline__ int col(int nf, int) { return nf * 16; }
+  static __device__ __forceinline__ bool owns(int, int) { return true; }
+};
+
 constexpr unsigned FAR = 0x40000000u;  // an offset past every descriptor's end: the copy writes zeros
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -104,11 +129,15 @@ __device__ __forceinline__ unsigned pack2(float lo, float hi) {
   return __builtin_bit_cast(unsigned, v);
 }
 
-// Block -> tile, XCD-aware: workgroups go round-robin over the 8 XCDs, so XCD x takes the
-// x-th run of tiles and the tiles of a run share panels in that XCD's L2.
-__device__ __forceinline__ void tile_of(int b, int nwg, int tiles_m, int tiles_n, int* tm, int* tn) {
+// Block -> place in the order of the work, XCD-aware: workgroups go round-robin over the 8 XCDs,
+// so XCD x takes the x-th run of the order, and what lies together in it shares panels in that
+// XCD's L2.
+__device__ __forceinline__ int run_of(int b, int nwg) {
   const int xcd = b & 7, q = nwg >> 3, rem = nwg & 7;
-  const int w = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + (b >> 3);
+  return (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + (b >> 3);
+}
+// Place -> tile: 8 rows of tiles at a time, down the columns.
+__device__ __forceinline__ void tile_of(int w, int tiles_m, int tiles_n, int* tm, int* tn) {
   constexpr int GROUP_M = 8;
   const int per_group = GROUP_M * tiles_n;
   const int g = w / per_group, first_m = g * GROUP_M;
@@ -126,14 +155,19 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
-// 16 bytes a lane from a buffer (offset `voff`, zeros past its end) to LDS at `lds` + 16 lane.
+// 16 bytes a lane from two buffers (offset `voff`, zeros past their ends) to LDS at `lds` and
+// `lds2` + 16 lane.
 // In asm, because the compiler would wait for every copy in flight before each
 // ds_read_b64_tr_b16 (2.25 instead of 1.83 ms for k_dx and k_dw at 8192 x 4096 x 32768); product() does the
-// waiting.  The copy has no register output; it reads its operands when it is issued.
-__device__ __forceinline__ void copy16(u32x4 buffer, unsigned voff, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff),
-               "s"(buffer)
-               : "memory", "m0");
+// waiting.  A copy has no register output; it reads its operands when it is issued.
+// (5 wait states before it: they would be needed had a vector instruction written the
+// descriptor, which the compiler does not see to for asm; 1 between m0 and its use.)
+__device__ __forceinline__ void copy16_twice(u32x4 one, u32x4 two, unsigned voff, unsigned lds, unsigned lds2) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds" ::"s"(lds),
+      "s"(lds2), "v"(voff), "s"(one), "s"(two)
+      : "memory", "m0");
 }
 __device__ __forceinline__ u32x4 buffer_of(const char* base, unsigned bytes) {
   const unsigned long long b = reinterpret_cast<unsigned long long>(base);
@@ -143,16 +177,17 @@ __device__ __forceinline__ u32x4 buffer_of(const char* base, unsigned bytes) {
   return u32x4{lo, hi & 0xffffu, (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
 
-// One 256-wide panel of an operand.  ALONG: a row of the panel lies along K (128 rows of 128
-// bytes are a half-tile); else K is the matrix's row index (64 rows of 128 columns), and the
-// fragments are transposed on their way out of LDS.
-template <bool ALONG>
+// A panel of an operand, staged in images of ROWS rows by THREADS threads.  ALONG: a row of the
+// panel lies along K (an image is ROWS rows of 128 bytes); else K is the matrix's row index (64
+// rows of ROWS columns), and the fragments are transposed on their way out of LDS.
+template <bool ALONG, int ROWS, int THREADS>
 struct Panel;
 
-// Rows along K: LDS image [128 rows][8 chunks of 16 bytes], chunk c of row r at c ^ (r/2 & 7)
-// (the 16 rows of a fragment read land in 16 bank slots).
-template <>
-struct Panel<true> {
+// Rows along K: LDS image [ROWS][8 chunks of 16 bytes], chunk c of row r at c ^ (r/2 & 7) (the
+// 16 rows of a fragment read land in 16 bank slots).
+template <int ROWS, int THREADS>
+struct Panel<true, ROWS, THREADS> {
+  static constexpr int COPIES = ROWS * 8 / THREADS;
   const char* base;
   unsigned ld, kbytes;  // row stride, valid bytes of a row
   unsigned bytes;       // from base to the end of the last valid row (at most 256 rows: below 2^31)
@@ -162,92 +197,147 @@ struct Panel<true> {
     base = static_cast<const char*>(m) + (long long)row0 * ldb + (long long)k0 * 2;
     ld = (unsigned)ldb;
     kbytes = k * 2;
-    bytes = (min(rows - row0, TILE) - 1) * ld + kbytes;
+    bytes = (min(rows - row0, 256) - 1) * ld + kbytes;
     const int r = tid >> 3;
     chunk = ((tid & 7) ^ ((r >> 1) & 7)) * 16;
     voff = r * ld + chunk;
   }
-  // the two copies of a thread for half-tile h of step t, to LDS at dst (of this wave)
+  // this thread's copies of step t, rows h * ROWS on, to LDS at dst (of this wave)
   __device__ __forceinline__ void stage(int t, int h, unsigned dst) const {
     const unsigned k = t * (KT * 2), v = k + chunk < kbytes ? voff : FAR;  // past the row's end: zeros
+    auto buffer = [&](int i) {
+      const unsigned at = (h * ROWS + i * (THREADS / 8)) * ld + k;
+      return buffer_of(base + at, max((int)bytes - (int)at, 0));
+    };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const unsigned at = (h * 128 + i * 64) * ld + k;
-      copy16(buffer_of(base + at, bytes > at ? bytes - at : 0), v, dst + i * THREADS * 16);
-    }
+    for (int i = 0; i < COPIES; i += 2)
+      copy16_twice(buffer(i), buffer(i + 1), v, dst + i * THREADS * 16, dst + (i + 1) * THREADS * 16);
   }
-  // the 16 rows at r0 of a half-tile, K chunk kk of 32
+  // the 16 rows at r0 of an image, K chunk kk of 32
   __device__ __forceinline__ static u32x4 frag(const char* img, int r0, int kk, int lane) {
     const int r = r0 + (lane & 15), c = kk * 4 + (lane >> 4);
     return *reinterpret_cast<const u32x4*>(img + r * 128 + ((c ^ ((r >> 1) & 7)) * 16));
   }
 };
 
-// K down the rows: LDS image [64 k][8 units of 32 bytes], unit u of row k at u ^ f(k), f(k) =
-// (k & 3) | (k >> 3 & 1) << 2: the 8 rows that half a wave reads at once land on different
-// banks.  ds_read_b64_tr_b16 gives lane c of a 16-lane group the 4 values of column c from the
-// 4 rows that the group reads.
-template <>
-struct Panel<false> {
+// K down the rows: LDS image [64 k][ROWS / 16 units of 32 bytes], unit u of row k at u ^ f(k).
+// Half a wave reads rows 0-3 and 8-11 (mod 16) at once; f spreads them over the banks: with 256
+// bytes a row all 8 differ, with 128 bytes those of equal parity do.  ds_read_b64_tr_b16 gives
+// lane c of a 16-lane group the 4 values of column c from the 4 rows that the group reads.
+template <int ROWS, int THREADS>
+struct Panel<false, ROWS, THREADS> {
+  static constexpr int COPIES = ROWS * 8 / THREADS, STRIDE = ROWS * 2, PER = ROWS / 8, KROWS = THREADS / PER;
   const char* base;
   int krows;
   unsigned ld, width;  // row stride, valid bytes of a row from base on
   unsigned voff;
 
+  static __device__ __forceinline__ int f(int k) {
+    return ROWS == 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+  }
   __device__ __forceinline__ Panel(const void* m, long long ldb, int col0, int cols, int k0, int k, int tid) {
     base = static_cast<const char*>(m) + (long long)k0 * ldb + (long long)col0 * 2;
     ld = (unsigned)ldb;
     krows = k;
     width = (cols - col0) * 2;
-    const int r = tid >> 4, c = tid & 15;
-    const int f = (r & 3) | ((r >> 1) & 4);
-    voff = r * ld + ((((c >> 1) ^ f) << 1) | (c & 1)) * 16;
+    const int r = tid / PER, c = tid % PER;
+    voff = r * ld + ((((c >> 1) ^ f(r)) << 1) | (c & 1)) * 16;
   }
   __device__ __forceinline__ void stage(int t, int h, unsigned dst) const {
+    auto buffer = [&](int i) {
+      const int k = t * KT + i * KROWS, rows = min(krows - k, KROWS);
+      const int end = rows > 0 ? (rows - 1) * (int)ld + (int)width - h * STRIDE : 0;  // at most 32 rows of 2^25 bytes
+      return buffer_of(base + (unsigned long long)(unsigned)k * ld + h * STRIDE, max(end, 0));
+    };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = t * KT + i * 32, rows = min(krows - k, 32);
-      const unsigned end = rows > 0 ? (rows - 1) * ld + width : 0;  // 32 rows of at most 2^25 bytes
-      copy16(buffer_of(base + (unsigned long long)(unsigned)k * ld + h * 256, end > h * 256u ? end - h * 256u : 0), voff,
-             dst + i * THREADS * 16);
-    }
+    for (int i = 0; i < COPIES; i += 2)
+      copy16_twice(buffer(i), buffer(i + 1), voff, dst + i * THREADS * 16, dst + (i + 1) * THREADS * 16);
   }
   __device__ __forceinline__ static u32x4 frag(const char* img, int c0, int kk, int lane) {
-    const int q = lane >> 4, l = lane & 15;
-    const int f = (l >> 2) | ((q & 1) << 2);
-    const char* p = img + (kk * 32 + q * 8 + (l >> 2)) * 256 + (((c0 >> 4) ^ f) * 32) + (l & 3) * 8;
+    const int q = lane >> 4, l = lane & 15, k = kk * 32 + q * 8 + (l >> 2);
+    const char* p = img + k * STRIDE + (((c0 >> 4) ^ f(q * 8 + (l >> 2))) * 32) + (l & 3) * 8;
     typedef __attribute__((address_space(3))) s16x4 lds4;
     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p));
-    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * 256)));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * STRIDE)));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
 };
 
-typedef f32x4 Acc[2][2][4][2];  // [mh][nh][i][j]
+__device__ __forceinline__ unsigned lds_of(const char* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
 
-// One 256x256 tile of A B^T over nk steps of 64.  Element (mh, nh, i, j, e) of a lane is
-// row mh*128 + wr*64 + i*16 + (lane/16)*4 + e and column nh*128 + wc*32 + j*16 + lane%16.
-//
+template <class Tile, bool ALONG>
+using PanelA = Panel<ALONG, 128, Tile::THREADS>;
+template <class Tile, bool ALONG>
+using PanelB = Panel<ALONG, Tile::BN == 256 ? 128 : Tile::BN, Tile::THREADS>;
+
+// acc = one tile of A B^T over nk steps of 64.
+template <class Tile>
+using Acc = f32x4[Tile::MF][Tile::NF];
+
+template <class Tile>
+__device__ __forceinline__ void clear(Acc<Tile>& acc) {
+#pragma unroll
+  for (int i = 0; i < Tile::MF; ++i)
+#pragma unroll
+    for (int j = 0; j < Tile::NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
+// Three steps in LDS, one barrier a step: while a step is multiplied the next two are on their
+// way.
+template <bool F16, bool AA, bool BA>
+__device__ __forceinline__ void product(Acc<Small>& acc, char* smem, const PanelA<Small, AA>& pa,
+                                        const PanelB<Small, BA>& pb, int nk, int tid) {
+  clear<Small>(acc);
+  if (nk <= 0) return;
+  constexpr int BYTES = (Small::BM + Small::BN) * KT * 2, AB = Small::BM * KT * 2;
+  constexpr int COPIES = PanelA<Small, AA>::COPIES + PanelB<Small, BA>::COPIES;
+  const int lane = tid & 63, wid = tid >> 6;
+  const unsigned lds0 = lds_of(smem) + __builtin_amdgcn_readfirstlane(wid) * 64 * 16;
+  auto stage = [&](int t) {
+    const unsigned dst = lds0 + t % Small::STEPS * BYTES;
+    pa.stage(t, 0, dst);
+    pb.stage(t, 0, dst + AB);
+  };
+  stage(0);
+  if (nk > 1) stage(1);
+  for (int t = 0; t < nk; ++t) {
+    if (t + 1 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(COPIES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    barrier();  // step t is there for every wave, and step t - 1 has been read
+    if (t + 2 < nk) stage(t + 2);
+    const char *ia = smem + t % Small::STEPS * BYTES, *ib = ia + AB;
+    u32x4 a[Small::MF][2], b[Small::NF][2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+      for (int i = 0; i < Small::MF; ++i) a[i][kk] = PanelA<Small, AA>::frag(ia, Small::row(i, wid), kk, lane);
+#pragma unroll
+      for (int j = 0; j < Small::NF; ++j) b[j][kk] = PanelB<Small, BA>::frag(ib, Small::col(j, wid), kk, lane);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < Small::MF; ++i)
+#pragma unroll
+        for (int j = 0; j < Small::NF; ++j) acc[i][j] = Type<F16>::mfma(a[i][kk], b[j][kk], acc[i][j]);
+  }
+}
+
 // The schedule is the one of tk_gemm_screen.hip's k_gemm8: LDS holds half-tiles of two steps,
 // a step is two phases of 32 matrix instructions per wave, and the wave groups wr = 0 and 1
 // run one barrier apart, so that on every SIMD one wave feeds the matrix pipe while the other
 // reads LDS and issues copies.
 template <bool F16, bool AA, bool BA>
-__device__ __forceinline__ void product(Acc& acc, char* smem, const Panel<AA>& pa, const Panel<BA>& pb, int nk,
-                                        int tid) {
+__device__ __forceinline__ void product(Acc<Big>& acc, char* smem, const PanelA<Big, AA>& pa,
+                                        const PanelB<Big, BA>& pb, int nk, int tid) {
+  constexpr int HBYTES = 128 * KT * 2;
   const int lane = tid & 63, wid = tid >> 6, wr = wid >> 2, wc = wid & 3;
-#pragma unroll
-  for (int mh = 0; mh < 2; ++mh)
-#pragma unroll
-    for (int nh = 0; nh < 2; ++nh)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[mh][nh][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  clear<Big>(acc);
   if (nk <= 0) return;
 
-  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem +
-                        __builtin_amdgcn_readfirstlane(wid) * 64 * 16;
+  const unsigned lds0 = lds_of(smem) + __builtin_amdgcn_readfirstlane(wid) * 64 * 16;
   auto slot = [&](int t, int h) { return smem + ((t & 1) * 4 + h) * HBYTES; };
   auto stage = [&](int t, int h) {  // h: 0 A0, 1 A1, 2 B0, 3 B1
     const unsigned dst = lds0 + ((t & 1) * 4 + h) * HBYTES;
@@ -259,13 +349,13 @@ __device__ __forceinline__ void product(Acc& acc, char* smem, const Panel<AA>& p
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) a[i][kk] = Panel<AA>::frag(slot(t, mh), wr * 64 + i * 16, kk, lane);
+      for (int kk = 0; kk < 2; ++kk) a[i][kk] = PanelA<Big, AA>::frag(slot(t, mh), wr * 64 + i * 16, kk, lane);
   };
   auto read_b = [&](int t, int nh) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) b[nh][j][kk] = Panel<BA>::frag(slot(t, 2 + nh), wc * 32 + j * 16, kk, lane);
+      for (int kk = 0; kk < 2; ++kk) b[nh][j][kk] = PanelB<Big, BA>::frag(slot(t, 2 + nh), wc * 32 + j * 16, kk, lane);
   };
   auto quad = [&](int mh, int nh) {
     __builtin_amdgcn_s_setprio(1);
@@ -275,7 +365,7 @@ __device__ __forceinline__ void product(Acc& acc, char* smem, const Panel<AA>& p
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
-          acc[mh][nh][i][j] = Type<F16>::mfma(a[i][kk], b[nh][j][kk], acc[mh][nh][i][j]);
+          acc[mh * 4 + i][nh * 2 + j] = Type<F16>::mfma(a[i][kk], b[nh][j][kk], acc[mh * 4 + i][nh * 2 + j]);
     __builtin_amdgcn_s_setprio(0);
   };
   // keep every matrix instruction between its phase's two barriers
@@ -295,7 +385,7 @@ __device__ __forceinline__ void product(Acc& acc, char* smem, const Panel<AA>& p
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) asm volatile("" : "+v"(acc[mh][nh][i][j]));
+        for (int j = 0; j < 2; ++j) asm volatile("" : "+v"(acc[mh * 4 + i][nh * 2 + j]));
   };
 
   stage(0, 0);
@@ -350,17 +440,6 @@ __device__ __forceinline__ void product(Acc& acc, char* smem, const Panel<AA>& p
   if (wr == 0) barrier();  // the other group's extra barrier
 }
 
-struct Lane {
-  int lane, wr, wc, fr, fq;
-  __device__ __forceinline__ Lane(int tid) {
-    lane = tid & 63;
-    wr = tid >> 8;
-    wc = (tid >> 6) & 3;
-    fr = lane & 15;
-    fq = lane >> 4;
-  }
-};
-
 // (m, s) of a softmax: maximum and sum of exp2(. - m).  An empty side has m = -inf, s = 0.
 __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
@@ -369,165 +448,285 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-// z^T of 256 vocabulary entries (A = W) by 256 tokens (B = Xc), so that a lane holds 32
-// entries of each of 4 tokens and the softmax's sums need two shuffles a token.
-// LSE: writes part[2 * tile + wr][token] = (max, sum).  DL: writes f (q - 0) in 16 bits.
-// sc = log2(e) / T.
-template <bool F16, bool DL>
-__global__ __launch_bounds__(THREADS) void k_logits(const void* __restrict__ w, long long ldw,
-                                                    const void* __restrict__ xc, long long ldxc, int v0, int vend,
-                                                    int d, const int* __restrict__ count, int n, float sc,
-                                                    float2* __restrict__ part, const float* __restrict__ lse,
-                                                    const float* __restrict__ factor, void* __restrict__ dl,
-                                                    long long lddl) {
+// What the derivative dl = factor (q - p) of a packed row's logits is multiplied with, and the
+// scale that the products are multiplied with afterwards, in 32 bits.  For the sum and the mean
+// factor is the upstream gradient's sign times `span`; without a reduction it is the row's
+// upstream gradient itself, or for fp16 span * that / the largest one's magnitude, from k_factor.
+// span is 1 for bf16, which has fp32's exponents, and 2^15 for fp16: |q - p| <= 1 stays below
+// its largest value 65504, and a probability keeps its 11 bits down to 2^-29 instead of 2^-14.
+// A row whose loss is NaN gets NaN gradients.
+template <bool F16>
+struct Upstream {
+  const float *grad, *rowloss, *factor;  // factor[n] is the scale that goes with them
+  const int *rowmap, *count;
+  long long ldg;
+  int reduction, n;
+  float t;
+  static constexpr float SPAN = F16 ? 32768.f : 1.f;
+
+  __device__ __forceinline__ float of(int pos) const {
+    const float l = rowloss[pos];
+    if (l != l) return NAN;
+    if (reduction == 0) return F16 ? factor[pos] : grad[rowmap[pos] * ldg];
+    const float g = grad[0];
+    return g > 0.f ? SPAN : g < 0.f ? -SPAN : g;
+  }
+  __device__ __forceinline__ float scale() const {
+    if (reduction == 0) return F16 ? factor[n] : t;
+    return fabsf(grad[0]) * t / SPAN / (reduction == 2 ? (float)max(count[0], 1) : 1.f);
+  }
+};
+
+// z^T of Tile::BM vocabulary entries (A = W) by Tile::BN tokens (B = Xc), so that a lane holds
+// many entries of few tokens and the softmax's sums need two shuffles a token.
+// LSE: writes part[tile][token] = (max, sum).  DL: writes f (q - p) in 16 bits, with a cross
+// entropy's p; `targets` is null for a teacher's lists.  sc = log2(e) / T.
+template <class Tile, bool F16, bool DL>
+__global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict__ w, long long ldw,
+                                                          const void* __restrict__ xc, long long ldxc, int v0,
+                                                          int vend, int d, const int* __restrict__ count, int n,
+                                                          float sc, float2* __restrict__ part,
+                                                          const float* __restrict__ lse, Upstream<F16> up,
+                                                          const int* __restrict__ targets, void* __restrict__ dl,
+                                                          long long lddl, float* __restrict__ lost) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
   const int rows = count[0];
-  const int tiles_v = (vend - v0 + TILE - 1) / TILE, tiles_n = (rows + TILE - 1) / TILE;
+  const int tiles_v = (vend - v0 + Tile::BM - 1) / Tile::BM, tiles_n = (rows + Tile::BN - 1) / Tile::BN;
   const int nwg = tiles_v * tiles_n;
   if ((int)blockIdx.x >= nwg) return;
   int tv, tn;
-  tile_of(blockIdx.x, nwg, tiles_v, tiles_n, &tv, &tn);
-  const int tid = threadIdx.x;
-  const Panel<true> pa(w, ldw, v0 + tv * TILE, vend, 0, d, tid), pb(xc, ldxc, tn * TILE, rows, 0, d, tid);
-  Acc acc;
+  tile_of(run_of(blockIdx.x, nwg), tiles_v, tiles_n, &tv, &tn);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, fr = lane & 15, fq = lane >> 4;
+  const PanelA<Tile, true> pa(w, ldw, v0 + tv * Tile::BM, vend, 0, d, tid);
+  const PanelB<Tile, true> pb(xc, ldxc, tn * Tile::BN, rows, 0, d, tid);
+  Acc<Tile> acc;
   product<F16, true, true>(acc, smem, pa, pb, (d + KT - 1) / KT, tid);
 
-  const Lane l(tid);
-  const int vb = tv * TILE + l.wr * 64 + l.fq * 4;  // the lane's first entry, in the piece
+  const int vb = tv * Tile::BM + fq * 4;  // the lane's entries are vb + row(i) + 0..3, in the piece
   const int vn = vend - v0;
-  const bool whole = (tv + 1) * TILE <= vn;
+  const bool whole = (tv + 1) * Tile::BM <= vn;
+  if constexpr (!DL) {
+    barrier();  // LDS has been read
+    float2* sums = reinterpret_cast<float2*>(smem);  // [WAVES_M][BN]
 #pragma unroll
-  for (int nh = 0; nh < 2; ++nh)
+    for (int j = 0; j < Tile::NF; ++j) {
+      float m = -INFINITY, s = 0.f;
+      if (!whole) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int token = tn * TILE + nh * 128 + l.wc * 32 + j * 16 + l.fr;
-      if constexpr (!DL) {
-        float m = -INFINITY, s = 0.f;
+        for (int i = 0; i < Tile::MF; ++i)
 #pragma unroll
-        for (int mh = 0; mh < 2; ++mh)
+          for (int e = 0; e < 4; ++e)
+            if (vb + Tile::row(i, wid) + e >= vn) acc[i][j][e] = -INFINITY;
+      }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < Tile::MF; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float z = acc[mh][nh][i][j][e] * sc;
-              if (!whole && vb + mh * 128 + i * 16 + e >= vn) z = -INFINITY;
-              acc[mh][nh][i][j][e] = z;
-              m = fmaxf(m, z);
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
+      m *= sc;
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < Tile::MF; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], sc, -base));
+      merge(m, s, __shfl_xor(m, 16, 64), __shfl_xor(s, 16, 64));
+      merge(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
+      if (fq == 0) sums[Tile::wave_m(wid) * Tile::BN + Tile::col(j, wid) + fr] = float2{m, s};
+    }
+    __syncthreads();
+    const int token = tn * Tile::BN + tid;
+    if (tid < Tile::BN && token < rows) {
+      float2 c = sums[tid];
+#pragma unroll
+      for (int o = 1; o < Tile::WAVES_M; ++o) merge(c.x, c.y, sums[o * Tile::BN + tid].x, sums[o * Tile::BN + tid].y);
+      part[(size_t)tv * n + token] = c;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < Tile::NF; ++j) {
+      const int token = tn * Tile::BN + Tile::col(j, wid) + fr;
+      if (token >= rows) continue;
+      const float f = up.of(token), ls = lse[token];
+      const int target = targets ? targets[token] - v0 - vb : -1;
+      T* out = static_cast<T*>(dl) + (size_t)token * lddl + vb;
+#pragma unroll
+      for (int i = 0; i < Tile::MF; ++i) {
+        const int at = Tile::row(i, wid);
+        float g[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = f * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], sc, -ls));
+        if ((unsigned)(target - at) < 4u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (at + e == target) {
+              g[e] -= f;
+              lost[token] = g[e] - (float)(T)g[e];
             }
-        const float base = m == -INFINITY ? 0.f : m;
+        }
+        if (!whole) {
 #pragma unroll
-        for (int mh = 0; mh < 2; ++mh)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(acc[mh][nh][i][j][e] - base);
-        merge(m, s, __shfl_xor(m, 16, 64), __shfl_xor(s, 16, 64));
-        merge(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
-        if (l.fq == 0 && token < rows) part[(size_t)(2 * tv + l.wr) * n + token] = float2{m, s};
-      } else {
-        if (token >= rows) continue;
-        const float f = factor[token], ls = lse[token];
-        T* out = static_cast<T*>(dl) + (size_t)token * lddl + vb;
-#pragma unroll
-        for (int mh = 0; mh < 2; ++mh)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float g[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float q = __builtin_amdgcn_exp2f(acc[mh][nh][i][j][e] * sc - ls);
-              g[e] = whole || vb + mh * 128 + i * 16 + e < vn ? f * q : 0.f;  // zeros pad the piece
-            }
-            *reinterpret_cast<u32x2*>(out + mh * 128 + i * 16) = u32x2{pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3])};
-          }
+          for (int e = 0; e < 4; ++e)
+            if (vb + at + e >= vn) g[e] = 0.f;  // zeros pad the piece
+        }
+        *reinterpret_cast<u32x2*>(out + Tile::row(i, wid)) = u32x2{pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3])};
       }
     }
+  }
 }
 
-// dX^T tile: A = W (K = vocabulary, down the rows), B = dl (K along the rows).  The piece's
-// vocabulary is split over blockIdx.y; each split owns its own fp32 sums, added to from piece
-// to piece, so the order of every sum is fixed.
-template <bool F16>
-__global__ __launch_bounds__(THREADS) void k_dx(const void* __restrict__ w, long long ldw, const void* __restrict__ dl,
-                                                long long lddl, int v0, int vn, int d, int dp,
-                                                const int* __restrict__ count, int n, int per_split, int first,
-                                                float* __restrict__ out) {
+// Into how many parts the vocabulary is split for dX of `rows` packed rows: as many as `fill`
+// workgroups have tiles for, at least 512 entries of a piece each.  Only the device knows `rows`.
+template <class Tile>
+__host__ __device__ __forceinline__ int splits_of(int rows, int d, int fill, int piece) {
+  const int tiles = ((d + Tile::BM - 1) / Tile::BM) * ((rows + Tile::BN - 1) / Tile::BN);
+  const int s = tiles ? fill / tiles : 1, most = piece / 512;
+  return s < 1 || most < 1 ? 1 : s < most ? s : most;
+}
+
+// dX^T tile: A = W (K = vocabulary, down the rows), B = dl (K along the rows).  Each split owns
+// its own fp32 sums [rows][dp], added to from piece to piece, so the order of every sum is fixed.
+template <class Tile, bool F16>
+__global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w, long long ldw,
+                                                      const void* __restrict__ dl, long long lddl, int v0, int vn,
+                                                      int d, int dp, const int* __restrict__ count, int fill,
+                                                      int first, float* __restrict__ out) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int rows = count[0];
-  const int tiles_d = (d + TILE - 1) / TILE, tiles_n = (rows + TILE - 1) / TILE, nwg = tiles_d * tiles_n;
+  const int rows = count[0], splits = splits_of<Tile>(rows, d, fill, (int)(lddl / 2));
+  const int tiles_d = (d + Tile::BM - 1) / Tile::BM, tiles_n = (rows + Tile::BN - 1) / Tile::BN;
+  const int tiles = tiles_d * tiles_n, nwg = tiles * splits;
   if ((int)blockIdx.x >= nwg) return;
+  const int place = run_of(blockIdx.x, nwg), split = place / tiles;
   int td, tn;
-  tile_of(blockIdx.x, nwg, tiles_d, tiles_n, &td, &tn);
-  const int tid = threadIdx.x, k0 = blockIdx.y * per_split, k = min(vn - k0, per_split);
-  const Panel<false> pa(w, ldw, td * TILE, d, v0 + k0, max(k, 0), tid);
-  const Panel<true> pb(dl, lddl, tn * TILE, rows, k0, (max(k, 0) + 7) & ~7, tid);  // dl is padded with zeros
-  Acc acc;
+  tile_of(place - split * tiles, tiles_d, tiles_n, &td, &tn);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int per_split = ((vn + KT - 1) / KT + splits - 1) / splits * KT;
+  const int k0 = split * per_split, k = max(0, min(vn - k0, per_split));
+  const PanelA<Tile, false> pa(w, ldw, td * Tile::BM, d, v0 + k0, k, tid);
+  const PanelB<Tile, true> pb(dl, lddl, tn * Tile::BN, rows, k0, (k + 7) & ~7, tid);  // dl is padded with zeros
+  Acc<Tile> acc;
   product<F16, false, true>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
-  const Lane l(tid);
-  out += (size_t)blockIdx.y * n * dp;
+  out += (size_t)split * rows * dp;
 #pragma unroll
-  for (int nh = 0; nh < 2; ++nh)
+  for (int j = 0; j < Tile::NF; ++j) {
+    const int token = tn * Tile::BN + Tile::col(j, wid) + (lane & 15);
+    if (token >= rows) continue;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int token = tn * TILE + nh * 128 + l.wc * 32 + j * 16 + l.fr;
-      if (token >= rows) continue;
-#pragma unroll
-      for (int mh = 0; mh < 2; ++mh)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = td * TILE + mh * 128 + l.wr * 64 + i * 16 + l.fq * 4;
-          if (c >= dp) continue;
-          f32x4* at = reinterpret_cast<f32x4*>(out + (size_t)token * dp + c);
-          f32x4 r = acc[mh][nh][i][j];
-          if (!first) r += *at;
-          *at = r;
-        }
+    for (int i = 0; i < Tile::MF; ++i) {
+      const int c = td * Tile::BM + Tile::row(i, wid) + (lane >> 4) * 4;
+      if (c >= dp) continue;
+      f32x4* at = reinterpret_cast<f32x4*>(out + (size_t)token * dp + c);
+      f32x4 r = acc[i][j];
+      if (!first) r += *at;
+      *at = r;
     }
+  }
 }
 
 // dW^T tile: A = Xc (K = tokens, down the rows), B = dl (K = tokens, down the rows).
-template <bool F16>
-__global__ __launch_bounds__(THREADS) void k_dw(const void* __restrict__ xc, long long ldxc,
-                                                const void* __restrict__ dl, long long lddl, int v0, int vn, int d,
-                                                const int* __restrict__ count, const float* __restrict__ scale,
-                                                void* __restrict__ dw, int lddw) {
+template <class Tile, bool F16>
+__global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ xc, long long ldxc,
+                                                      const void* __restrict__ dl, long long lddl, int v0, int vn,
+                                                      int d, const int* __restrict__ count, Upstream<F16> up,
+                                                      const int* __restrict__ at, const float* __restrict__ lost,
+                                                      int residuals, void* __restrict__ dw, int lddw) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
   const int rows = count[0];
-  const int tiles_d = (d + TILE - 1) / TILE, tiles_v = (vn + TILE - 1) / TILE;
+  const int tiles_d = (d + Tile::BM - 1) / Tile::BM, tiles_v = (vn + Tile::BN - 1) / Tile::BN;
   int td, tv;
-  tile_of(blockIdx.x, tiles_d * tiles_v, tiles_d, tiles_v, &td, &tv);
-  const int tid = threadIdx.x;
-  const Panel<false> pa(xc, ldxc, td * TILE, (int)(ldxc / 2), 0, rows, tid);
-  const Panel<false> pb(dl, lddl, tv * TILE, (int)(lddl / 2), 0, rows, tid);
-  Acc acc;
+  tile_of(run_of(blockIdx.x, tiles_d * tiles_v), tiles_d, tiles_v, &td, &tv);
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const PanelA<Tile, false> pa(xc, ldxc, td * Tile::BM, (int)(ldxc / 2), 0, rows, tid);
+  const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), 0, rows, tid);
+  Acc<Tile> acc;
   product<F16, false, false>(acc, smem, pa, pb, (rows + KT - 1) / KT, tid);
-  const Lane l(tid);
-  const float sc = scale[0];
+
+  // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
+  // share of the packed rows, in order; beyond ROOM of them a sum has so many targets that their
+  // roundings average out.  Their rows of Xc come through LDS, 64 at a time.
+  if (rows <= FEW_ROWS) {
+    constexpr int WAVES = Tile::THREADS / 64, ROOM = 32, PER = Tile::BM / 8;
+    struct Hit {
+      int pos, col;
+      float lost;
+    };
+    Hit* list = reinterpret_cast<Hit*>(smem);  // [WAVES][ROOM]
+    Hit* all = list + WAVES * ROOM;
+    int* lengths = reinterpret_cast<int*>(all + WAVES * ROOM);
+    u32x4* xrows = reinterpret_cast<u32x4*>(smem + 16384);  // [64][PER]
+    static_assert(2 * WAVES * ROOM * sizeof(Hit) + WAVES * 4 <= 16384, "the lists fit");
+    static_assert(16384 + 64 * PER * 16 <= Tile::LDS, "the rows fit");
+    __syncthreads();  // LDS has been read
+    const int entries = rows * residuals, share = (entries + Tile::THREADS - 1) / Tile::THREADS * 64;
+    const int end = min(entries, (wid + 1) * share);
+    const int first = v0 + tv * Tile::BN, width = min(Tile::BN, vn - tv * Tile::BN);
+    int found = 0;
+    for (int i = wid * share; i < end && found < ROOM; i += 64) {
+      const int e = i + lane, v = e < end ? at[e] - first : -1;
+      const bool here = v >= 0 && v < width;
+      const unsigned long long mask = __ballot(here);
+      const int slot = found + __popcll(mask & ((1ull << lane) - 1));
+      if (here && slot < ROOM) list[wid * ROOM + slot] = Hit{e / residuals, v, lost[e]};
+      found = min(ROOM, found + __popcll(mask));
+    }
+    if (lane == 0) lengths[wid] = found;
+    __syncthreads();
+    int total = 0;
+    for (int o = 0; o < WAVES; ++o) {
+      if (tid < lengths[o]) all[total + tid] = list[o * ROOM + tid];
+      total += lengths[o];
+    }
+    __syncthreads();
+    for (int b = 0; b < total; b += 64) {
+      const int here = min(64, total - b);
+      if (b) __syncthreads();
+      for (int i = tid; i < here * PER; i += Tile::THREADS) {
+        const int c = td * Tile::BM + i % PER * 8;
+        xrows[i] = c < (int)(ldxc / 2) ? *reinterpret_cast<const u32x4*>(static_cast<const T*>(xc) +
+                                                                       (size_t)all[b + i / PER].pos * (ldxc / 2) + c)
+                                       : u32x4{0, 0, 0, 0};
+      }
+      __syncthreads();
+      const Hit own = lane < here ? all[b + lane] : Hit{0, 0, 0.f};
+      for (int i = 0; i < here; ++i) {
+        const int col = __builtin_amdgcn_readlane(own.col, i);
+        if (!Tile::owns(col, __builtin_amdgcn_readfirstlane(wid))) continue;
+        const float l = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own.lost), i));
+        typedef __attribute__((ext_vector_type(4))) T t4;
+        const t4* x = reinterpret_cast<const t4*>(xrows + i * PER);
+#pragma unroll
+        for (int j = 0; j < Tile::NF; ++j)
+          if (Tile::col(j, wid) + (lane & 15) == col) {
+#pragma unroll
+            for (int m = 0; m < Tile::MF; ++m) {
+              const t4 v4 = x[(Tile::row(m, wid) + (lane >> 4) * 4) / 4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][j][e] += l * (float)v4[e];
+            }
+          }
+      }
+    }
+  }
+  const float sc = up.scale();
   const bool wide = (lddw & 3) == 0 && (reinterpret_cast<uintptr_t>(dw) & 7) == 0;
 #pragma unroll
-  for (int nh = 0; nh < 2; ++nh)
+  for (int j = 0; j < Tile::NF; ++j) {
+    const int row = tv * Tile::BN + Tile::col(j, wid) + (lane & 15);
+    if (row >= vn) continue;
+    T* out = static_cast<T*>(dw) + (size_t)(v0 + row) * lddw;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = tv * TILE + nh * 128 + l.wc * 32 + j * 16 + l.fr;
-      if (row >= vn) continue;
-      T* out = static_cast<T*>(dw) + (size_t)(v0 + row) * lddw;
+    for (int i = 0; i < Tile::MF; ++i) {
+      const int c = td * Tile::BM + Tile::row(i, wid) + (lane >> 4) * 4;
+      const f32x4 r = rows ? acc[i][j] * sc : f32x4{0.f, 0.f, 0.f, 0.f};
+      if (wide && c + 4 <= d) {
+        *reinterpret_cast<u32x2*>(out + c) = u32x2{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3])};
+      } else {
 #pragma unroll
-      for (int mh = 0; mh < 2; ++mh)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = td * TILE + mh * 128 + l.wr * 64 + i * 16 + l.fq * 4;
-          const f32x4 r = rows ? acc[mh][nh][i][j] * sc : f32x4{0.f, 0.f, 0.f, 0.f};
-          if (wide && c + 4 <= d) {
-            *reinterpret_cast<u32x2*>(out + c) = u32x2{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3])};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c + e < d) out[c + e] = (T)r[e];
-          }
-        }
+        for (int e = 0; e < 4; ++e)
+          if (c + e < d) out[c + e] = (T)r[e];
+      }
     }
+  }
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -570,17 +769,17 @@ __global__ __launch_bounds__(256) void k_teacher(const long long* __restrict__ i
   if (lane == 0) flag[row] = any;
 }
 
-// Packs the rows that have a loss into xc [rows][dp] (zeros behind d).  A block takes 16 rows
-// and counts the kept rows before them itself, which needs no second launch for a scan (8192
-// tokens: 512 blocks read at most 64 KiB of targets each, out of L2).
+// Packs the rows that have a loss into xc [rows][dp] (zeros behind d).  A block takes 8 rows, two
+// a wave, and counts the kept rows before them itself, which needs no second launch for a scan
+// (8192 tokens: 1024 blocks read at most 64 KiB of targets each, out of L2).
 template <typename T>
 __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long long ldx, int n, int d, int dp,
                                                 const long long* __restrict__ target, long long ignore,
                                                 const int* __restrict__ flag, T* __restrict__ xc,
                                                 int* __restrict__ rowmap, int* __restrict__ posof,
                                                 int* __restrict__ count, float* __restrict__ loss) {
-  __shared__ int total[4], kept[16];
-  const int row0 = blockIdx.x * 16, tid = threadIdx.x;
+  __shared__ int total[4], kept[8];
+  const int row0 = blockIdx.x * 8, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c = 0;
   if (flag) {
     for (int r = tid; r < row0; r += 256) c += flag[r] != 0;
@@ -589,18 +788,26 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
-  if ((tid & 63) == 0) total[tid >> 6] = c;
-  if (tid < 16) {
+  if (lane == 0) total[wave] = c;
+  if (tid < 8) {
     const int r = row0 + tid;
     kept[tid] = r < n && (flag ? flag[r] != 0 : target[r] != ignore);
   }
   __syncthreads();
   int pos = total[0] + total[1] + total[2] + total[3];
+  if (tid == 0 && row0 + 8 >= n) {
+    int all = pos;
+    for (int i = 0; i < 8; ++i) all += kept[i];
+    count[0] = all;
+    count[1] = 0;
+  }
+  for (int i = 0; i < wave * 2; ++i) pos += kept[i];
   const bool wide = (d & 7) == 0 && (ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  for (int i = 0; i < 16 && row0 + i < n; ++i) {
+  for (int i = wave * 2; i < wave * 2 + 2; ++i) {
     const int r = row0 + i;
+    if (r >= n) break;
     if (!kept[i]) {
-      if (tid == 0) {
+      if (lane == 0) {
         posof[r] = -1;
         if (loss) loss[r] = 0.f;
       }
@@ -609,18 +816,18 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
     T* out = xc + (size_t)pos * dp;
     const T* in = x + (long long)r * ldx;
     if (wide) {
-      for (int e = tid * 8; e < dp; e += 256 * 8)
+#pragma unroll 4
+      for (int e = lane * 8; e < dp; e += 512)
         *reinterpret_cast<u32x4*>(out + e) = e < d ? *reinterpret_cast<const u32x4*>(in + e) : u32x4{0, 0, 0, 0};
     } else {
-      for (int e = tid; e < dp; e += 256) out[e] = e < d ? in[e] : (T)0.f;
+      for (int e = lane; e < dp; e += 64) out[e] = e < d ? in[e] : (T)0.f;
     }
-    if (tid == 0) {
+    if (lane == 0) {
       rowmap[pos] = r;
       posof[r] = pos;
     }
     ++pos;
   }
-  if (tid == 0 && row0 + 16 >= n) count[0] = pos;
 }
 
 // A copy of w with rows of dp elements, zeros behind d: for a w whose rows are not 16-byte
@@ -632,46 +839,69 @@ __global__ __launch_bounds__(256) void k_pad(const T* __restrict__ w, long long 
     for (int e = threadIdx.x; e < dp; e += 256) out[r * dp + e] = e < d ? w[r * ldw + e] : (T)0.f;
 }
 
-// zk[pos][j] = x . w[id], one wave a target.  A cross entropy target outside the vocabulary
-// gives NaN, as does a listed id past its end; an id below 0 in a list is no entry.
+// x . w[id] over `lanes` neighbouring lanes, the sum in all of them.  A target outside the
+// vocabulary gives NaN.
+template <typename T>
+__device__ __forceinline__ float dot(const T* x, const T* w, long long ldw, int dk, long long id, long long v, int lane,
+                                     int lanes) {
+  if (id < 0 || id >= v) return NAN;
+  const T* b = w + id * ldw;
+  float s = 0.f;
+#pragma unroll 4
+  for (int e = lane * 8; e < dk; e += lanes * 8) {
+    typedef __attribute__((ext_vector_type(8))) T t8;
+    const t8 p = *reinterpret_cast<const t8*>(x + e), q = *reinterpret_cast<const t8*>(b + e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += (float)p[i] * (float)q[i];
+  }
+  for (int o = lanes / 2; o; o >>= 1) s += __shfl_xor(s, o, 64);
+  return s;
+}
+
+// A teacher's lists: zk[pos][j] = x . w[id], one wave a target.  An id below 0 is no entry.
 template <typename T>
 __global__ __launch_bounds__(256) void k_dots(const T* __restrict__ xc, int dp, const T* __restrict__ w,
                                               long long ldw, int dk, const long long* __restrict__ ids, int k,
-                                              long long v, int distill, const int* __restrict__ rowmap,
+                                              long long v, const int* __restrict__ rowmap,
                                               const int* __restrict__ count, float* __restrict__ zk) {
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int pos = (int)(item / k), j = (int)(item - (long long)pos * k), lane = threadIdx.x & 63;
   if (pos >= count[0]) return;
   const long long id = ids[(size_t)rowmap[pos] * k + j];
-  float s = 0.f;
-  if (id >= 0 && id < v) {
-    const T* a = xc + (size_t)pos * dp;
-    const T* b = w + id * ldw;
-    for (int e = lane * 8; e < dk; e += 512) {
-      typedef __attribute__((ext_vector_type(8))) T t8;
-      const t8 p = *reinterpret_cast<const t8*>(a + e), q = *reinterpret_cast<const t8*>(b + e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += (float)p[i] * (float)q[i];
-    }
-    s = wave_sum(s);
-  } else if (!distill || id >= 0) {
-    s = NAN;
-  }
+  const float s = id < 0 ? 0.f : dot(xc + (size_t)pos * dp, w, ldw, dk, id, v, lane, 64);
   if (lane == 0) zk[(size_t)pos * k + j] = s;
 }
 
-// Joins the tiles' (max, sum) of 8 rows, 32 threads a row, and forms the rows' losses.
-// lse is kept in the exponent's base 2.
+// Joins the tiles' (max, sum) of 8 rows, 32 threads a row, and forms the rows' losses; of a cross
+// entropy (p null) also the targets' logits.  lse is kept in the exponent's base 2.  With a
+// reduction the block that ends last adds the rows' losses, always in the same order (`done` not
+// null; the release that this takes of every block costs 60 us of 1024 blocks, so many rows have
+// k_reduce).  A batch without any loss has 0.
+template <typename T>
 __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, int parts, int n,
+                                              const T* __restrict__ xc, int dp, const T* __restrict__ w, long long ldw,
+                                              int dk, const long long* __restrict__ ids, long long v,
                                               const float* __restrict__ zk, const float* __restrict__ p, int k,
                                               const int* __restrict__ rowmap, const int* __restrict__ count, float sc,
                                               float t2, float* __restrict__ lse, float* __restrict__ rowloss,
-                                              float* __restrict__ loss) {
-  __shared__ float sm[32][8], ss[32][8], sd[32][8];
+                                              float* __restrict__ loss, int reduction, int* __restrict__ at_out,
+                                              int* __restrict__ done) {
+  __shared__ float sm[32][8], ss[32][8], sd[32][8], sz[8];
   const int r = threadIdx.x & 7, slice = threadIdx.x >> 3, pos = blockIdx.x * 8 + r, rows = count[0];
-  if ((int)blockIdx.x * 8 >= rows) return;
+  if (!p) {
+    const int own = threadIdx.x >> 5, at = blockIdx.x * 8 + own;
+    if (at < rows) {
+      const long long id = ids[rowmap[at]];
+      const float z = dot(xc + (size_t)at * dp, w, ldw, dk, id, v, threadIdx.x & 31, 32);
+      if ((threadIdx.x & 31) == 0) {
+        sz[own] = z;
+        at_out[at] = id >= 0 && id < v ? (int)id : -1;
+      }
+    }
+  }
   float m = -INFINITY, s = 0.f, dot = 0.f;
   if (pos < rows) {
+#pragma unroll 4
     for (int i = slice; i < parts; i += 32) {
       const float2 c = part[(size_t)i * n + pos];
       merge(m, s, c.x, c.y);
@@ -684,8 +914,6 @@ __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, i
         if (q > 0.f) dot += q * (logf(q) - LN2 * sc * z);
         else if (q != q || z != z) dot = NAN;
       }
-    } else if (slice == 0) {
-      dot = -LN2 * sc * zk[pos];
     }
   }
   sm[slice][r] = m;
@@ -697,16 +925,36 @@ __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, i
       merge(m, s, sm[i][r], ss[i][r]);
       dot += sd[i][r];
     }
+    if (!p) dot = -LN2 * sc * sz[r];
     const float l = m + log2f(s), out = t2 * (dot + LN2 * l);
     lse[pos] = l;
-    rowloss[pos] = out;
-    if (loss) loss[rowmap[pos]] = out;
+    __hip_atomic_store(rowloss + pos, out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!reduction) loss[rowmap[pos]] = out;
+  }
+  if (!done) return;
+  __shared__ int last;
+  __shared__ double part_sum[4];
+  __syncthreads();
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  double total = 0.;
+  for (int i = threadIdx.x; i < rows; i += 256)
+    total += __hip_atomic_load(rowloss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
+  if ((threadIdx.x & 63) == 0) part_sum[threadIdx.x >> 6] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    total = part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3];
+    loss[0] = (float)(reduction == 2 ? total / max(rows, 1) : total);
   }
 }
 
-// The sum or mean of the rows' losses in a fixed order; a batch without any loss has 0.
+// The sum or mean of the rows' losses, in a fixed order.
 __global__ __launch_bounds__(1024) void k_reduce(const float* __restrict__ rowloss, const int* __restrict__ count,
-                                                 int mean, float* __restrict__ loss) {
+                                                 int reduction, float* __restrict__ loss) {
   __shared__ double sum[16];
   const int rows = count[0];
   double s = 0.;
@@ -717,87 +965,170 @@ __global__ __launch_bounds__(1024) void k_reduce(const float* __restrict__ rowlo
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) s += sum[i];
-    loss[0] = (float)(mean ? s / max(rows, 1) : s);
+    loss[0] = (float)(reduction == 2 ? s / max(rows, 1) : s);
   }
 }
 
-// factor[pos] = span * g / max|g|, scale = max|g| T / span: dl holds factor * (q - p), and the
-// products are scaled once, in 32 bits.  span is 1 for bf16, which has an fp32 exponent, and
-// 2^15 for fp16: |q - p| <= 1 stays below its largest value 65504, and a probability keeps
-// its 11 bits down to 2^-29 instead of 2^-14.  A row whose loss is NaN gets NaN gradients.
-__global__ __launch_bounds__(1024) void k_factor(const float* __restrict__ grad, long long ldg, int reduction,
-                                                 const int* __restrict__ rowmap, const int* __restrict__ count,
-                                                 const float* __restrict__ rowloss, float t, float span,
-                                                 float* __restrict__ factor, float* __restrict__ scale) {
+// fp16 without a reduction: factor[pos] = span g / max|g|, factor[n] = max|g| T / span.
+__global__ __launch_bounds__(1024) void k_factor(const float* __restrict__ grad, long long ldg,
+                                                 const int* __restrict__ rowmap, const int* __restrict__ count, int n,
+                                                 float t, float span, float* __restrict__ factor) {
   __shared__ float top[16];
   const int rows = count[0];
   float m = 0.f;
-  if (reduction == 0) {
-    for (int i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(grad[rowmap[i] * ldg]));
-    m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, top[i]);
-  } else {
-    m = fabsf(grad[0]);
-  }
+  for (int i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(grad[rowmap[i] * ldg]));
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+  __syncthreads();
+  for (int i = 0; i < 16; ++i) m = fmaxf(m, top[i]);
   for (int i = threadIdx.x; i < rows; i += 1024) {
-    const float g = grad[reduction == 0 ? rowmap[i] * ldg : 0];
-    const float l = rowloss[i];
-    factor[i] = l != l ? NAN : g == 0.f ? 0.f : g / m * span;
+    const float g = grad[rowmap[i] * ldg];
+    factor[i] = g == 0.f ? 0.f : g / m * span;
   }
-  if (threadIdx.x == 0) scale[0] = m * t / span / (reduction == 2 ? (float)max(rows, 1) : 1.f);
+  if (threadIdx.x == 0) factor[n] = m * t / span;
 }
 
-// Puts the targets into the piece's dl: f (q - sum of the p of that id).  One wave a row.
-template <typename T>
+// Puts a teacher's targets into the piece's dl: f (q - sum of the p of that id).  One wave a row.
+// The first RESIDUALS entries of the list whose derivative is large are those that are made good.
+template <bool F16>
 __global__ __launch_bounds__(256) void k_fix(const long long* __restrict__ ids, const float* __restrict__ p, int k,
-                                             const float* __restrict__ zk, const float* __restrict__ lse,
-                                             const float* __restrict__ factor, const int* __restrict__ rowmap,
-                                             const int* __restrict__ count, float sc, long long v0, long long vn,
-                                             T* __restrict__ dl, long long lddl) {
-  const int pos = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (pos >= count[0]) return;
-  const size_t row = (size_t)rowmap[pos] * k;
+                                             long long v, const float* __restrict__ zk, const float* __restrict__ lse,
+                                             Upstream<F16> up, float sc, long long v0, long long vn,
+                                             void* __restrict__ dl, long long lddl, int* __restrict__ at,
+                                             float* __restrict__ lost) {
+  using T = typename Type<F16>::T;
+  __shared__ int list[4][MAX_TARGETS];  // vocabulary entries, -1: none
+  const int wave = threadIdx.x >> 6, pos = blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
+  if (pos >= up.count[0]) return;
+  const size_t row = (size_t)up.rowmap[pos] * k;
   for (int i = lane; i < k; i += 64) {
     const long long id = ids[row + i];
-    if (id < v0 || id >= v0 + vn) continue;
-    float sum = 1.f;
-    bool firstone = true;
-    if (p) {
-      sum = 0.f;
+    list[wave][i] = id >= 0 && id < v ? (int)id : -1;
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list: no barrier
+  const float f = up.of(pos), ls = lse[pos];
+  int large = 0;
+  for (int i0 = 0; i0 < k; i0 += 64) {
+    const int i = i0 + lane, id = i < k ? list[wave][i] : -1;
+    float sum = 0.f;
+    bool firstone = id >= 0;
+    if (firstone)
       for (int o = 0; o < k; ++o)
-        if (ids[row + o] == id) {
+        if (list[wave][o] == id) {
           sum += p[row + o];
           firstone &= o >= i;
         }
+    const float g = firstone ? __builtin_amdgcn_exp2f(zk[(size_t)pos * k + i] * sc - ls) - sum : 0.f;
+    const unsigned long long mask = __ballot(fabsf(g) >= LARGE);
+    const int slot = large + __popcll(mask & ((1ull << lane) - 1));
+    large += __popcll(mask);
+    if (!firstone) continue;
+    const bool here = id >= v0 && id < v0 + vn;
+    const T r = (T)(f * g);
+    if (here) static_cast<T*>(dl)[(size_t)pos * lddl + (id - v0)] = r;
+    if (fabsf(g) >= LARGE && slot < RESIDUALS) {
+      if (v0 == 0) at[pos * RESIDUALS + slot] = id;
+      if (here) lost[pos * RESIDUALS + slot] = f * g - (float)r;
     }
-    if (firstone)
-      dl[(size_t)pos * lddl + (id - v0)] =
-          (T)(factor[pos] * (__builtin_amdgcn_exp2f(zk[(size_t)pos * k + i] * sc - lse[pos]) - sum));
   }
+  if (v0 == 0 && lane >= large && lane < RESIDUALS) at[pos * RESIDUALS + lane] = -1;
 }
 
-// Joins the splits of dX, scales, rounds once, and puts zeros into the rows without a loss.
-template <typename T>
-__global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, int splits, int n, int d, int dp,
-                                                const int* __restrict__ posof, const float* __restrict__ scale,
-                                                T* __restrict__ dx) {
+// Joins the splits of dX, adds what dl's rounding took, scales, rounds once, and puts zeros into
+// the rows without a loss.
+template <bool F16>
+__global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, int small, int fill, int piece,
+                                                int dk, int d, int dp,
+                                                const int* __restrict__ posof, Upstream<F16> up,
+                                                const int* __restrict__ at, const float* __restrict__ lost,
+                                                int residuals, const void* __restrict__ w, long long ldw,
+                                                void* __restrict__ dx) {
+  using T = typename Type<F16>::T;
+  typedef __attribute__((ext_vector_type(4))) T t4;
   const int per_row = (d + 1023) / 1024, row = blockIdx.x / per_row, pos = posof[row];
   const int c = ((blockIdx.x - row * per_row) * 256 + threadIdx.x) * 4;
   if (c >= d) return;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (pos >= 0) {
+    const int rows = up.count[0];
+    const int splits = small ? splits_of<Small>(rows, dk, fill, piece) : splits_of<Big>(rows, dk, fill, piece);
     for (int i = 0; i < splits; ++i)
-      s += *reinterpret_cast<const f32x4*>(part + ((size_t)i * n + pos) * dp + c);
-    s *= scale[0];
+      s += *reinterpret_cast<const f32x4*>(part + ((size_t)i * rows + pos) * dp + c);
+    for (int i = 0; rows <= FEW_ROWS && i < residuals; ++i) {
+      const int id = at[pos * residuals + i];
+      if (id < 0) break;
+      const t4 v = *reinterpret_cast<const t4*>(static_cast<const T*>(w) + id * ldw + c);
+      const float l = lost[pos * residuals + i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += l * (float)v[e];
+    }
+    s *= up.scale();
   }
-  T* out = dx + (size_t)row * d + c;
+  T* out = static_cast<T*>(dx) + (size_t)row * d + c;
   if ((d & 3) == 0) {
     *reinterpret_cast<u32x2*>(out) = u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])};
   } else {
     for (int e = 0; e < 4 && c + e < d; ++e) out[e] = (T)s[e];
   }
+}
+
+int padded(long long d) { return (int)((d + 63) / 64 * 64); }
+
+int residuals(const tkl_args& a) { return a.distill ? RESIDUALS : 1; }
+
+// What the forward pass keeps, in one buffer.  Without a teacher zk, p and flag are not there.
+struct Kept {
+  char* xc;                        // [n][dp], the packed rows
+  float *lse, *rowloss;            // by packed row
+  int *rowmap, *posof, *count;     // packed row -> token and back; count[0] packed rows, count[1] k_loss's
+  float *zk, *p;                   // [packed row][k] logits of the targets, [token][k] probabilities
+  int* flag;                       // by token: whether it has a target
+  int* at;                         // [packed row][residuals] vocabulary entries, -1: none
+  long long bytes;
+};
+Kept kept_of(const tkl_args& a) {
+  Kept r;
+  const long long n = a.n, lists = a.distill ? n * a.k : 0;
+  char* at = static_cast<char*>(a.kept);
+  auto take = [&](long long size) {
+    char* was = at;
+    at += size;
+    return was;
+  };
+  r.xc = take(2 * n * padded(a.d));
+  r.lse = reinterpret_cast<float*>(take(4 * n));
+  r.rowloss = reinterpret_cast<float*>(take(4 * n));
+  r.rowmap = reinterpret_cast<int*>(take(4 * n));
+  r.posof = reinterpret_cast<int*>(take(4 * n));
+  r.count = reinterpret_cast<int*>(take(8));
+  r.zk = a.distill ? reinterpret_cast<float*>(take(4 * lists)) : nullptr;
+  r.p = a.distill ? reinterpret_cast<float*>(take(4 * lists)) : nullptr;
+  r.flag = a.distill ? reinterpret_cast<int*>(take(4 * n)) : nullptr;
+  r.at = reinterpret_cast<int*>(take(4 * n * residuals(a)));
+  r.bytes = at - static_cast<char*>(a.kept);
+  return r;
+}
+// The backward pass' workspace, in one buffer.
+struct Room {
+  void* dl;       // [n][piece] 16-bit
+  float* sums;    // [splits][packed rows][dp] of dX: n dp, or what `fill` tiles hold
+  float* factor;  // [n + 1]
+  float* lost;    // [packed row][residuals] what dl's rounding took
+  long long bytes;
+};
+Room room_of(const tkl_args& a) {
+  Room r;
+  char* at = static_cast<char*>(a.room);
+  r.dl = at;
+  at += 2 * a.n * a.piece;
+  r.sums = reinterpret_cast<float*>(at);
+  const long long once = a.n * padded(a.d), tile = a.small & 2 ? Small::BM * Small::BN : Big::BM * Big::BN;
+  if (a.want & 1) at += 4 * std::max(once, std::min(a.piece / 512 * once, a.fill * tile));
+  r.factor = reinterpret_cast<float*>(at);
+  at += 4 * (a.n + 1);
+  r.lost = reinterpret_cast<float*>(at);
+  r.bytes = at + 4 * a.n * residuals(a) - static_cast<char*>(a.room);
+  return r;
 }
 
 // Where the kernels read w: w itself, or its padded copy.
@@ -812,14 +1143,12 @@ Weight weight_of(const tkl_args& a, int dp) {
   return {a.w, a.ldw * 2, (int)a.d};
 }
 
-int padded(long long d) { return (int)((d + 63) / 64 * 64); }
-
 int check(const tkl_args& a) {
   const char* bad = nullptr;
   if (a.n < 1 || a.n > (1 << 20)) bad = "tokens must be 1 to 2^20";
   else if (a.d < 1 || a.d > (1 << 16)) bad = "the width must be 1 to 65536";
   else if (a.v < 1 || a.v > (1 << 24)) bad = "the vocabulary must have 1 to 2^24 entries";
-  else if (a.k < 1 || a.k > 1024) bad = "1 to 1024 targets a token";
+  else if (a.k < 1 || a.k > MAX_TARGETS) bad = "1 to 1024 targets a token";
   else if (!a.wc && ((a.d & 7) || (a.ldw & 7) || (reinterpret_cast<uintptr_t>(a.w) & 15)))
     bad = "w's rows are not 16-byte aligned and there is no room for a copy";
   else if (!a.wc && (a.ldw < a.d || a.ldw > (1 << 21))) bad = "w's row stride must be its width to 2^21 elements";
@@ -832,6 +1161,19 @@ int check(const tkl_args& a) {
   return 0;
 }
 
+// A matrix product's kernel may use more LDS than the default limit.
+template <class Kernel>
+hipError_t allow(Kernel* k, int lds) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+}
+template <class Tile, bool F16>
+hipError_t allow_all() {
+  hipError_t e = allow(&k_logits<Tile, F16, false>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_logits<Tile, F16, true>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_dx<Tile, F16>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_dw<Tile, F16>, Tile::LDS);
+  return e;
+}
 hipError_t set_lds_limit() {
   static std::once_flag once[64];
   static hipError_t result[64];
@@ -840,20 +1182,30 @@ hipError_t set_lds_limit() {
   if (e != hipSuccess) return e;
   if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
   std::call_once(once[dev], [dev] {
-    const void* fns[] = {
-        reinterpret_cast<const void*>(&k_logits<false, false>), reinterpret_cast<const void*>(&k_logits<true, false>),
-        reinterpret_cast<const void*>(&k_logits<false, true>),  reinterpret_cast<const void*>(&k_logits<true, true>),
-        reinterpret_cast<const void*>(&k_dx<false>),            reinterpret_cast<const void*>(&k_dx<true>),
-        reinterpret_cast<const void*>(&k_dw<false>),            reinterpret_cast<const void*>(&k_dw<true>)};
-    for (const void* f : fns) {
-      result[dev] = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-      if (result[dev] != hipSuccess) return;
-    }
+    result[dev] = allow_all<Big, false>();
+    if (result[dev] == hipSuccess) result[dev] = allow_all<Big, true>();
+    if (result[dev] == hipSuccess) result[dev] = allow_all<Small, false>();
+    if (result[dev] == hipSuccess) result[dev] = allow_all<Small, true>();
   });
   return result[dev];
 }
 
 unsigned blocks(long long items, long long per) { return (unsigned)((items + per - 1) / per); }
+
+template <typename T>
+void pad(const tkl_args& a, int dp, hipStream_t s) {
+  if (a.wc)
+    k_pad<T><<<(unsigned)std::min<long long>(a.v, 65536), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, a.v, (int)a.d,
+                                                                       dp, static_cast<T*>(a.wc));
+}
+
+template <class Tile, bool F16, bool DL>
+void logits(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
+            float* lost, hipStream_t s) {
+  k_logits<Tile, F16, DL><<<blocks(vn, Tile::BM) * blocks(a.n, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
+      w.at, w.ldb, kept.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, kept.count, (int)a.n, LOG2E / a.temperature,
+      static_cast<float2*>(a.room), kept.lse, up, a.distill ? nullptr : kept.at, a.room, a.piece, lost);
+}
 
 template <bool F16>
 hipError_t forward(const tkl_args& a) {
@@ -861,31 +1213,41 @@ hipError_t forward(const tkl_args& a) {
   hipStream_t s = static_cast<hipStream_t>(a.stream);
   const int n = (int)a.n, d = (int)a.d, k = (int)a.k, dp = padded(a.d);
   const long long* ids = static_cast<const long long*>(a.ids);
-  int *rowmap = static_cast<int*>(a.rowmap), *posof = static_cast<int*>(a.posof), *count = static_cast<int*>(a.count),
-      *flag = a.distill ? static_cast<int*>(a.flag) : nullptr;
-  float *p = a.distill ? static_cast<float*>(a.p) : nullptr, *each = a.reduction == 0 ? static_cast<float*>(a.loss) : nullptr;
-  const float t = a.temperature, sc = LOG2E / t;
-  if (a.distill) k_teacher<<<blocks(n, 4), 256, 0, s>>>(ids, static_cast<const float*>(a.teacher), n, k, 1.f / t, p, flag);
-  k_gather<T><<<blocks(n, 16), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, dp, ids, a.ignore, flag,
-                                            static_cast<T*>(a.xc), rowmap, posof, count, each);
-  if (a.wc)
-    k_pad<T><<<(unsigned)std::min<long long>(a.v, 65536), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, a.v, d, dp,
-                                                                       static_cast<T*>(a.wc));
+  const Kept q = kept_of(a);
+  float *loss = static_cast<float*>(a.loss), t = a.temperature;
+  T* xc = reinterpret_cast<T*>(q.xc);
+  if (a.distill)
+    k_teacher<<<blocks(n, 4), 256, 0, s>>>(ids, static_cast<const float*>(a.teacher), n, k, 1.f / t, q.p, q.flag);
+  k_gather<T><<<blocks(n, 8), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, dp, ids, a.ignore, q.flag, xc,
+                                           q.rowmap, q.posof, q.count, a.reduction ? nullptr : loss);
+  pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
-  const unsigned tiles_v = blocks(a.v, TILE), tiles_n = blocks(n, TILE);
-  k_logits<F16, false><<<tiles_v * tiles_n, THREADS, LDS, s>>>(w.at, w.ldb, a.xc, (long long)dp * 2, 0, (int)a.v, w.dk,
-                                                               count, n, sc, static_cast<float2*>(a.part), nullptr,
-                                                               nullptr, nullptr, 0);
-  k_dots<T><<<blocks((long long)n * k, 4), 256, 0, s>>>(static_cast<const T*>(a.xc), dp, static_cast<const T*>(w.at),
-                                                        w.ldb / 2, w.dk, ids, k, a.v, a.distill, rowmap, count,
-                                                        static_cast<float*>(a.zk));
-  k_loss<<<blocks(n, 8), 256, 0, s>>>(static_cast<const float2*>(a.part), 2 * (int)tiles_v, n,
-                                      static_cast<const float*>(a.zk), p, k, rowmap, count, sc, t * t,
-                                      static_cast<float*>(a.lse), static_cast<float*>(a.rowloss), each);
-  if (a.reduction)
-    k_reduce<<<1, 1024, 0, s>>>(static_cast<const float*>(a.rowloss), count, a.reduction == 2,
-                                static_cast<float*>(a.loss));
+  const T* wt = static_cast<const T*>(w.at);
+  if (a.small & 1) logits<Small, F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
+  else logits<Big, F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
+  if (a.distill)
+    k_dots<T><<<blocks((long long)n * k, 4), 256, 0, s>>>(xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count,
+                                                          q.zk);
+  k_loss<T><<<blocks(n, 8), 256, 0, s>>>(static_cast<const float2*>(a.room),
+                                         (int)blocks(a.v, a.small & 1 ? Small::BM : Big::BM), n, xc, dp, wt, w.ldb / 2,
+                                         w.dk, ids, a.v, q.zk, q.p, k, q.rowmap, q.count, LOG2E / t, t * t, q.lse,
+                                         q.rowloss, loss, a.reduction, q.at, a.reduction && n <= 512 ? q.count + 1 : nullptr);
+  if (a.reduction && n > 512) k_reduce<<<1, 1024, 0, s>>>(q.rowloss, q.count, a.reduction, loss);
   return hipGetLastError();
+}
+
+template <class Tile, bool F16>
+void dx(const tkl_args& a, const Kept& q, const Room& r, const Weight& w, int dp, long long v0, int vn, hipStream_t s) {
+  const unsigned most = std::max<long long>((long long)blocks(w.dk, Tile::BM) * blocks(a.n, Tile::BN), a.fill);
+  k_dx<Tile, F16><<<most, Tile::THREADS, Tile::LDS, s>>>(w.at, w.ldb, r.dl, a.piece * 2, (int)v0, vn, w.dk, dp, q.count,
+                                                         (int)a.fill, v0 == 0, r.sums);
+}
+
+template <class Tile, bool F16>
+void dw(const tkl_args& a, const Kept& q, const Room& r, int dp, long long v0, int vn, const Upstream<F16>& up,
+        hipStream_t s) {
+  k_dw<Tile, F16><<<blocks(a.d, Tile::BM) * blocks(vn, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
+      q.xc, (long long)dp * 2, r.dl, a.piece * 2, (int)v0, vn, (int)a.d, q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d);
 }
 
 template <bool F16>
@@ -893,40 +1255,34 @@ hipError_t backward(const tkl_args& a) {
   using T = typename Type<F16>::T;
   hipStream_t s = static_cast<hipStream_t>(a.stream);
   const int n = (int)a.n, d = (int)a.d, k = (int)a.k, dp = padded(a.d);
-  const long long* ids = static_cast<const long long*>(a.ids);
-  const int *rowmap = static_cast<const int*>(a.rowmap), *count = static_cast<const int*>(a.count);
-  const float* p = a.distill ? static_cast<const float*>(a.p) : nullptr;
-  const float *lse = static_cast<const float*>(a.lse), *zk = static_cast<const float*>(a.zk);
-  const float t = a.temperature, sc = LOG2E / t, span = F16 ? 32768.f : 1.f;
-  float *factor = static_cast<float*>(a.factor), *scale = factor + n;
-  k_factor<<<1, 1024, 0, s>>>(static_cast<const float*>(a.grad), a.ldg, a.reduction, rowmap, count,
-                              static_cast<const float*>(a.rowloss), t, span, factor, scale);
-  if (a.wc)
-    k_pad<T><<<(unsigned)std::min<long long>(a.v, 65536), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, a.v, d, dp,
-                                                                       static_cast<T*>(a.wc));
+  const Kept q = kept_of(a);
+  const Room r = room_of(a);
+  const Upstream<F16> up = {static_cast<const float*>(a.grad), q.rowloss, r.factor, q.rowmap, q.count, a.ldg, a.reduction,
+                            n, a.temperature};
+  if (F16 && a.reduction == 0)
+    k_factor<<<1, 1024, 0, s>>>(up.grad, up.ldg, up.rowmap, up.count, n, a.temperature, Upstream<F16>::SPAN, r.factor);
+  pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
-  const unsigned tiles_n = blocks(n, TILE), tiles_d = blocks(d, TILE);
-  const long long ldl = a.piece * 2;  // bytes of a row of dl
   for (long long v0 = 0; v0 < a.v; v0 += a.piece) {
     const int vn = (int)std::min(a.piece, a.v - v0);
-    k_logits<F16, true><<<blocks(vn, TILE) * tiles_n, THREADS, LDS, s>>>(
-        w.at, w.ldb, a.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, count, n, sc, nullptr, lse, factor, a.dl,
-        a.piece);
-    k_fix<T><<<blocks(n, 4), 256, 0, s>>>(ids, p, k, zk, lse, factor, rowmap, count, sc, v0, vn, static_cast<T*>(a.dl),
-                                          a.piece);
+    if (a.small & 1) logits<Small, F16, true>(a, q, w, dp, v0, vn, up, r.lost, s);
+    else logits<Big, F16, true>(a, q, w, dp, v0, vn, up, r.lost, s);
+    if (a.distill)
+      k_fix<F16><<<blocks(n, 4), 256, 0, s>>>(static_cast<const long long*>(a.ids), q.p, k, a.v, q.zk, q.lse, up,
+                                              LOG2E / a.temperature, v0, vn, r.dl, a.piece, q.at, r.lost);
     if (a.want & 1) {
-      const int per = (int)blocks(blocks(vn, KT), a.splits) * KT;
-      k_dx<F16><<<dim3(tiles_d * tiles_n, (unsigned)a.splits), THREADS, LDS, s>>>(
-          w.at, w.ldb, a.dl, ldl, (int)v0, vn, w.dk, dp, count, n, per, v0 == 0, static_cast<float*>(a.dxpart));
+      if (a.small & 2) dx<Small, F16>(a, q, r, w, dp, v0, vn, s);
+      else dx<Big, F16>(a, q, r, w, dp, v0, vn, s);
     }
-    if (a.want & 2)
-      k_dw<F16><<<tiles_d * blocks(vn, TILE), THREADS, LDS, s>>>(a.xc, (long long)dp * 2, a.dl, ldl, (int)v0, vn, d,
-                                                                 count, scale, a.dw, d);
+    if (a.want & 2) {
+      if (a.small & 4) dw<Small, F16>(a, q, r, dp, v0, vn, up, s);
+      else dw<Big, F16>(a, q, r, dp, v0, vn, up, s);
+    }
   }
   if (a.want & 1)
-    k_dx_out<T><<<blocks(d, 1024) * (unsigned)n, 256, 0, s>>>(static_cast<const float*>(a.dxpart), (int)a.splits,
-                                                                   n, d, dp, static_cast<const int*>(a.posof), scale,
-                                                                   static_cast<T*>(a.dx));
+    k_dx_out<F16><<<blocks(d, 1024) * (unsigned)n, 256, 0, s>>>(r.sums, a.small & 2, (int)a.fill, (int)a.piece, w.dk, d,
+                                                                dp, q.posof, up, q.at,
+                                                                r.lost, residuals(a), w.at, w.ldb / 2, a.dx);
   return hipGetLastError();
 }
 
@@ -947,16 +1303,18 @@ int on_device(const tkl_args* a, hipError_t (*run)(const tkl_args&)) {
 
 }  // namespace
 
-// The caller's struct has to be this one.
+// What the caller has to agree on: the struct's size, and the bytes of its `kept` and (with a
+// piece) backward's `room`.
 extern "C" int tkl_args_size() { return (int)sizeof(tkl_args); }
+extern "C" long long tkl_kept_bytes(const tkl_args* a) { return kept_of(*a).bytes; }
+extern "C" long long tkl_room_bytes(const tkl_args* a) { return room_of(*a).bytes; }
 
 // Both are queued on a->stream and wait for nothing.  0, or -1 / a HIP error (tkl_last_error).
 extern "C" int tkl_forward(const tkl_args* a) { return on_device(a, a->f16 ? forward<true> : forward<false>); }
 
 extern "C" int tkl_backward(const tkl_args* a) {
-  if (a->piece < TILE || a->piece % TILE || a->piece > (1 << 24) || a->splits < 1 || a->splits > 1024) {
-    snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, splits %lld 1 to 1024", a->piece, TILE,
-             a->splits);
+  if (a->piece < Big::BM || a->piece % Big::BM || a->piece > (1 << 24) || a->fill < 1 || a->fill > 4096) {
+    snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, fill %lld 1 to 4096", a->piece, Big::BM, a->fill);
     return -1;
   }
   return on_device(a, a->f16 ? backward<true> : backward<false>);

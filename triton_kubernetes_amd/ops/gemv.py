@@ -29,6 +29,9 @@ _loaded = None
 def _lib():
     global _loaded
     if _loaded is None:
+        from .native import require_torch_first
+
+        require_torch_first()
         lib = load("libtk_gemv.so")
         lib.tkv_last_error.restype = ctypes.c_char_p
         i, ll, p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
@@ -81,42 +84,43 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
     wants one is refused."""
     import torch
 
-    from .native import require_torch_first
-
-    require_torch_first()
-    if x.dtype not in (torch.bfloat16, torch.float16) or scales.dtype != x.dtype:
+    dtype = x.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or scales.dtype is not dtype:
         raise GemvError(f"gemv_w4 wants x and scales both bf16 or both fp16, not {x.dtype} and {scales.dtype}")
     n, k, group = _check_weight(codes, scales, zeros)
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise GemvError(f"x {list(x.shape)} does not go with {k} columns")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] != k:
+        raise GemvError(f"x {list(shape)} does not go with {k} columns")
     if n > MAX_OUT or k > MAX_IN:
         raise GemvError(f"a weight of {n} x {k} (at most {MAX_OUT} x {MAX_IN})")
-    weight = (codes, scales) if zeros is None else (codes, scales, zeros)
-    if not x.is_cuda or any(t.device != x.device for t in weight):
+    dev = x.device
+    if not x.is_cuda or codes.device != dev or scales.device != dev or (zeros is not None and zeros.device != dev):
         raise GemvError("gemv_w4 wants CUDA tensors on one device")
-    if not all(t.is_contiguous() for t in weight) or codes.data_ptr() % 16:
+    if not (codes.is_contiguous() and scales.is_contiguous() and (zeros is None or zeros.is_contiguous())) \
+            or codes.data_ptr() % 16:
         raise GemvError("gemv_w4 wants a contiguous weight, its codes 16-byte aligned")
-    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad):
+    if (x.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
         raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
     m = x.numel() // k
     if m > MAX_ROWS:
         raise GemvError(f"{m} rows of x (at most {MAX_ROWS}): dequantize_w4 and a matrix product serve more")
-    shape = (*x.shape[:-1], n)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
-        raise GemvError(f"out must be contiguous {x.dtype} {list(shape)} on x's device")
+        out = torch.empty((*shape[:-1], n), dtype=dtype, device=dev)
+    elif out.shape != (*shape[:-1], n) or out.dtype is not dtype or out.device != dev or not out.is_contiguous():
+        raise GemvError(f"out must be contiguous {dtype} {[*shape[:-1], n]} on x's device")
     if m == 0 or n == 0:
         return out
-    x = x.reshape(m, k)
-    if x.stride(1) != 1 or x.stride(0) < k or x.stride(0) % 8 or x.data_ptr() % 16:
+    if len(shape) != 2:
+        x = x.reshape(m, k)
+    ldx = x.stride(0)
+    if x.stride(1) != 1 or ldx < k or ldx % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
+        ldx = k
     parts = splits(m, n, k)
-    room = torch.empty((parts, m, n), dtype=torch.float32, device=x.device) if parts > 1 else None
-    rc = _lib().tkv_gemv_w4(x.device.index, x.dtype == torch.float16, x.data_ptr(), x.stride(0), codes.data_ptr(),
-                            scales.data_ptr(), None if zeros is None else zeros.data_ptr(), out.data_ptr(), n, m, n, k,
-                            group, parts, None if room is None else room.data_ptr(),
-                            torch.cuda.current_stream(x.device).cuda_stream)
+    room = torch.empty((parts, m, n), dtype=torch.float32, device=dev) if parts > 1 else None
+    rc = _lib().tkv_gemv_w4(dev.index, dtype is torch.float16, x.data_ptr(), ldx, codes.data_ptr(), scales.data_ptr(),
+                            None if zeros is None else zeros.data_ptr(), out.data_ptr(), n, m, n, k, group, parts,
+                            None if room is None else room.data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
     if rc != 0:
         raise GemvError(_lib().tkv_last_error().decode())
     return out

@@ -10,13 +10,14 @@ waits for it here, and both directions can be captured into a graph.
 """
 
 import ctypes
-from typing import Any, Tuple
+import math
+import struct
 
 from .native import NativeUnavailable, load
 
-TILE = 256  # vocabulary entries and tokens of a tile
+TILE = 256  # vocabulary entries and tokens of a large tile
+SMALL_M, SMALL_N = 128, 64  # of a small one
 DL_BYTES = 512 << 20  # the backward pass' 16-bit derivative of the logits, per piece
-DX_BYTES = 512 << 20  # fp32 partial sums of x's gradient, over the splits
 MAX_TARGETS = 1024  # ids of a token's list
 MAX_TOKENS = 1 << 20
 MAX_WIDTH = 1 << 16
@@ -28,18 +29,9 @@ class LossError(RuntimeError):
     pass
 
 
-_LL, _I, _F, _P = ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
-
-
-class _Args(ctypes.Structure):
-    """``struct tkl_args`` of ``csrc/tk_loss.hip``."""
-
-    _fields_ = ([(f, _LL) for f in ("n", "d", "v", "k", "ldx", "ldw", "ldg", "ignore", "piece", "splits")]
-                + [(f, _I) for f in ("dev", "f16", "distill", "reduction")] + [("temperature", _F), ("want", _I)]
-                + [(f, _P) for f in ("x", "w", "ids", "teacher", "grad", "loss", "xc", "lse", "zk", "p", "rowloss",
-                                     "rowmap", "posof", "count", "flag", "part", "wc", "dl", "dxpart", "factor", "dx",
-                                     "dw", "stream")])
-
+# struct tkl_args of csrc/tk_loss.hip: n d v k ldx ldw ldg ignore piece fill, dev f16 distill
+# reduction, temperature, want small, x w ids teacher grad loss kept room wc dx dw stream
+_ARGS = struct.Struct("@10q4if2i12P")
 
 _loaded = None
 
@@ -47,11 +39,15 @@ _loaded = None
 def _lib():
     global _loaded
     if _loaded is None:
+        from .native import require_torch_first
+
+        require_torch_first()
         lib = load("libtk_loss.so")
         lib.tkl_last_error.restype = ctypes.c_char_p
-        lib.tkl_forward.argtypes = [ctypes.POINTER(_Args)]
-        lib.tkl_backward.argtypes = [ctypes.POINTER(_Args)]
-        if lib.tkl_args_size() != ctypes.sizeof(_Args):
+        lib.tkl_kept_bytes.restype = lib.tkl_room_bytes.restype = ctypes.c_longlong
+        for call in (lib.tkl_forward, lib.tkl_backward, lib.tkl_kept_bytes, lib.tkl_room_bytes):
+            call.argtypes = [ctypes.c_char_p]
+        if lib.tkl_args_size() != _ARGS.size:
             raise NativeUnavailable("libtk_loss.so does not match ops/loss.py: run `python -m triton_kubernetes_amd.ops.build`")
         _loaded = lib
     return _loaded
@@ -68,48 +64,62 @@ def pieces(n: int, v: int) -> int:
     return _up(-(-v // -(-v // most)), TILE)
 
 
-def splits(n: int, d: int, piece: int) -> int:
-    """Into how many parts the vocabulary is split for x's gradient: enough tiles for 256
-    compute units, at least 512 entries a part, and no more than ``DX_BYTES`` of sums."""
-    tiles = -(-n // TILE) * -(-d // TILE)
-    return max(1, min(512 // tiles, piece // 512, DX_BYTES // (4 * n * _up(d, 64))))
+def small_products(n: int, d: int, v: int) -> int:
+    """Which products run in small tiles (bits 1: the logits, 2: x's gradient, 4: w's).
+
+    A large tile multiplies faster, a small one wastes less on few tokens and fills more
+    compute units.  Measured gain of a small tile over a large one, in us of a whole step at
+    bf16 (n x d x v), where the rules turn: logits, n 64 x 4096 x 32000 61, 128 37, 192 -2, 256 -26;
+    1024 x 512 x 1000 24.  x's gradient, 64 x 4096 x 32000 26, 128 7, 128 x 4096 x 131072 -70.
+    w's, 1024 x 512 x 1000 (8 large tiles) 22, 128 x 2048 x 32000 (1000) -7."""
+
+    def tiles(a, b):
+        return -(-a // TILE) * -(-b // TILE)
+
+    logits = n <= SMALL_N or tiles(n, v) <= 64 or (tiles(n, v) <= 128 and n <= 2 * SMALL_N)
+    dx = n <= SMALL_N or n * d * v <= 1 << 34
+    return logits | dx << 1 | (tiles(d, v) <= 128) << 2
 
 
-def _padded_weight(w) -> bool:
-    """Whether the kernels need a copy of ``w`` with padded rows."""
-    d = w.shape[1]
-    return bool(d % 8 or w.stride(0) % 8 or w.data_ptr() % 16)
+def fill(small: bool) -> int:
+    """Workgroups for x's gradient, among which the vocabulary is split where there are fewer tiles:
+    a large tile for each of the 256 compute units (more only cost joining: 2048 x 2048 x 65536,
+    472 us with 256, 516 with 512), or two small ones."""
+    return 512 if small else 256
 
 
-def _plain(w):
-    """``w`` with a row stride that the kernels take."""
-    return w if w.stride(1) == 1 and w.shape[1] <= w.stride(0) <= 1 << 21 else w.contiguous()
+def kept_bytes(n: int, d: int, lists: int) -> int:
+    """Of what the forward pass keeps for the backward pass; ``lists`` entries of a teacher."""
+    return 2 * n * _up(d, 64) + 20 * n + 8 + (8 * lists + 16 * n if lists else 0)
 
 
-class _Kept:
-    """Sizes, settings and the addresses of what the forward pass keeps for the backward pass."""
+def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, lists: int) -> int:
+    """Of the backward pass' workspace: the derivative of a piece's logits, fp32 sums of x's
+    gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors and
+    residuals."""
+    once = n * _up(d, 64)
+    tiles = groups * (SMALL_M * SMALL_N if small else TILE * TILE)
+    sums = max(once, min(piece // 512 * once, tiles)) if want & 1 else 0
+    return 2 * n * piece + 4 * sums + 4 * (n + 1) + (16 * n if lists else 4 * n)
 
-    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore")
 
-    def fields(self, a: _Args, slab) -> None:
-        """The addresses within ``slab``, one fp32 tensor that holds them all."""
-        at, n, k = slab.data_ptr(), self.n, self.k
-        for name, count in (("lse", n), ("rowloss", n), ("rowmap", n), ("posof", n), ("count", 1), ("zk", n * k),
-                            ("p", n * k if self.distill else 0), ("flag", n if self.distill else 0)):
-            setattr(a, name, at)
-            at += 4 * count
+def _weight(w):
+    """``w`` with a row stride that the kernels take, and room for a copy with padded rows where
+    they need one."""
+    import torch
 
-    def words(self) -> int:
-        return 4 * self.n + 1 + self.n * self.k + (self.n * (self.k + 1) if self.distill else 0)
+    v, d = w.shape
+    if w.stride(1) != 1 or not d <= w.stride(0) <= 1 << 21:
+        w = w.contiguous()
+    if d % 8 or w.stride(0) % 8 or w.data_ptr() % 16:
+        return w, torch.empty((v, _up(d, 64)), dtype=w.dtype, device=w.device)
+    return w, None
 
-    def args(self, device, f16: bool, slab) -> _Args:
-        import torch
 
-        a = _Args(n=self.n, d=self.d, v=self.v, k=self.k, ignore=self.ignore, distill=self.distill,
-                  reduction=self.reduction, temperature=self.temperature, f16=f16, dev=device.index,
-                  stream=torch.cuda.current_stream(device).cuda_stream)
-        self.fields(a, slab)
-        return a
+class _Plan:
+    """The sizes and settings of a call, from its forward to its backward pass."""
+
+    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore", "f16", "small", "lead")
 
 
 _function = None
@@ -122,111 +132,111 @@ def _autograd():
         return _function
     import torch
 
+    stream_of = torch._C._cuda_getCurrentRawStream
+
     class HeadLoss(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, x, w, ids, teacher, kept):
+        def forward(ctx, x, w, ids, teacher, plan):
             dev = x.device
-            f16 = x.dtype == torch.float16
-            lead = x.shape[:-1]
-            ctx.kept, ctx.lead = kept, lead
-            loss = torch.empty(lead if kept.reduction == 0 else (), dtype=torch.float32, device=dev)
-            if kept.n == 0 or kept.k == 0:  # nothing has a loss
+            n, d, v, k = plan.n, plan.d, plan.v, plan.k
+            ctx.plan = plan
+            loss = torch.empty(() if plan.reduction else plan.lead, dtype=torch.float32, device=dev)
+            if n == 0 or k == 0:  # nothing has a loss
                 ctx.save_for_backward(x, w)
                 return loss.zero_()
-            x = x.reshape(-1, kept.d)
+            if x.dim() != 2:
+                x = x.reshape(n, d)
             if x.stride(1) != 1:
                 x = x.contiguous()
-            plain = _plain(w)
-            dp = _up(kept.d, 64)
-            xc = torch.empty((kept.n, dp), dtype=x.dtype, device=dev)
-            slab = torch.empty(kept.words(), dtype=torch.float32, device=dev)
-            part = torch.empty(4 * -(-kept.v // TILE) * kept.n, dtype=torch.float32, device=dev)
-            a = kept.args(dev, f16, slab)
-            wc = torch.empty((kept.v, dp), dtype=w.dtype, device=dev) if _padded_weight(plain) else None
-            a.x, a.ldx, a.w, a.ldw, a.ids = x.data_ptr(), x.stride(0), plain.data_ptr(), plain.stride(0), ids.data_ptr()
-            a.teacher = teacher.data_ptr() if teacher is not None else None
-            a.wc = wc.data_ptr() if wc is not None else None
-            a.loss, a.xc, a.part = loss.data_ptr(), xc.data_ptr(), part.data_ptr()
-            if _lib().tkl_forward(ctypes.byref(a)) != 0:
+            plan.small = small_products(n, d, v)
+            plain, copy = _weight(w)
+            kept = torch.empty(kept_bytes(n, d, n * k if plan.distill else 0), dtype=torch.uint8, device=dev)
+            room = torch.empty(8 * n * -(-v // (SMALL_M if plan.small & 1 else TILE)), dtype=torch.uint8, device=dev)
+            args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
+                              plan.distill, plan.reduction, plan.temperature, 0, plan.small, x.data_ptr(),
+                              plain.data_ptr(), ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0,
+                              loss.data_ptr(), kept.data_ptr(), room.data_ptr(), 0 if copy is None else copy.data_ptr(),
+                              0, 0, stream_of(dev.index))
+            if _lib().tkl_forward(args) != 0:
                 raise LossError(_lib().tkl_last_error().decode())
-            ctx.save_for_backward(w, ids, xc, slab)
+            ctx.save_for_backward(w, ids, kept)
             return loss
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
-            kept = ctx.kept
-            want = (1 if ctx.needs_input_grad[0] else 0) | (2 if ctx.needs_input_grad[1] else 0)
-            if kept.n == 0 or kept.k == 0:
+            plan = ctx.plan
+            need = ctx.needs_input_grad
+            want = (1 if need[0] else 0) | (2 if need[1] else 0)
+            n, d, v, k = plan.n, plan.d, plan.v, plan.k
+            if n == 0 or k == 0:
                 x, w = ctx.saved_tensors
                 return (torch.zeros_like(x) if want & 1 else None, torch.zeros_like(w) if want & 2 else None, None, None,
                         None)
-            w, ids, xc, slab = ctx.saved_tensors
-            dev = xc.device
-            if kept.reduction == 0:
+            w, ids, kept = ctx.saved_tensors
+            dev = w.device
+            if not plan.reduction:
                 grad = grad.reshape(-1)
-            grad = grad.float()
-            plain = _plain(w)
-            dp = _up(kept.d, 64)
-            a = kept.args(dev, xc.dtype == torch.float16, slab)
-            a.want, a.piece = want, pieces(kept.n, kept.v)
-            a.splits = splits(kept.n, kept.d, a.piece)
-            a.grad, a.ldg = grad.data_ptr(), grad.stride(0) if kept.reduction == 0 else 0
-            a.w, a.ldw, a.ids, a.xc = plain.data_ptr(), plain.stride(0), ids.data_ptr(), xc.data_ptr()
-            wc = torch.empty((kept.v, dp), dtype=w.dtype, device=dev) if _padded_weight(plain) else None
-            a.wc = wc.data_ptr() if wc is not None else None
-            dl = torch.empty((kept.n, a.piece), dtype=xc.dtype, device=dev)
-            factor = torch.empty(kept.n + 1, dtype=torch.float32, device=dev)
-            a.dl, a.factor = dl.data_ptr(), factor.data_ptr()
-            dx = dw = None
-            if want & 1:
-                dxpart = torch.empty((a.splits, kept.n, dp), dtype=torch.float32, device=dev)
-                dx = torch.empty((kept.n, kept.d), dtype=xc.dtype, device=dev)
-                a.dxpart, a.dx = dxpart.data_ptr(), dx.data_ptr()
-            if want & 2:
-                dw = torch.empty((kept.v, kept.d), dtype=xc.dtype, device=dev)
-                a.dw = dw.data_ptr()
-            if want and _lib().tkl_backward(ctypes.byref(a)) != 0:
+            if grad.dtype != torch.float32:
+                grad = grad.float()
+            plain, copy = _weight(w)
+            piece = pieces(n, v)
+            groups = fill(bool(plan.small & 2))
+            room = torch.empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill),
+                               dtype=torch.uint8, device=dev)
+            dx = torch.empty((n, d), dtype=w.dtype, device=dev) if want & 1 else None
+            dw = torch.empty((v, d), dtype=w.dtype, device=dev) if want & 2 else None
+            args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
+                              piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
+                              want, plan.small, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
+                              kept.data_ptr(), room.data_ptr(), 0 if copy is None else copy.data_ptr(),
+                              0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                              stream_of(dev.index))
+            if want and _lib().tkl_backward(args) != 0:
                 raise LossError(_lib().tkl_last_error().decode())
-            return None if dx is None else dx.view(*ctx.lead, kept.d), dw, None, None, None
+            if dx is not None and plan.lead != (n,):
+                dx = dx.view(*plan.lead, d)
+            return dx, dw, None, None, None
 
     _function = HeadLoss
     return _function
 
 
-def _check(what: str, x, w, reduction: str) -> Tuple[Any, _Kept]:
+def _check(what: str, x, w, reduction: str) -> _Plan:
     import torch
 
-    from .native import require_torch_first
-
-    require_torch_first()
-    if x.dtype not in (torch.bfloat16, torch.float16) or w.dtype != x.dtype:
+    dtype = x.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or w.dtype is not dtype:
         raise LossError(f"{what} wants x and w both bf16 or both fp16, not {x.dtype} and {w.dtype}")
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+    shape = x.shape
+    if len(shape) < 1 or w.dim() != 2 or shape[-1] != w.shape[1]:
         raise LossError(f"{what} wants x [..., D] and w [V, D], not {list(x.shape)} and {list(w.shape)}")
-    if not (x.is_cuda and w.is_cuda) or x.device != w.device:
+    if not x.is_cuda or x.device != w.device:
         raise LossError(f"{what} wants CUDA tensors on one device, not {x.device} and {w.device}")
     if reduction not in REDUCTIONS:
         raise LossError(f"unknown reduction '{reduction}' ({' | '.join(REDUCTIONS)})")
-    kept = _Kept()
-    kept.v, kept.d = w.shape
-    kept.n = x.numel() // kept.d if kept.d else 0
-    kept.reduction = REDUCTIONS[reduction]
-    if not (1 <= kept.d <= MAX_WIDTH and 1 <= kept.v <= MAX_VOCAB and kept.n <= MAX_TOKENS):
-        raise LossError(f"{what}: {kept.n} tokens of width {kept.d} over {kept.v} entries (at most {MAX_TOKENS}, "
+    plan = _Plan()
+    plan.v, plan.d = w.shape
+    plan.lead = shape[:-1]
+    plan.n = plan.lead.numel()
+    plan.reduction = REDUCTIONS[reduction]
+    plan.f16 = dtype is torch.float16
+    if not (1 <= plan.d <= MAX_WIDTH and 1 <= plan.v <= MAX_VOCAB and plan.n <= MAX_TOKENS):
+        raise LossError(f"{what}: {plan.n} tokens of width {plan.d} over {plan.v} entries (at most {MAX_TOKENS}, "
                         f"{MAX_WIDTH}, {MAX_VOCAB})")
-    return x, kept
+    return plan
 
 
-_INTEGERS = ("int64", "int32", "int16", "uint8", "int8")
+_INTEGERS = ("torch.int64", "torch.int32", "torch.int16", "torch.uint8", "torch.int8")
 
 
 def _ids(what: str, name: str, ids, x, dims: int):
     import torch
 
-    if str(ids.dtype).replace("torch.", "") not in _INTEGERS or ids.device != x.device:
+    if ids.dtype is not torch.int64 and str(ids.dtype) not in _INTEGERS or ids.device != x.device:
         raise LossError(f"{what} wants {name} as integers on x's device, not {ids.dtype} on {ids.device}")
-    if ids.dim() != x.dim() - 1 + dims or ids.shape[:x.dim() - 1] != x.shape[:-1]:
+    lead = x.shape[:-1]
+    if ids.dim() != len(lead) + dims or ids.shape[:len(lead)] != lead:
         raise LossError(f"{what}: {name} {list(ids.shape)} does not go with x {list(x.shape)}")
     return ids.to(torch.int64).contiguous()
 
@@ -240,10 +250,10 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
     holds; a target outside the vocabulary gives that token a NaN loss (and NaN gradients).
     ``reduction`` is ``mean`` over the tokens that count (0 if none does), ``sum``, or
     ``none`` for a loss per token.  Gradients flow to ``x`` and ``w``, once."""
-    x, kept = _check("linear_cross_entropy", x, w, reduction)
+    plan = _check("linear_cross_entropy", x, w, reduction)
     ids = _ids("linear_cross_entropy", "target", target, x, 0)
-    kept.k, kept.distill, kept.temperature, kept.ignore = 1, 0, 1.0, int(ignore_index)
-    return _autograd().apply(x, w, ids, None, kept)
+    plan.k, plan.distill, plan.temperature, plan.ignore = 1, 0, 1.0, int(ignore_index)
+    return _autograd().apply(x, w, ids, None, plan)
 
 
 def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean"):
@@ -257,12 +267,10 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     in no sum.  An entry listed twice counts twice.  An id past the vocabulary makes the
     token's loss NaN.  ``x``, ``w`` and ``reduction`` are those of
     :func:`linear_cross_entropy`."""
-    import math
-
     import torch
 
     what = "linear_distill"
-    x, kept = _check(what, x, w, reduction)
+    plan = _check(what, x, w, reduction)
     ids = _ids(what, "ids", ids, x, 1)
     if not logits.is_floating_point() or logits.device != x.device or logits.shape != ids.shape:
         raise LossError(f"{what} wants logits as numbers of ids' shape on x's device, not {logits.dtype} "
@@ -274,5 +282,5 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     temperature = float(temperature)
     if not (math.isfinite(temperature) and temperature > 0):
         raise LossError(f"{what}: the temperature must be above 0, not {temperature}")
-    kept.k, kept.distill, kept.temperature, kept.ignore = ids.shape[-1], 1, temperature, 0
-    return _autograd().apply(x, w, ids, logits.detach().float().contiguous(), kept)
+    plan.k, plan.distill, plan.temperature, plan.ignore = ids.shape[-1], 1, temperature, 0
+    return _autograd().apply(x, w, ids, logits.detach().float().contiguous(), plan)
