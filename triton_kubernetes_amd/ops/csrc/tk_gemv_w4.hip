@@ -166,8 +166,8 @@ struct Scales {
   }
 };
 
-// One row of x.  WN tiles of 16 rows of W a workgroup, WK waves to a tile, which share its
-// columns.
+// One row of x (blockIdx.y).  WN tiles of 16 rows of W a workgroup, WK waves to a tile, which
+// share its columns.
 //
 // The codes go to LDS by copies without registers, a stage of 16 rows x 256 bytes (4 chunks of
 // 128 columns) at a time and wave, two stages in flight: 16 neighbouring lanes read 256 bytes of
@@ -183,16 +183,18 @@ struct Scales {
 constexpr int STAGE = 4, STAGES = 2, STAGE_BYTES = 16 * STAGE * CHUNK / 2, SEGMENT = 256;
 
 template <bool F16, int G, bool ZEROS, int WN, int WK>
-__global__ __launch_bounds__(64 * WN * WK) void k_one(const void* __restrict__ x, const uint8_t* __restrict__ codes,
+__global__ __launch_bounds__(64 * WN * WK) void k_one(const void* __restrict__ xs_in, long long ldx,
+                                                      const uint8_t* __restrict__ codes,
                                                       const void* __restrict__ scales,
-                                                      const uint8_t* __restrict__ zeros, void* __restrict__ y, int n,
-                                                      int k, int group, int seg) {
+                                                      const uint8_t* __restrict__ zeros, void* __restrict__ y,
+                                                      long long ldy, int n, int k, int group, int seg) {
   using Y = Type<F16>;
   using T = typename Y::T;
   using Sc = Scales<F16, G, ZEROS>;
   constexpr int STEPS = 4 / Sc::SPC, THREADS = 64 * WN * WK;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   u32x4* xs = reinterpret_cast<u32x4*>(smem + WN * WK * STAGES * STAGE_BYTES);
+  const T* x = static_cast<const T*>(xs_in) + blockIdx.y * ldx;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave % WK, wn = wave / WK, j = lane >> 4, r = lane & 15;
   const int row0 = (blockIdx.x * WN + wn) * 16, row = row0 + r, groups = k / group, per_group = group / CHUNK;
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(64 * WN * WK) void k_one(const void* __restrict__ x
       for (int i = 0; i < 4; ++i) {
         const int unit = u0 + i * THREADS, ks = first * CHUNK + unit * 8;
         v[i] = u32x4{0, 0, 0, 0};
-        if (unit < units && ks < k) v[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(x) + ks);
+        if (unit < units && ks < k) v[i] = *reinterpret_cast<const u32x4*>(x + ks);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -320,29 +322,30 @@ __global__ __launch_bounds__(64 * WN * WK) void k_one(const void* __restrict__ x
 #pragma unroll
     for (int o = 1; o < WK; ++o) total += sums[(wave + o) * 16 + r];
   }
-  if (j == 0 && row < n) static_cast<T*>(y)[row] = (T)total;
+  if (j == 0 && row < n) static_cast<T*>(y)[blockIdx.y * ldy + row] = (T)total;
 }
 
 template <bool F16, int G, bool ZEROS, int WN, int WK>
-hipError_t one_as(const void* x, const uint8_t* codes, const void* scales, const uint8_t* zeros, void* y, int n, int k,
-                  int group, hipStream_t s) {
+hipError_t one_as(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, void* y,
+                  long long ldy, int m, int n, int k, int group, hipStream_t s) {
   const int tiles = (n + 15) / 16, chunks = (k + CHUNK - 1) / CHUNK, seg = std::min(chunks, SEGMENT);
-  k_one<F16, G, ZEROS, WN, WK><<<(tiles + WN - 1) / WN, 64 * WN * WK, WN * WK * STAGES * STAGE_BYTES + seg * 256, s>>>(
-      x, codes, scales, zeros, y, n, k, group, seg);
+  const dim3 grid((tiles + WN - 1) / WN, m);
+  k_one<F16, G, ZEROS, WN, WK><<<grid, 64 * WN * WK, WN * WK * STAGES * STAGE_BYTES + seg * 256, s>>>(
+      x, ldx, codes, scales, zeros, y, ldy, n, k, group, seg);
   return hipGetLastError();
 }
 
 template <bool F16, int G, bool ZEROS>
-hipError_t one(const void* x, const uint8_t* codes, const void* scales, const uint8_t* zeros, void* y, int n, int k,
-               int group, hipStream_t s) {
-  const int tiles = (n + 15) / 16;
+hipError_t one(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, void* y,
+               long long ldy, int m, int n, int k, int group, hipStream_t s) {
+  const int tiles = (n + 15) / 16 * m;  // over all rows of x
   const int chunks = (k + CHUNK - 1) / CHUNK;
   // Enough tiles for every compute unit: one wave a tile, and 4 tiles share what is read of x
   // (32768 x 4096: 17.4 us, 20.2 with 4 waves a tile).  Fewer: 4 waves a tile (4096 x 4096: 6.0
   // and 9.9 us), or 8 where the columns are long (4096 x 16384: 12.2 us, 13.5 with 4).
-  if (tiles >= 2048) return one_as<F16, G, ZEROS, 4, 1>(x, codes, scales, zeros, y, n, k, group, s);
-  if (tiles > 256 || chunks < 96) return one_as<F16, G, ZEROS, 1, 4>(x, codes, scales, zeros, y, n, k, group, s);
-  return one_as<F16, G, ZEROS, 1, 8>(x, codes, scales, zeros, y, n, k, group, s);
+  if (tiles >= 2048) return one_as<F16, G, ZEROS, 4, 1>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, s);
+  if (tiles > 256 || chunks < 96) return one_as<F16, G, ZEROS, 1, 4>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, s);
+  return one_as<F16, G, ZEROS, 1, 8>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, s);
 }
 
 // 2 to 64 rows of x, in MT tiles of 16.  8 waves a workgroup, RT tiles of 16 rows of W each, all
@@ -550,8 +553,8 @@ hipError_t batch_as(const void* x, long long ldx, const uint8_t* codes, const vo
 
 template <bool F16, int G, bool ZEROS>
 hipError_t run(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, void* y,
-               long long ldy, int m, int n, int k, int group, int splits, float* part, hipStream_t s) {
-  if (m == 1) return one<F16, G, ZEROS>(x, codes, scales, zeros, y, n, k, group, s);
+               long long ldy, int m, int n, int k, int group, int splits, float* part, bool each, hipStream_t s) {
+  if (each) return one<F16, G, ZEROS>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, s);
   if (m <= 16) return batch_as<F16, G, ZEROS, 1, 1>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, s);
   if (m <= 32) return batch_as<F16, G, ZEROS, 2, 2>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, s);
   return batch_as<F16, G, ZEROS, 4, 2>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, s);
@@ -559,11 +562,11 @@ hipError_t run(const void* x, long long ldx, const uint8_t* codes, const void* s
 
 template <bool F16>
 hipError_t launch(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros,
-                  void* y, long long ldy, int m, int n, int k, int group, int splits, float* part, hipStream_t s) {
+                  void* y, long long ldy, int m, int n, int k, int group, int splits, float* part, bool each, hipStream_t s) {
   const int g = group % CHUNK == 0 ? 1 : k < CHUNK ? 0 : group == 64 ? 2 : group == 32 ? 4 : 0;
 #define RUN(G)                                                                                                \
-  (zeros ? run<F16, G, true>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, s)           \
-         : run<F16, G, false>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, s))
+  (zeros ? run<F16, G, true>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, each, s)     \
+         : run<F16, G, false>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, each, s))
   return g == 1 ? RUN(1) : g == 2 ? RUN(2) : g == 4 ? RUN(4) : RUN(0);
 #undef RUN
 }
@@ -577,8 +580,8 @@ int refuse(const char* why) {
 
 // y[m][n] = x[m][k] W^T, queued on `stream` of device `dev`; nothing waits for it.  codes
 // [n][k/2] (the lower half of a byte first), scales [n][k/group] of x's type, zeros
-// [n][k/group] bytes or null for 8.  More than one row of x may split the columns: `part` holds
-// splits x m x n fp32 sums.  0, or -1 / a HIP error with tkv_last_error() set.
+// [n][k/group] bytes or null for 8.  splits 0: each row of x by itself, k_one; else together,
+// k_batch, the columns split, and `part` holds splits x m x n fp32 sums.  0, or -1 / a HIP error with tkv_last_error() set.
 extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const void* codes, const void* scales,
                            const void* zeros, void* y, long long ldy, int m, int n, int k, int group, int splits,
                            void* part, void* stream) {
@@ -589,7 +592,8 @@ extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const
   if (ldx < k || (ldx & 7) || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(codes) & 15))
     return refuse("rows of x and of the codes must be 16-byte aligned");
   if (ldy < n) return refuse("y's row stride is below its width");
-  if (splits < 1 || splits > 64 || (splits > 1 && !part)) return refuse("1 to 64 splits, with room for their sums");
+  if (splits < 0 || splits > 64 || (splits > 1 && !part)) return refuse("0 to 64 splits, with room for their sums");
+  if (splits == 0 && m > 64) return refuse("1 to 64 rows of x");
   int prev = 0;
   hipError_t e = hipGetDevice(&prev);
   if (e == hipSuccess && prev != dev) e = hipSetDevice(dev);
@@ -597,8 +601,8 @@ extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const
     const auto s = static_cast<hipStream_t>(stream);
     const auto *c = static_cast<const uint8_t*>(codes), *z = static_cast<const uint8_t*>(zeros);
     float* p = static_cast<float*>(part);
-    e = f16 ? launch<true>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, s)
-            : launch<false>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, s);
+    e = f16 ? launch<true>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, splits == 0, s)
+            : launch<false>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, splits == 0, s);
     if (prev != dev) {
       const hipError_t back = hipSetDevice(prev);
       if (e == hipSuccess) e = back;

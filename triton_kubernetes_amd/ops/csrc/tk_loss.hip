@@ -69,7 +69,7 @@ struct tkl_args {
   const void *x, *w, *ids, *teacher, *grad;
   void *loss, *kept;           // kept: from forward to backward (struct Kept)
   void *room;                  // forward: the tiles' maxima and sums; backward: dl, sums of dX, factors
-  void *wc;                    // a padded copy of w, where w's rows are not 16-byte aligned
+  void *wc;                    // a padded copy of w, where w's rows are not 16-byte aligned; forward makes it
   void *dx, *dw;
   void* stream;
 };
@@ -84,14 +84,14 @@ constexpr int FEW_ROWS = 512;
 
 // The two tilings of the matrix products.  A fragment is 16 x 16; a lane of a wave holds rows
 // row(mf) + (lane / 16) * 4 + 0..3 and column col(nf) + lane % 16 of fragment (mf, nf).
-struct Big {  // 8 waves, the schedule of product<Big>
-  static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2, LDS = 8 * 128 * KT * 2;
+struct Big {  // 8 waves, the schedule of product_big
+  static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2, LDS = 256 * (256 * 2 + 16);  // of the tile on its way out; the steps take 128 KiB
   static __device__ __forceinline__ int wave_m(int wid) { return wid >> 2; }
   static __device__ __forceinline__ int row(int mf, int wid) { return (mf >> 2) * 128 + (wid >> 2) * 64 + (mf & 3) * 16; }
   static __device__ __forceinline__ int col(int nf, int wid) { return (nf >> 1) * 128 + (wid & 3) * 32 + (nf & 1) * 16; }
   static __device__ __forceinline__ bool owns(int col, int wid) { return (col >> 5 & 3) == (wid & 3); }
 };
-struct Small {  // 4 waves, three steps in LDS: for few tokens, two workgroups to a compute unit
+struct Small {  // 4 waves, STEPS steps in LDS, two workgroups to a compute unit: for few tokens
   static constexpr int BM = 128, BN = 64, THREADS = 256, MF = 2, NF = 4, WAVES_M = 4, STEPS = 3,
                        LDS = STEPS * (BM + BN) * KT * 2;
   static __device__ __forceinline__ int wave_m(int wid) { return wid; }
@@ -284,44 +284,54 @@ __device__ __forceinline__ void clear(Acc<Tile>& acc) {
     for (int j = 0; j < Tile::NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// Three steps in LDS, one barrier a step: while a step is multiplied the next two are on their
-// way.
+// Three steps in LDS: while one is multiplied the next two are on their way.  (Six steps and one
+// workgroup to a compute unit took as long at 1 x 4096 x 4096, 24 us.)
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
 template <bool F16, bool AA, bool BA>
-__device__ __forceinline__ void product(Acc<Small>& acc, char* smem, const PanelA<Small, AA>& pa,
-                                        const PanelB<Small, BA>& pb, int nk, int tid) {
-  clear<Small>(acc);
+__device__ __forceinline__ void product_small(f32x4 (&acc)[2][4], char* smem, const Panel<AA, 128, 256>& pa,
+                                              const Panel<BA, 64, 256>& pb, int nk, int tid) {
+  using Tile = Small;
+  clear<Tile>(acc);
   if (nk <= 0) return;
-  constexpr int BYTES = (Small::BM + Small::BN) * KT * 2, AB = Small::BM * KT * 2;
-  constexpr int COPIES = PanelA<Small, AA>::COPIES + PanelB<Small, BA>::COPIES;
+  constexpr int BYTES = (Tile::BM + Tile::BN) * KT * 2, AB = Tile::BM * KT * 2, DEPTH = Tile::STEPS;
+  constexpr int COPIES = Panel<AA, 128, 256>::COPIES + Panel<BA, 64, 256>::COPIES;
   const int lane = tid & 63, wid = tid >> 6;
   const unsigned lds0 = lds_of(smem) + __builtin_amdgcn_readfirstlane(wid) * 64 * 16;
   auto stage = [&](int t) {
-    const unsigned dst = lds0 + t % Small::STEPS * BYTES;
+    const unsigned dst = lds0 + t % DEPTH * BYTES;
     pa.stage(t, 0, dst);
     pb.stage(t, 0, dst + AB);
   };
-  stage(0);
-  if (nk > 1) stage(1);
-  for (int t = 0; t < nk; ++t) {
-    if (t + 1 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(COPIES) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    barrier();  // step t is there for every wave, and step t - 1 has been read
-    if (t + 2 < nk) stage(t + 2);
-    const char *ia = smem + t % Small::STEPS * BYTES, *ib = ia + AB;
-    u32x4 a[Small::MF][2], b[Small::NF][2];
+  auto step = [&](int t) {
+    const char *ia = smem + t % DEPTH * BYTES, *ib = ia + AB;
+    u32x4 a[2][2], b[4][2];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-      for (int i = 0; i < Small::MF; ++i) a[i][kk] = PanelA<Small, AA>::frag(ia, Small::row(i, wid), kk, lane);
+      for (int i = 0; i < 2; ++i) a[i][kk] = Panel<AA, 128, 256>::frag(ia, Tile::row(i, wid), kk, lane);
 #pragma unroll
-      for (int j = 0; j < Small::NF; ++j) b[j][kk] = PanelB<Small, BA>::frag(ib, Small::col(j, wid), kk, lane);
+      for (int j = 0; j < 4; ++j) b[j][kk] = Panel<BA, 64, 256>::frag(ib, Tile::col(j, wid), kk, lane);
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-      for (int i = 0; i < Small::MF; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < Small::NF; ++j) acc[i][j] = Type<F16>::mfma(a[i][kk], b[j][kk], acc[i][j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = Type<F16>::mfma(a[i][kk], b[j][kk], acc[i][j]);
+  };
+#pragma unroll
+  for (int t = 0; t < DEPTH - 1; ++t)
+    if (t < nk) stage(t);
+  for (int t = 0; t < nk; ++t) {
+    // step t is there: younger are the DEPTH - 2 behind it, if they exist
+    if (t + DEPTH - 1 <= nk) wait_copies<COPIES * (DEPTH - 2)>();
+    else wait_copies<0>();
+    barrier();  // for every wave, and the step before it has been read
+    if (t + DEPTH - 1 < nk) stage(t + DEPTH - 1);
+    step(t);
   }
 }
 
@@ -330,7 +340,7 @@ __device__ __forceinline__ void product(Acc<Small>& acc, char* smem, const Panel
 // run one barrier apart, so that on every SIMD one wave feeds the matrix pipe while the other
 // reads LDS and issues copies.
 template <bool F16, bool AA, bool BA>
-__device__ __forceinline__ void product(Acc<Big>& acc, char* smem, const PanelA<Big, AA>& pa,
+__device__ __forceinline__ void product_big(Acc<Big>& acc, char* smem, const PanelA<Big, AA>& pa,
                                         const PanelB<Big, BA>& pb, int nk, int tid) {
   constexpr int HBYTES = 128 * KT * 2;
   const int lane = tid & 63, wid = tid >> 6, wr = wid >> 2, wc = wid & 3;
@@ -440,6 +450,13 @@ __device__ __forceinline__ void product(Acc<Big>& acc, char* smem, const PanelA<
   if (wr == 0) barrier();  // the other group's extra barrier
 }
 
+template <class Tile, bool F16, bool AA, bool BA>
+__device__ __forceinline__ void multiply(Acc<Tile>& acc, char* smem, const PanelA<Tile, AA>& pa,
+                                         const PanelB<Tile, BA>& pb, int nk, int tid) {
+  if constexpr (Tile::BM == 256) product_big<F16, AA, BA>(acc, smem, pa, pb, nk, tid);
+  else product_small<F16, AA, BA>(acc, smem, pa, pb, nk, tid);
+}
+
 // (m, s) of a softmax: maximum and sum of exp2(. - m).  An empty side has m = -inf, s = 0.
 __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
@@ -447,6 +464,36 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   s = s * a + s2 * b;
   m = top;
 }
+
+// A tile on its way out: column c of it is a row of the matrix, BM numbers of 16 bits, which go
+// through LDS so that 16 (or 32) lanes store a whole row 16 bytes each.  (Straight out of the
+// fragments, 4 lanes to 32 bytes of a row: 427 us for 388 of the logits' derivative at
+// 1217 x 288 x 242340, 58 for 26 of w's gradient at 30 x 927 x 19663, whose rows start anywhere.)
+template <class Tile, typename T>
+struct Outgoing {
+  static constexpr int STRIDE = Tile::BM * 2 + 16, PER = Tile::BM / 8;
+  static_assert(Tile::BN * STRIDE <= Tile::LDS, "the tile fits");
+  static __device__ __forceinline__ void put(char* smem, int col, int row, float a, float b, float c, float d) {
+    *reinterpret_cast<u32x2*>(smem + col * STRIDE + row * 2) = u32x2{pack2<T>(a, b), pack2<T>(c, d)};
+  }
+  // rows first .. first + count of `out`, from column c0 on, `width` of them
+  static __device__ __forceinline__ void store(const char* smem, T* out, long long ld, long long first, int count, int c0,
+                                               int width, int tid) {
+    for (int i = tid; i < count * PER; i += Tile::THREADS) {
+      const int r = i / PER, c = i % PER * 8;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(smem + r * STRIDE + c * 2);
+      T* to = out + (first + r) * ld + c0 + c;
+      if (c + 8 <= width) __builtin_memcpy(to, &v, 16);  // at any alignment
+      else if (c < width) {
+        typedef __attribute__((ext_vector_type(8))) T t8;
+        const t8 e = __builtin_bit_cast(t8, v);
+#pragma unroll
+        for (int o = 0; o < 8; ++o)
+          if (c + o < width) to[o] = e[o];
+      }
+    }
+  }
+};
 
 // What the derivative dl = factor (q - p) of a packed row's logits is multiplied with, and the
 // scale that the products are multiplied with afterwards, in 32 bits.  For the sum and the mean
@@ -501,7 +548,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
   const PanelA<Tile, true> pa(w, ldw, v0 + tv * Tile::BM, vend, 0, d, tid);
   const PanelB<Tile, true> pb(xc, ldxc, tn * Tile::BN, rows, 0, d, tid);
   Acc<Tile> acc;
-  product<F16, true, true>(acc, smem, pa, pb, (d + KT - 1) / KT, tid);
+  multiply<Tile, F16, true, true>(acc, smem, pa, pb, (d + KT - 1) / KT, tid);
 
   const int vb = tv * Tile::BM + fq * 4;  // the lane's entries are vb + row(i) + 0..3, in the piece
   const int vn = vend - v0;
@@ -542,13 +589,13 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
       part[(size_t)tv * n + token] = c;
     }
   } else {
+__syncthreads();  // LDS has been read
 #pragma unroll
     for (int j = 0; j < Tile::NF; ++j) {
       const int token = tn * Tile::BN + Tile::col(j, wid) + fr;
-      if (token >= rows) continue;
-      const float f = up.of(token), ls = lse[token];
-      const int target = targets ? targets[token] - v0 - vb : -1;
-      T* out = static_cast<T*>(dl) + (size_t)token * lddl + vb;
+      const bool there = token < rows;
+      const float f = there ? up.of(token) : 0.f, ls = there ? lse[token] : 0.f;
+      const int target = there && targets ? targets[token] - v0 - vb : -1;
 #pragma unroll
       for (int i = 0; i < Tile::MF; ++i) {
         const int at = Tile::row(i, wid);
@@ -568,9 +615,12 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
           for (int e = 0; e < 4; ++e)
             if (vb + at + e >= vn) g[e] = 0.f;  // zeros pad the piece
         }
-        *reinterpret_cast<u32x2*>(out + Tile::row(i, wid)) = u32x2{pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3])};
+        Outgoing<Tile, T>::put(smem, Tile::col(j, wid) + fr, at + fq * 4, g[0], g[1], g[2], g[3]);
       }
     }
+    __syncthreads();
+    Outgoing<Tile, T>::store(smem, static_cast<T*>(dl), lddl, tn * Tile::BN, min(Tile::BN, rows - tn * Tile::BN),
+                             tv * Tile::BM, Tile::BM, tid);
   }
 }
 
@@ -604,7 +654,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w
   const PanelA<Tile, false> pa(w, ldw, td * Tile::BM, d, v0 + k0, k, tid);
   const PanelB<Tile, true> pb(dl, lddl, tn * Tile::BN, rows, k0, (k + 7) & ~7, tid);  // dl is padded with zeros
   Acc<Tile> acc;
-  product<F16, false, true>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  multiply<Tile, F16, false, true>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
   out += (size_t)split * rows * dp;
 #pragma unroll
   for (int j = 0; j < Tile::NF; ++j) {
@@ -639,7 +689,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
   const PanelA<Tile, false> pa(xc, ldxc, td * Tile::BM, (int)(ldxc / 2), 0, rows, tid);
   const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), 0, rows, tid);
   Acc<Tile> acc;
-  product<F16, false, false>(acc, smem, pa, pb, (rows + KT - 1) / KT, tid);
+  multiply<Tile, F16, false, false>(acc, smem, pa, pb, (rows + KT - 1) / KT, tid);
 
   // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
   // share of the packed rows, in order; beyond ROOM of them a sum has so many targets that their
@@ -708,25 +758,18 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
     }
   }
   const float sc = up.scale();
-  const bool wide = (lddw & 3) == 0 && (reinterpret_cast<uintptr_t>(dw) & 7) == 0;
+  __syncthreads();  // LDS has been read
 #pragma unroll
-  for (int j = 0; j < Tile::NF; ++j) {
-    const int row = tv * Tile::BN + Tile::col(j, wid) + (lane & 15);
-    if (row >= vn) continue;
-    T* out = static_cast<T*>(dw) + (size_t)(v0 + row) * lddw;
+  for (int j = 0; j < Tile::NF; ++j)
 #pragma unroll
     for (int i = 0; i < Tile::MF; ++i) {
-      const int c = td * Tile::BM + Tile::row(i, wid) + (lane >> 4) * 4;
       const f32x4 r = rows ? acc[i][j] * sc : f32x4{0.f, 0.f, 0.f, 0.f};
-      if (wide && c + 4 <= d) {
-        *reinterpret_cast<u32x2*>(out + c) = u32x2{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3])};
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < d) out[c + e] = (T)r[e];
-      }
+      Outgoing<Tile, T>::put(smem, Tile::col(j, wid) + (lane & 15), Tile::row(i, wid) + (lane >> 4) * 4, r[0], r[1], r[2],
+                             r[3]);
     }
-  }
+  __syncthreads();
+  Outgoing<Tile, T>::store(smem, static_cast<T*>(dw), lddw, v0 + tv * Tile::BN, min(Tile::BN, vn - tv * Tile::BN),
+                           td * Tile::BM, d - td * Tile::BM, tid);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -802,7 +845,6 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
     count[1] = 0;
   }
   for (int i = 0; i < wave * 2; ++i) pos += kept[i];
-  const bool wide = (d & 7) == 0 && (ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   for (int i = wave * 2; i < wave * 2 + 2; ++i) {
     const int r = row0 + i;
     if (r >= n) break;
@@ -815,13 +857,13 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
     }
     T* out = xc + (size_t)pos * dp;
     const T* in = x + (long long)r * ldx;
-    if (wide) {
 #pragma unroll 4
-      for (int e = lane * 8; e < dp; e += 512)
-        *reinterpret_cast<u32x4*>(out + e) = e < d ? *reinterpret_cast<const u32x4*>(in + e) : u32x4{0, 0, 0, 0};
-    } else {
-      for (int e = lane; e < dp; e += 64) out[e] = e < d ? in[e] : (T)0.f;
+    for (int e = lane * 8; e + 8 <= d; e += 512) {
+      u32x4 v;
+      __builtin_memcpy(&v, in + e, 16);  // at any alignment
+      *reinterpret_cast<u32x4*>(out + e) = v;
     }
+    for (int e = (d & ~7) + lane; e < dp; e += 64) out[e] = e < d ? in[e] : (T)0.f;
     if (lane == 0) {
       rowmap[pos] = r;
       posof[r] = pos;
@@ -831,12 +873,27 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
 }
 
 // A copy of w with rows of dp elements, zeros behind d: for a w whose rows are not 16-byte
-// aligned, or whose width is no multiple of 8.
+// aligned, or whose width is no multiple of 8.  16 bytes a thread, read at any alignment.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pad(const T* __restrict__ w, long long ldw, long long rows, int d, int dp,
                                              T* __restrict__ out) {
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int e = threadIdx.x; e < dp; e += 256) out[r * dp + e] = e < d ? w[r * ldw + e] : (T)0.f;
+  const int per = dp / 8;
+  const long long all = rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+    const long long r = i / per;
+    const int e = (int)(i - r * per) * 8;
+    u32x4 v = {0, 0, 0, 0};
+    if (e + 8 <= d) {
+      __builtin_memcpy(&v, w + r * ldw + e, 16);
+    } else if (e < d) {
+      typedef __attribute__((ext_vector_type(8))) T t8;
+      t8 one;
+#pragma unroll
+      for (int o = 0; o < 8; ++o) one[o] = e + o < d ? w[r * ldw + e + o] : (T)0.f;
+      v = __builtin_bit_cast(u32x4, one);
+    }
+    *reinterpret_cast<u32x4*>(out + r * dp + e) = v;
+  }
 }
 
 // x . w[id] over `lanes` neighbouring lanes, the sum in all of them.  A target outside the
@@ -998,12 +1055,14 @@ __global__ __launch_bounds__(256) void k_fix(const long long* __restrict__ ids, 
                                              float* __restrict__ lost) {
   using T = typename Type<F16>::T;
   __shared__ int list[4][MAX_TARGETS];  // vocabulary entries, -1: none
+  __shared__ float prob[4][MAX_TARGETS];
   const int wave = threadIdx.x >> 6, pos = blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
   if (pos >= up.count[0]) return;
   const size_t row = (size_t)up.rowmap[pos] * k;
   for (int i = lane; i < k; i += 64) {
     const long long id = ids[row + i];
     list[wave][i] = id >= 0 && id < v ? (int)id : -1;
+    prob[wave][i] = p[row + i];
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list: no barrier
   const float f = up.of(pos), ls = lse[pos];
@@ -1012,12 +1071,12 @@ __global__ __launch_bounds__(256) void k_fix(const long long* __restrict__ ids, 
     const int i = i0 + lane, id = i < k ? list[wave][i] : -1;
     float sum = 0.f;
     bool firstone = id >= 0;
-    if (firstone)
-      for (int o = 0; o < k; ++o)
-        if (list[wave][o] == id) {
-          sum += p[row + o];
-          firstone &= o >= i;
-        }
+#pragma unroll 8
+    for (int o = 0; o < k; ++o) {
+      const bool same = list[wave][o] == id;
+      sum += same ? prob[wave][o] : 0.f;
+      firstone &= !same || o >= i;
+    }
     const float g = firstone ? __builtin_amdgcn_exp2f(zk[(size_t)pos * k + i] * sc - ls) - sum : 0.f;
     const unsigned long long mask = __ballot(fabsf(g) >= LARGE);
     const int slot = large + __popcll(mask & ((1ull << lane) - 1));
@@ -1065,8 +1124,9 @@ __global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, 
     s *= up.scale();
   }
   T* out = static_cast<T*>(dx) + (size_t)row * d + c;
-  if ((d & 3) == 0) {
-    *reinterpret_cast<u32x2*>(out) = u32x2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])};
+  if (c + 4 <= d) {
+    const u32x2 v = {pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])};
+    __builtin_memcpy(out, &v, 8);  // at any alignment
   } else {
     for (int e = 0; e < 4 && c + e < d; ++e) out[e] = (T)s[e];
   }
@@ -1195,16 +1255,23 @@ unsigned blocks(long long items, long long per) { return (unsigned)((items + per
 template <typename T>
 void pad(const tkl_args& a, int dp, hipStream_t s) {
   if (a.wc)
-    k_pad<T><<<(unsigned)std::min<long long>(a.v, 65536), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, a.v, (int)a.d,
+    k_pad<T><<<(unsigned)std::min<long long>(blocks(a.v * (dp / 8), 256), 16384), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, a.v, (int)a.d,
                                                                        dp, static_cast<T*>(a.wc));
 }
 
 template <class Tile, bool F16, bool DL>
-void logits(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
+void logits_as(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
             float* lost, hipStream_t s) {
   k_logits<Tile, F16, DL><<<blocks(vn, Tile::BM) * blocks(a.n, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
       w.at, w.ldb, kept.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, kept.count, (int)a.n, LOG2E / a.temperature,
       static_cast<float2*>(a.room), kept.lse, up, a.distill ? nullptr : kept.at, a.room, a.piece, lost);
+}
+
+template <bool F16, bool DL>
+void logits(const tkl_args& a, const Kept& q, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
+            float* lost, hipStream_t s) {
+  if (a.small & 1) logits_as<Small, F16, DL>(a, q, w, dp, v0, vn, up, lost, s);
+  else logits_as<Big, F16, DL>(a, q, w, dp, v0, vn, up, lost, s);
 }
 
 template <bool F16>
@@ -1223,8 +1290,7 @@ hipError_t forward(const tkl_args& a) {
   pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
   const T* wt = static_cast<const T*>(w.at);
-  if (a.small & 1) logits<Small, F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
-  else logits<Big, F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
+  logits<F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
   if (a.distill)
     k_dots<T><<<blocks((long long)n * k, 4), 256, 0, s>>>(xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count,
                                                           q.zk);
@@ -1252,7 +1318,6 @@ void dw(const tkl_args& a, const Kept& q, const Room& r, int dp, long long v0, i
 
 template <bool F16>
 hipError_t backward(const tkl_args& a) {
-  using T = typename Type<F16>::T;
   hipStream_t s = static_cast<hipStream_t>(a.stream);
   const int n = (int)a.n, d = (int)a.d, k = (int)a.k, dp = padded(a.d);
   const Kept q = kept_of(a);
@@ -1261,12 +1326,10 @@ hipError_t backward(const tkl_args& a) {
                             n, a.temperature};
   if (F16 && a.reduction == 0)
     k_factor<<<1, 1024, 0, s>>>(up.grad, up.ldg, up.rowmap, up.count, n, a.temperature, Upstream<F16>::SPAN, r.factor);
-  pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
   for (long long v0 = 0; v0 < a.v; v0 += a.piece) {
     const int vn = (int)std::min(a.piece, a.v - v0);
-    if (a.small & 1) logits<Small, F16, true>(a, q, w, dp, v0, vn, up, r.lost, s);
-    else logits<Big, F16, true>(a, q, w, dp, v0, vn, up, r.lost, s);
+    logits<F16, true>(a, q, w, dp, v0, vn, up, r.lost, s);
     if (a.distill)
       k_fix<F16><<<blocks(n, 4), 256, 0, s>>>(static_cast<const long long*>(a.ids), q.p, k, a.v, q.zk, q.lse, up,
                                               LOG2E / a.temperature, v0, vn, r.dl, a.piece, q.at, r.lost);

@@ -56,12 +56,16 @@ def _check_weight(codes, scales, zeros) -> Tuple[int, int, int]:
 
 
 def splits(m: int, n: int, k: int) -> int:
-    """Into how many parts ``k`` is split: a workgroup takes 128 rows of the weight (256 for more
-    than 16 rows of ``x``), and one for each of the 256 compute units is best (64 rows of ``x``,
-    16384 x 16384: 70 us; 104 with 128 of them, 84 with 512, whose sums cost more to join); a
-    part has at least 4 chunks of 128 columns.  For one row of ``x`` the waves of a workgroup share the columns instead."""
-    if m == 1:
-        return 1
+    """How the product is run: 0, each row of ``x`` by itself, or into how many parts ``k`` is split.
+
+    A row by itself is one launch and no join, and small weights come out of the cache for every
+    row (4 x 1024 x 4096: 5.6 us, 8.8 together; 16 rows 9.5 both ways; 4 x 4096 x 4096 10.6 and
+    10.3).  Together a workgroup takes 128 rows of the weight (256 for more than 16 rows of
+    ``x``), and one for each of the 256 compute units is best (64 rows of ``x``, 16384 x 16384:
+    70 us; 104 with 128 of them, 84 with 512, whose sums cost more to join); a part has at least
+    4 chunks of 128 columns."""
+    if m == 1 or m * n * k <= 1 << 26:
+        return 0
     blocks = -(-n // (128 if m <= 16 else 256))
     chunks = -(-k // 128)
     want = max(1, min(256 // blocks, chunks // 4, 64))

@@ -103,17 +103,20 @@ def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, 
     return 2 * n * piece + 4 * sums + 4 * (n + 1) + (16 * n if lists else 4 * n)
 
 
-def _weight(w):
-    """``w`` with a row stride that the kernels take, and room for a copy with padded rows where
-    they need one."""
+def _row_strided(w):
+    """``w`` with a row stride that the kernels take."""
+    return w if w.stride(1) == 1 and w.shape[1] <= w.stride(0) <= 1 << 21 else w.contiguous()
+
+
+def _room_for_copy(w):
+    """Room for a copy of ``w`` with padded rows, where the kernels need one (the forward pass makes
+    it, and keeps it for the backward pass)."""
     import torch
 
     v, d = w.shape
-    if w.stride(1) != 1 or not d <= w.stride(0) <= 1 << 21:
-        w = w.contiguous()
     if d % 8 or w.stride(0) % 8 or w.data_ptr() % 16:
-        return w, torch.empty((v, _up(d, 64)), dtype=w.dtype, device=w.device)
-    return w, None
+        return torch.empty((v, _up(d, 64)), dtype=w.dtype, device=w.device)
+    return None
 
 
 class _Plan:
@@ -149,7 +152,8 @@ def _autograd():
             if x.stride(1) != 1:
                 x = x.contiguous()
             plan.small = small_products(n, d, v)
-            plain, copy = _weight(w)
+            plain = _row_strided(w)
+            copy = _room_for_copy(plain)
             kept = torch.empty(kept_bytes(n, d, n * k if plan.distill else 0), dtype=torch.uint8, device=dev)
             room = torch.empty(8 * n * -(-v // (SMALL_M if plan.small & 1 else TILE)), dtype=torch.uint8, device=dev)
             args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
@@ -159,7 +163,7 @@ def _autograd():
                               0, 0, stream_of(dev.index))
             if _lib().tkl_forward(args) != 0:
                 raise LossError(_lib().tkl_last_error().decode())
-            ctx.save_for_backward(w, ids, kept)
+            ctx.save_for_backward(w, ids, kept, *(() if copy is None else (copy,)))
             return loss
 
         @staticmethod
@@ -173,13 +177,13 @@ def _autograd():
                 x, w = ctx.saved_tensors
                 return (torch.zeros_like(x) if want & 1 else None, torch.zeros_like(w) if want & 2 else None, None, None,
                         None)
-            w, ids, kept = ctx.saved_tensors
+            w, ids, kept, *copy = ctx.saved_tensors
             dev = w.device
             if not plan.reduction:
                 grad = grad.reshape(-1)
             if grad.dtype != torch.float32:
                 grad = grad.float()
-            plain, copy = _weight(w)
+            plain = copy[0] if copy else _row_strided(w)
             piece = pieces(n, v)
             groups = fill(bool(plan.small & 2))
             room = torch.empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill),
@@ -189,7 +193,7 @@ def _autograd():
             args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
                               piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
                               want, plan.small, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
-                              kept.data_ptr(), room.data_ptr(), 0 if copy is None else copy.data_ptr(),
+                              kept.data_ptr(), room.data_ptr(), copy[0].data_ptr() if copy else 0,
                               0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
                               stream_of(dev.index))
             if want and _lib().tkl_backward(args) != 0:
