@@ -190,3 +190,58 @@ def test_refusals_on_the_gpu():
             gemv.gemv_w4(*ok, out=out)
     with torch.no_grad():
         gemv.gemv_w4(x.clone().requires_grad_(), packed, scales, zero)
+
+
+def test_out_may_not_share_memory_with_what_is_read():
+    from triton_kubernetes_amd.ops import gemv
+
+    codes, scales, zero = _weight(128, 128, 64, torch.bfloat16, True, _gen(7))
+    packed = gemv.pack_w4(codes)
+    room = torch.zeros((5, 128), device="cuda", dtype=torch.bfloat16)
+    for x, out in ((room[:2], room[:2]), (room[:2], room[1:3]), (room[1:4:2], room[2:4])):
+        with pytest.raises(gemv.GemvError, match="share"):
+            gemv.gemv_w4(x, packed, scales, zero, out=out)
+    with pytest.raises(gemv.GemvError, match="share"):
+        gemv.gemv_w4(room[:2], packed, scales, zero, out=scales.view(-1)[:256].view(2, 128))
+    with pytest.raises(gemv.GemvError, match="no gradient"):
+        gemv.gemv_w4(room[:2], packed, scales, zero, out=torch.zeros_like(room[:2]).requires_grad_())
+    gemv.gemv_w4(room[:2], packed, scales, zero, out=room[2:4])
+
+
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 64])
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+def test_both_forms_of_few_rows_and_calls_at_once(m, dt, monkeypatch):
+    """Each row by itself and all together, split and whole, on small integers: the same bits; on
+    three streams at once."""
+    from triton_kubernetes_amd.ops import gemv
+
+    n, k, group = 530, 3200, 32
+    gen = _gen(8, m)
+    codes, scales, zero = _weight(n, k, group, dt, True, gen, exact=True)
+    packed = gemv.pack_w4(codes)
+    x = torch.randint(-2, 3, (m, k), device="cuda", generator=gen).to(dt)
+    want = (x.double() @ _true(codes, scales, zero).T).to(dt)
+    torch.cuda.synchronize()
+    got = []
+    for parts in (0, 1, 5):
+        monkeypatch.setattr(gemv, "splits", lambda *a, parts=parts: parts)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(gemv.gemv_w4(x, packed, scales, zero))
+    torch.cuda.synchronize()
+    for one in got:
+        assert torch.equal(one, want)
+
+
+def test_an_infinite_x_shows_in_its_row_alone(monkeypatch):
+    from triton_kubernetes_amd.ops import gemv
+
+    codes, scales, zero = _weight(100, 256, 64, torch.bfloat16, True, _gen(9))
+    packed = gemv.pack_w4(codes)
+    x = torch.ones((20, 256), device="cuda", dtype=torch.bfloat16)
+    bad = x.clone()
+    bad[7, 100] = float("inf")
+    keep = torch.arange(20, device="cuda") != 7
+    for parts in (0, 1):
+        monkeypatch.setattr(gemv, "splits", lambda *a, parts=parts: parts)
+        want, got = (gemv.gemv_w4(a, packed, scales, zero) for a in (x, bad))
+        assert torch.equal(got[keep], want[keep]) and bool(got[7].isnan().all())

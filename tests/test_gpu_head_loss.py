@@ -402,3 +402,152 @@ def test_long_offsets():
     for at, value in ((v - 2, 4 * (3 * q - 1)), (v - 1, 4 * (3 * rest - 1)), (0, 4 * (3 * rest - 1)), (7, 12 * rest)):
         assert abs(float(got[at]) - value) <= 3 * 2.0 ** -8 * 4, (at, float(got[at]), value)
     assert not bool(dw[:, 1:].any())
+
+
+@pytest.mark.parametrize("distill", [False, True], ids=["target", "teacher"])
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+def test_the_targets_derivative_is_not_rounded_for_few_tokens(dt, distill):
+    """One token: w's gradient at its target is (q - 1) x.  With q <= 2^-5 from a logit off by at most
+    2^-12, q - 1 is good to 2^-16, so that little but the result's own rounding is left of it
+    (a 16-bit q - 1 alone would be off by up to half a step more)."""
+    from triton_kubernetes_amd.ops.loss import linear_cross_entropy, linear_distill
+
+    d, v = 2048, 300
+    gen = _gen(21, int(distill))
+    x, w, t = _inputs(1, d, v, dt, gen, sure=0.0)
+    if distill:
+        call = lambda x, w: linear_distill(x, w, t[:, None], torch.zeros((1, 1), device="cuda"))  # noqa: E731
+    else:
+        call = lambda x, w: linear_cross_entropy(x, w, t)  # noqa: E731
+    _, _, dw = _run(call, x, w, None)
+    q = torch.softmax(x.double() @ w.double().T, 1)[0, t[0]]
+    assert float(q) <= 2.0 ** -5
+    true = (q - 1) * x.double()[0]
+    # (fp16 results under 2^-14 have absolute steps of 2^-24)
+    off = (dw[t[0]].double() - true).abs() - true.abs() * (ref.U[dt] + 2.0 ** -15) - 2.0 ** -25
+    assert float(off.max()) <= 0
+
+
+def test_a_teachers_list_of_the_lowest_value_is_uniform():
+    """A mask of fp32's lowest value, which a division by the temperature would turn into -inf."""
+    from triton_kubernetes_amd.ops.loss import linear_distill
+
+    gen = _gen(22)
+    x, w, t = _inputs(3, 64, 400, torch.bfloat16, gen)
+    ids = torch.stack((t, (t + 1) % 400), 1)
+    low = torch.finfo(torch.float32).min
+    logits = torch.tensor([[low, low], [0.0, low], [-float("inf"), low]], device="cuda")
+    for temp in (0.5, 1.0):
+        got = _run(lambda x, w: linear_distill(x, w, ids, logits, temperature=temp, reduction="none"), x, w,
+                   torch.ones(3, device="cuda"))
+        same = torch.tensor([[0.0, 0.0], [0.0, -1e4], [-float("inf"), 0.0]], device="cuda")
+        want = _run(lambda x, w: linear_distill(x, w, ids, same, temperature=temp, reduction="none"), x, w,
+                    torch.ones(3, device="cuda"))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+def test_many_tokens_with_gaps(monkeypatch):
+    """More tokens than two rows a wave pack, most of them masked; those that are left are the last
+    ones of a run, the first and the last token among them."""
+    from triton_kubernetes_amd.ops import loss
+    from triton_kubernetes_amd.ops.loss import linear_cross_entropy
+
+    # (the tiles go by all tokens, and small ones add the same numbers in another order)
+    monkeypatch.setattr(loss, "small_products", lambda *a: 0)
+    n, d, v = 100_003, 16, 40
+    gen = _gen(23)
+    x, w, t = _inputs(n, d, v, torch.bfloat16, gen)
+    keep = torch.rand(n, device="cuda", generator=gen) < 0.01
+    keep[[0, n - 1]] = True
+    t[~keep] = -100
+    loss, dx, dw = _run(lambda x, w: linear_cross_entropy(x, w, t, reduction="none"), x, w, torch.ones(n, device="cuda"))
+    few = _run(lambda x, w: linear_cross_entropy(x, w, t[keep], reduction="none"), x[keep], w,
+               torch.ones(int(keep.sum()), device="cuda"))
+    assert torch.equal(loss[keep], few[0]) and not bool(loss[~keep].any())
+    assert torch.equal(dx[keep], few[1]) and not bool(dx[~keep].any())
+    assert torch.equal(dw, few[2])
+
+
+def test_more_listed_entries_than_a_launch_has_waves():
+    from triton_kubernetes_amd.ops.loss import linear_distill
+
+    n, d, v, k = 65536, 8, 1024, 1024
+    gen = _gen(24)
+    x, w, _ = _inputs(n, d, v, torch.bfloat16, gen)
+    ids = torch.arange(k, device="cuda").expand(n, k)
+    logits = torch.randn((n, k), device="cuda", generator=gen)
+    loss = linear_distill(x, w, ids, logits, reduction="none")
+    at = torch.cat((torch.arange(300), torch.arange(n - 300, n))).to("cuda")
+    want = ref.head(x[at], w, ids[at], *[ref.teacher_of(ids[at], logits[at], 1.0)[1]], 1.0, torch.ones(600, device="cuda"))
+    ref.check("loss", loss[at], want[0])
+
+
+def test_a_weight_of_one_row_with_any_stride():
+    from triton_kubernetes_amd.ops.loss import linear_cross_entropy
+
+    gen = _gen(25)
+    x, w, t = _inputs(4, 64, 1, torch.bfloat16, gen)
+    lone = torch.empty((1, 128), device="cuda", dtype=w.dtype)
+    lone[:, ::2] = w
+    for other in (w[0].expand(1, 64), lone[:, ::2], lone[0, ::2].expand(1, 64)):
+        # the only entry there is: 0, but for the logit, which the kernels add up in two orders
+        _against(lambda x, w: linear_cross_entropy(x, w, t, reduction="none"), x, other, *ref.targets_of(t, -100, 4, 1),
+                 gen=gen)
+
+
+def test_capture_is_refused_while_an_eager_graph_of_the_same_leaves_lives():
+    """torch would leave the eager stream unjoined in the capture, which ends the process."""
+    from triton_kubernetes_amd.ops.loss import LossError, linear_cross_entropy
+
+    x, w, t = _inputs(40, 64, 300, torch.bfloat16, _gen(26))
+    x.requires_grad_()
+    w.requires_grad_()
+    alive = linear_cross_entropy(x, w, t)
+    for leaves in ((x, w), (x.detach(), w), (x, w.detach())):
+        with pytest.raises(LossError, match="eager graph"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            linear_cross_entropy(*leaves, t)
+    with torch.cuda.stream(torch.cuda.Stream()):  # another stream alone is no trouble
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        linear_cross_entropy(x, w, t)
+        torch.cuda.current_stream().synchronize()
+    want = torch.autograd.grad(alive, (x, w))
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(linear_cross_entropy(x, w, t), (x, w))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_first_call_of_a_process_may_be_a_captured_one():
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from triton_kubernetes_amd.ops.gemv import gemv_w4, pack_w4
+from triton_kubernetes_amd.ops.loss import linear_cross_entropy
+gen = torch.Generator(device="cuda").manual_seed(1)
+w = torch.randn((500, 128), device="cuda", generator=gen).bfloat16().requires_grad_()
+x = torch.randn((70, 128), device="cuda", generator=gen).bfloat16().requires_grad_()
+t = torch.randint(0, 500, (70,), device="cuda", generator=gen)
+codes = pack_w4(torch.randint(0, 16, (500, 128), device="cuda", generator=gen, dtype=torch.uint8))
+scales = torch.ones((500, 1), device="cuda", dtype=torch.bfloat16)
+def run():
+    loss = linear_cross_entropy(x, w, t)
+    return (loss.detach(), *torch.autograd.grad(loss, (x, w)), gemv_w4(x.detach()[:3], codes, scales),
+            gemv_w4(x.detach()[:40], codes, scales))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, run()))
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and done.stdout.strip().endswith("same"), done.stderr[-2000:]

@@ -62,7 +62,8 @@ def test_buffers_have_the_sizes_that_the_kernels_take(n, d, k):
     (dict(v=0), "vocabulary"), (dict(v=(1 << 24) + 1), "vocabulary"), (dict(k=0), "targets"), (dict(k=1025), "targets"),
     (dict(d=7), "aligned"), (dict(ldw=9), "aligned"), (dict(w=4098), "aligned"), (dict(ldw=0), "row stride"),
     (dict(ldw=1 << 22), "row stride"), (dict(reduction=3), "reduction"), (dict(temperature=0.0), "temperature"),
-    (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=float("nan")), "temperature"), (dict(n=1 << 20, v=1 << 19), "tokens x vocabulary"),
+    (dict(n=1 << 20, d=1 << 14, ldw=1 << 14), "tokens x width"),
 ])
 def test_the_c_entries_check_before_the_gpu(fields, message):
     lib = loss._lib()
@@ -71,7 +72,8 @@ def test_the_c_entries_check_before_the_gpu(fields, message):
         assert message in lib.tkl_last_error().decode()
 
 
-@pytest.mark.parametrize("fields", [dict(piece=0), dict(piece=255), dict(piece=1 << 25), dict(fill=0), dict(fill=4097)])
+@pytest.mark.parametrize("fields", [dict(piece=0), dict(piece=255), dict(piece=1 << 25), dict(fill=0), dict(fill=4097),
+                                    dict(n=300, piece=1 << 21)])
 def test_the_c_backward_checks_its_pieces(fields):
     assert loss._lib().tkl_backward(_args(**fields)) == -1
 
@@ -177,3 +179,14 @@ def test_tile_rules_at_their_corners():
     assert loss.small_products(1, 512, 1000) == 7 and loss.small_products(1024, 512, 1000) == 7
     assert loss.small_products(64, 4096, 131072) == 3 and loss.small_products(65, 4096, 131072) == 0
     assert loss.small_products(8192, 4096, 131072) == 0
+
+
+def test_a_group_whose_scale_is_as_small_as_the_type_has():
+    w = torch.zeros((2, 64), dtype=torch.bfloat16)
+    w[0, 3] = 2.0 ** -130  # the scale is subnormal in bf16, and 1 / scale no fp32 number
+    w[1] = 2.0 ** -130
+    for symmetric in (True, False):
+        codes, scales, zeros = gemv.quantize_w4(w, 32, symmetric)
+        back = gemv.dequantize_w4(codes, scales, zeros)
+        assert bool(torch.isfinite(back).all())
+        assert float((back - w.float()).abs().max()) <= 2.0 ** -133  # 8 steps of 2^-133, 7 of them reached

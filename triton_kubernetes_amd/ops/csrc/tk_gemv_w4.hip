@@ -180,14 +180,15 @@ struct Scales {
 // x goes through LDS a segment of `seg` chunks at a time, in the order that the codes unpack
 // to.  Columns behind k are zeros in x, so whatever codes are read there change nothing.  All 16
 // rows of the matrix instruction get the same x; the first one's sums are kept.
+//
+// The waits count what is in flight, so no load may move across the empty asm statements: the
+// pointers are not __restrict__, which would let the compiler do that.
 constexpr int STAGE = 4, STAGES = 2, STAGE_BYTES = 16 * STAGE * CHUNK / 2, SEGMENT = 256;
 
 template <bool F16, int G, bool ZEROS, int WN, int WK>
-__global__ __launch_bounds__(64 * WN * WK) void k_one(const void* __restrict__ xs_in, long long ldx,
-                                                      const uint8_t* __restrict__ codes,
-                                                      const void* __restrict__ scales,
-                                                      const uint8_t* __restrict__ zeros, void* __restrict__ y,
-                                                      long long ldy, int n, int k, int group, int seg) {
+__global__ __launch_bounds__(64 * WN * WK) void k_one(const void* xs_in, long long ldx, const uint8_t* codes,
+                                                      const void* scales, const uint8_t* zeros, void* y, long long ldy,
+                                                      int n, int k, int group, int seg) {
   using Y = Type<F16>;
   using T = typename Y::T;
   using Sc = Scales<F16, G, ZEROS>;
@@ -358,14 +359,13 @@ hipError_t one(const void* x, long long ldx, const uint8_t* codes, const void* s
 // are split over blockIdx.y: each split writes its own fp32 sums (`part`), which k_join adds in
 // order; a single split writes y.
 template <bool F16, int G, bool ZEROS, int MT, int RT>
-__global__ __launch_bounds__(512) void k_batch(const void* __restrict__ x, long long ldx,
-                                               const uint8_t* __restrict__ codes, const void* __restrict__ scales,
-                                               const uint8_t* __restrict__ zeros, void* __restrict__ y, long long ldy,
-                                               int m, int n, int k, int group, int per, float* __restrict__ part_out) {
+__global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, const uint8_t* codes, const void* scales,
+                                               const uint8_t* zeros, void* y, long long ldy, int m, int n, int k,
+                                               int group, int per, float* part_out) {
   using Y = Type<F16>;
   using T = typename Y::T;
   using Sc = Scales<F16, G, ZEROS>;
-    constexpr int STEPS = 4 / Sc::SPC, ROWS = 16 * MT, SLOT = RT * 2048, COPIES = 2 * RT;
+  constexpr int STEPS = 4 / Sc::SPC, ROWS = 16 * MT, SLOT = RT * 2048, COPIES = 2 * RT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane >> 4, r = lane & 15;
@@ -562,7 +562,8 @@ hipError_t run(const void* x, long long ldx, const uint8_t* codes, const void* s
 
 template <bool F16>
 hipError_t launch(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros,
-                  void* y, long long ldy, int m, int n, int k, int group, int splits, float* part, bool each, hipStream_t s) {
+                  void* y, long long ldy, int m, int n, int k, int group, int splits, float* part, bool each,
+                  hipStream_t s) {
   const int g = group % CHUNK == 0 ? 1 : k < CHUNK ? 0 : group == 64 ? 2 : group == 32 ? 4 : 0;
 #define RUN(G)                                                                                                \
   (zeros ? run<F16, G, true>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, splits, part, each, s)     \
@@ -581,7 +582,8 @@ int refuse(const char* why) {
 // y[m][n] = x[m][k] W^T, queued on `stream` of device `dev`; nothing waits for it.  codes
 // [n][k/2] (the lower half of a byte first), scales [n][k/group] of x's type, zeros
 // [n][k/group] bytes or null for 8.  splits 0: each row of x by itself, k_one; else together,
-// k_batch, the columns split, and `part` holds splits x m x n fp32 sums.  0, or -1 / a HIP error with tkv_last_error() set.
+// k_batch, the columns split, and `part` holds splits x m x n fp32 sums.  0, or -1 / a HIP error
+// with tkv_last_error() set.
 extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const void* codes, const void* scales,
                            const void* zeros, void* y, long long ldy, int m, int n, int k, int group, int splits,
                            void* part, void* stream) {
@@ -593,7 +595,6 @@ extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const
     return refuse("rows of x and of the codes must be 16-byte aligned");
   if (ldy < n) return refuse("y's row stride is below its width");
   if (splits < 0 || splits > 64 || (splits > 1 && !part)) return refuse("0 to 64 splits, with room for their sums");
-  if (splits == 0 && m > 64) return refuse("1 to 64 rows of x");
   int prev = 0;
   hipError_t e = hipGetDevice(&prev);
   if (e == hipSuccess && prev != dev) e = hipSetDevice(dev);

@@ -85,7 +85,8 @@ constexpr int FEW_ROWS = 512;
 // The two tilings of the matrix products.  A fragment is 16 x 16; a lane of a wave holds rows
 // row(mf) + (lane / 16) * 4 + 0..3 and column col(nf) + lane % 16 of fragment (mf, nf).
 struct Big {  // 8 waves, the schedule of product_big
-  static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2, LDS = 256 * (256 * 2 + 16);  // of the tile on its way out; the steps take 128 KiB
+  static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2,
+                       LDS = 256 * (256 * 2 + 16);  // of the tile on its way out; the steps take 128 KiB
   static __device__ __forceinline__ int wave_m(int wid) { return wid >> 2; }
   static __device__ __forceinline__ int row(int mf, int wid) { return (mf >> 2) * 128 + (wid >> 2) * 64 + (mf & 3) * 16; }
   static __device__ __forceinline__ int col(int nf, int wid) { return (nf >> 1) * 128 + (wid & 3) * 32 + (nf & 1) * 16; }
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
       part[(size_t)tv * n + token] = c;
     }
   } else {
-__syncthreads();  // LDS has been read
+    __syncthreads();  // LDS has been read
 #pragma unroll
     for (int j = 0; j < Tile::NF; ++j) {
       const int token = tn * Tile::BN + Tile::col(j, wid) + fr;
@@ -797,32 +798,34 @@ __global__ __launch_bounds__(256) void k_teacher(const long long* __restrict__ i
   bool any = false;
   for (int i = lane; i < k; i += 64)
     if (ids[i] >= 0) {
-      const float t = logits[i] * inv_t;
-      any |= t != -INFINITY;  // NaN counts: it has to show in the loss
-      m = fmaxf(m, t);
+      any |= logits[i] != -INFINITY;  // NaN counts: it has to show in the loss
+      m = fmaxf(m, logits[i]);
     }
   m = wave_max(m);
   any = __any(any);
   if (m == -INFINITY) m = 0.f;
+  // (the difference before the division: a list of the type's lowest value is uniform at any T)
+  const float sc = inv_t * LOG2E;
   float s = 0.f;
-  for (int i = lane; i < k; i += 64) s += ids[i] >= 0 ? exp2f((logits[i] * inv_t - m) * LOG2E) : 0.f;
+  for (int i = lane; i < k; i += 64) s += ids[i] >= 0 ? exp2f((logits[i] - m) * sc) : 0.f;
   s = wave_sum(s);
-  for (int i = lane; i < k; i += 64)
-    p[i] = any && ids[i] >= 0 ? exp2f((logits[i] * inv_t - m) * LOG2E) / s : 0.f;
+  for (int i = lane; i < k; i += 64) p[i] = any && ids[i] >= 0 ? exp2f((logits[i] - m) * sc) / s : 0.f;
   if (lane == 0) flag[row] = any;
 }
 
-// Packs the rows that have a loss into xc [rows][dp] (zeros behind d).  A block takes 8 rows, two
-// a wave, and counts the kept rows before them itself, which needs no second launch for a scan
+// Packs the rows that have a loss into xc [rows][dp] (zeros behind d).  A wave takes `per` rows, and
+// its block counts the kept rows before them itself, which needs no second launch for a scan
 // (8192 tokens: 1024 blocks read at most 64 KiB of targets each, out of L2).
+constexpr int MOST_PER = 32;
+int gather_rows(int n) { return n <= 65536 ? 2 : (n + 32767) / 32768; }  // at most about 8192 blocks
 template <typename T>
 __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long long ldx, int n, int d, int dp,
                                                 const long long* __restrict__ target, long long ignore,
                                                 const int* __restrict__ flag, T* __restrict__ xc,
                                                 int* __restrict__ rowmap, int* __restrict__ posof,
-                                                int* __restrict__ count, float* __restrict__ loss) {
-  __shared__ int total[4], kept[8];
-  const int row0 = blockIdx.x * 8, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+                                                int* __restrict__ count, float* __restrict__ loss, int per) {
+  __shared__ int total[4], kept[4 * MOST_PER];
+  const int row0 = blockIdx.x * 4 * per, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c = 0;
   if (flag) {
     for (int r = tid; r < row0; r += 256) c += flag[r] != 0;
@@ -832,20 +835,20 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
 #pragma unroll
   for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
   if (lane == 0) total[wave] = c;
-  if (tid < 8) {
+  if (tid < 4 * per) {
     const int r = row0 + tid;
     kept[tid] = r < n && (flag ? flag[r] != 0 : target[r] != ignore);
   }
   __syncthreads();
   int pos = total[0] + total[1] + total[2] + total[3];
-  if (tid == 0 && row0 + 8 >= n) {
+  if (tid == 0 && row0 + 4 * per >= n) {
     int all = pos;
-    for (int i = 0; i < 8; ++i) all += kept[i];
+    for (int i = 0; i < 4 * per; ++i) all += kept[i];
     count[0] = all;
     count[1] = 0;
   }
-  for (int i = 0; i < wave * 2; ++i) pos += kept[i];
-  for (int i = wave * 2; i < wave * 2 + 2; ++i) {
+  for (int i = 0; i < wave * per; ++i) pos += kept[i];
+  for (int i = wave * per; i < (wave + 1) * per; ++i) {
     const int r = row0 + i;
     if (r >= n) break;
     if (!kept[i]) {
@@ -921,12 +924,14 @@ __global__ __launch_bounds__(256) void k_dots(const T* __restrict__ xc, int dp, 
                                               long long ldw, int dk, const long long* __restrict__ ids, int k,
                                               long long v, const int* __restrict__ rowmap,
                                               const int* __restrict__ count, float* __restrict__ zk) {
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int pos = (int)(item / k), j = (int)(item - (long long)pos * k), lane = threadIdx.x & 63;
-  if (pos >= count[0]) return;
-  const long long id = ids[(size_t)rowmap[pos] * k + j];
-  const float s = id < 0 ? 0.f : dot(xc + (size_t)pos * dp, w, ldw, dk, id, v, lane, 64);
-  if (lane == 0) zk[(size_t)pos * k + j] = s;
+  const long long items = (long long)count[0] * k;
+  const int lane = threadIdx.x & 63;
+  for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += (long long)gridDim.x * 4) {
+    const int pos = (int)(i / k), j = (int)(i - (long long)pos * k);
+    const long long id = ids[(size_t)rowmap[pos] * k + j];
+    const float s = id < 0 ? 0.f : dot(xc + (size_t)pos * dp, w, ldw, dk, id, v, lane, 64);
+    if (lane == 0) zk[i] = s;
+  }
 }
 
 // Joins the tiles' (max, sum) of 8 rows, 32 threads a row, and forms the rows' losses; of a cross
@@ -1212,6 +1217,9 @@ int check(const tkl_args& a) {
   else if (!a.wc && ((a.d & 7) || (a.ldw & 7) || (reinterpret_cast<uintptr_t>(a.w) & 15)))
     bad = "w's rows are not 16-byte aligned and there is no room for a copy";
   else if (!a.wc && (a.ldw < a.d || a.ldw > (1 << 21))) bad = "w's row stride must be its width to 2^21 elements";
+  // a launch has fewer than 2^32 threads: 512 to a tile of 256 x 256, 256 to 1024 numbers of dX
+  else if ((a.v + 255) / 256 * ((a.n + 255) / 256) >= 1 << 23) bad = "tokens x vocabulary must be below 2^39";
+  else if ((a.d + 1023) / 1024 * a.n >= 1 << 24) bad = "tokens x width must be below 2^34";
   else if (a.reduction < 0 || a.reduction > 2) bad = "reduction must be 0 to 2";
   else if (!(a.temperature > 0.f)) bad = "the temperature must be above 0";
   if (bad) {
@@ -1255,8 +1263,8 @@ unsigned blocks(long long items, long long per) { return (unsigned)((items + per
 template <typename T>
 void pad(const tkl_args& a, int dp, hipStream_t s) {
   if (a.wc)
-    k_pad<T><<<(unsigned)std::min<long long>(blocks(a.v * (dp / 8), 256), 16384), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, a.v, (int)a.d,
-                                                                       dp, static_cast<T*>(a.wc));
+    k_pad<T><<<(unsigned)std::min<long long>(blocks(a.v * (dp / 8), 256), 16384), 256, 0, s>>>(
+        static_cast<const T*>(a.w), a.ldw, a.v, (int)a.d, dp, static_cast<T*>(a.wc));
 }
 
 template <class Tile, bool F16, bool DL>
@@ -1285,15 +1293,16 @@ hipError_t forward(const tkl_args& a) {
   T* xc = reinterpret_cast<T*>(q.xc);
   if (a.distill)
     k_teacher<<<blocks(n, 4), 256, 0, s>>>(ids, static_cast<const float*>(a.teacher), n, k, 1.f / t, q.p, q.flag);
-  k_gather<T><<<blocks(n, 8), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, dp, ids, a.ignore, q.flag, xc,
-                                           q.rowmap, q.posof, q.count, a.reduction ? nullptr : loss);
+  const int per = gather_rows(n);
+  k_gather<T><<<blocks(n, 4 * per), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, dp, ids, a.ignore, q.flag, xc,
+                                                 q.rowmap, q.posof, q.count, a.reduction ? nullptr : loss, per);
   pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
   const T* wt = static_cast<const T*>(w.at);
   logits<F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
   if (a.distill)
-    k_dots<T><<<blocks((long long)n * k, 4), 256, 0, s>>>(xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count,
-                                                          q.zk);
+    k_dots<T><<<(unsigned)std::min<long long>(((long long)n * k + 3) / 4, 1 << 22), 256, 0, s>>>(
+        xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count, q.zk);
   k_loss<T><<<blocks(n, 8), 256, 0, s>>>(static_cast<const float2*>(a.room),
                                          (int)blocks(a.v, a.small & 1 ? Small::BM : Big::BM), n, xc, dp, wt, w.ldb / 2,
                                          w.dk, ids, a.v, q.zk, q.p, k, q.rowmap, q.count, LOG2E / t, t * t, q.lse,
@@ -1376,8 +1385,11 @@ extern "C" long long tkl_room_bytes(const tkl_args* a) { return room_of(*a).byte
 extern "C" int tkl_forward(const tkl_args* a) { return on_device(a, a->f16 ? forward<true> : forward<false>); }
 
 extern "C" int tkl_backward(const tkl_args* a) {
-  if (a->piece < Big::BM || a->piece % Big::BM || a->piece > (1 << 24) || a->fill < 1 || a->fill > 4096) {
-    snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, fill %lld 1 to 4096", a->piece, Big::BM, a->fill);
+  // (a tile's rows of dl are addressed below FAR)
+  if (a->piece < Big::BM || a->piece % Big::BM || a->piece > (1 << 24) || a->fill < 1 || a->fill > 4096 ||
+      std::min<long long>(a->n, Big::BN) * a->piece > (1 << 28)) {
+    snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, at most 2^28 over 256 tokens; fill %lld 1 to 4096",
+             a->piece, Big::BM, a->fill);
     return -1;
   }
   return on_device(a, a->f16 ? backward<true> : backward<false>);

@@ -9,6 +9,7 @@ and undo them, on any device.
 """
 
 import ctypes
+import math
 from typing import Any, Optional, Tuple
 
 from .native import load
@@ -77,13 +78,22 @@ def _up(n: int, to: int) -> int:
     return -(-n // to) * to
 
 
+def _overlap(a, b) -> bool:
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
+        1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def gemv_w4(x, codes, scales, zeros=None, *, out=None):
     """``x @ w.T`` for ``x [..., K]`` of at most 64 rows, bf16 or fp16, of any strides.
 
     ``codes`` is uint8 ``[N, K/2]``, two codes to a byte, the lower half first; ``scales``
     ``[N, K/group]`` has ``x``'s type, ``zeros`` (uint8, the same shape) may be left out for
     symmetric weights, whose zero is 8.  The weight's tensors are contiguous; ``group`` is a
-    multiple of 32.  Sums are fp32 and rounded once.  The result (``out``, if given: contiguous,
+    multiple of 32.  Sums are fp32 and rounded once; they are of ``(16 + code) * x``, so an infinite
+    ``x`` gives NaN.  The result (``out``, if given: contiguous,
     ``[..., N]``) has ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that
     wants one is refused."""
     import torch
@@ -112,6 +122,10 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
         out = torch.empty((*shape[:-1], n), dtype=dtype, device=dev)
     elif out.shape != (*shape[:-1], n) or out.dtype is not dtype or out.device != dev or not out.is_contiguous():
         raise GemvError(f"out must be contiguous {dtype} {[*shape[:-1], n]} on x's device")
+    elif any(_overlap(out, t) for t in (x, codes, scales, zeros) if t is not None):
+        raise GemvError("out must not share memory with x or the weight")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
     if m == 0 or n == 0:
         return out
     if len(shape) != 2:
@@ -163,11 +177,11 @@ def quantize_w4(w, group: int = 128, symmetric: bool = True) -> Tuple[Any, Any, 
         scales = ((hi - lo) / 15).to(w.dtype)
     # codes go by the rounded scale; a scale of 0 (a group of zeros, or too small for the type) has code = zero
     step = scales.float()
-    inv = torch.where(step > 0, 1 / step, 0.0)
+    step = torch.where(step > 0, step, math.inf)
     if not symmetric:
-        zeros = (-lo * inv).round().clamp(0, 15).to(torch.uint8)
+        zeros = (-lo / step).round().clamp(0, 15).to(torch.uint8)
     zero = float(SYMMETRIC_ZERO) if zeros is None else zeros.float()[:, :, None]
-    codes = (v * inv[:, :, None] + zero).round().clamp(0, 15).to(torch.uint8)
+    codes = (v / step[:, :, None] + zero).round().clamp(0, 15).to(torch.uint8)
     return pack_w4(codes.reshape(n, k)), scales, zeros
 
 

@@ -7,6 +7,12 @@ being stored: the forward pass keeps a few numbers a token, and the backward pas
 the logits again, a piece of the vocabulary at a time.  Like ``gemm.gemm_bt`` they take torch
 tensors on the GPU and queue their work on torch's current stream of that device; nothing
 waits for it here, and both directions can be captured into a graph.
+
+A captured backward pass needs everything that it goes through to be made on the capture's
+stream.  torch keeps a leaf's gradient node, and its stream, for as long as any graph of that
+leaf lives; captured then, the pass would leave that stream behind in the capture, which ends
+the process.  A call that meets such a node of an earlier call is refused; drop the earlier loss
+first, or capture with leaves made in the capture (``x.detach().requires_grad_()``).
 """
 
 import ctypes
@@ -105,6 +111,8 @@ def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, 
 
 def _row_strided(w):
     """``w`` with a row stride that the kernels take."""
+    if w.shape[0] == 1:
+        return w.reshape(-1).contiguous().view(1, -1)  # a lone row's stride may be anything
     return w if w.stride(1) == 1 and w.shape[1] <= w.stride(0) <= 1 << 21 else w.contiguous()
 
 
@@ -117,6 +125,23 @@ def _room_for_copy(w):
     if d % 8 or w.stride(0) % 8 or w.data_ptr() % 16:
         return torch.empty((v, _up(d, 64)), dtype=w.dtype, device=w.device)
     return None
+
+
+def _apply(x, w, ids, teacher, plan):
+    import torch
+
+    loss = _autograd().apply(x, w, ids, teacher, plan)
+    if loss.grad_fn is not None:
+        stream = torch._C._cuda_getCurrentRawStream(x.device.index)
+        for node, _ in loss.grad_fn.next_functions[:2]:
+            # (kept by the node itself, as long as a graph holds it)
+            if node is not None and node.metadata.setdefault("tk_loss_stream", stream) != stream:
+                with torch.cuda.device(x.device):
+                    if torch.cuda.is_current_stream_capturing():
+                        del loss, node  # or the error's traceback keeps them
+                        raise LossError("captured while an eager graph of the same x or w lives: its gradient cannot be "
+                                        "captured (drop the earlier loss, or detach x and w in the capture)")
+    return loss
 
 
 class _Plan:
@@ -257,7 +282,7 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
     plan = _check("linear_cross_entropy", x, w, reduction)
     ids = _ids("linear_cross_entropy", "target", target, x, 0)
     plan.k, plan.distill, plan.temperature, plan.ignore = 1, 0, 1.0, int(ignore_index)
-    return _autograd().apply(x, w, ids, None, plan)
+    return _apply(x, w, ids, None, plan)
 
 
 def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean"):
@@ -287,4 +312,4 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     if not (math.isfinite(temperature) and temperature > 0):
         raise LossError(f"{what}: the temperature must be above 0, not {temperature}")
     plan.k, plan.distill, plan.temperature, plan.ignore = ids.shape[-1], 1, temperature, 0
-    return _autograd().apply(x, w, ids, logits.detach().float().contiguous(), plan)
+    return _apply(x, w, ids, logits.detach().float().contiguous(), plan)
