@@ -3,7 +3,12 @@
 Error model of the kernels.  u is half a step of the 16-bit type relative to a value (bf16
 2^-8, fp16 2^-11).  A logit is a sum of D exact products in fp32: its error is at most
 (D + 8) 2^-23 sum |x w| (each addition rounds or cuts off the last bit of a partial sum).  The
-exponent's argument rounds once more, and exp2 and log2 are good to 2^-21 of their result."""
+exponent's argument rounds once more, and exp2 and log2 are good to 2^-21 of their result.
+Where the logits are kept in 16 bits for the backward pass, an entry that is no target is off by
+half a step of 2^-12 in exp2's argument, ln 2 2^-13 = 8.5e-5 of its value, or of 2^-10, 3.4e-4,
+where it is less than 2^-8 of its tile's largest, or of 2^-7, 2.71e-3, where less than 2^-24; the
+number of steps, up to 65535, is itself rounded to fp32 on both ways, which adds 2^-6 of a step.
+2^-13, 2^-11 and 2^-8 are above these."""
 
 import math
 
@@ -28,8 +33,9 @@ def teacher_of(ids, logits, t):
     return torch.where(total > 0, ids, -1), torch.where(total > 0, e / total, 0.0)
 
 
-def head(x, w, ids, p, t, g):
-    """loss [n], dx, dw and their bounds for ``sum(g * loss)``, all in 64 bits."""
+def head(x, w, ids, p, t, g, kept=True):
+    """loss [n], dx, dw and their bounds for ``sum(g * loss)``, all in 64 bits; ``kept``: with the
+    logits kept in 16 bits."""
     dt = x.dtype
     u = U[dt]
     has = (ids >= 0).any(1)
@@ -47,6 +53,11 @@ def head(x, w, ids, p, t, g):
     dl = q.clone().scatter_add_(1, at, -used) * (g * t)[:, None]
     # the stored derivative: q's error, one rounding, and what fp16 cannot hold under 2^-25 2^-15
     ddl = (q * (dz + off[:, None] + 2.0 ** -20)) * (g.abs() * t)[:, None] + u * dl.abs() + g.abs().max() * t * 2.0 ** -39
+    if kept:
+        code = torch.where(q < 2.0 ** -24, 2.0 ** -8, torch.where(q < 2.0 ** -8, 2.0 ** -11, 2.0 ** -13))
+        code = q * code * (g.abs() * t)[:, None]
+        listed = torch.zeros_like(q).scatter_add_(1, at, (ids >= 0).double()) > 0
+        ddl = ddl + torch.where(listed, 0.0, code)
     ddl = torch.where(has[:, None], ddl, 0.0)
     size = dl.abs() + ddl
 

@@ -29,7 +29,7 @@ def _run(call, x, w, g):
     return (loss.detach(), *torch.autograd.grad(loss, (x, w), g))
 
 
-def _against(call, x, w, ids, p, t=1.0, reduction="none", gen=None):
+def _against(call, x, w, ids, p, t=1.0, reduction="none", gen=None, kept=True):
     n = x.shape[0]
     count = max(1, int((ids >= 0).any(1).sum()))
     up = torch.rand(n, device="cuda", generator=gen) - 0.3 if reduction == "none" else torch.tensor(0.75, device="cuda")
@@ -37,7 +37,7 @@ def _against(call, x, w, ids, p, t=1.0, reduction="none", gen=None):
     g = up.double() if reduction == "none" else torch.full((n,), 0.75, device="cuda", dtype=torch.float64)
     if reduction == "mean":
         g = g / count
-    want, wdx, wdw = ref.head(x, w, ids, p, t, g)
+    want, wdx, wdw = ref.head(x, w, ids, p, t, g, kept)
     if reduction != "none":
         over = 1 if reduction == "sum" else count
         want = dict(value=want["value"].sum() / over, bound=(want["bound"].sum() + want["value"].abs().sum() * 1e-6) / over)
@@ -53,28 +53,32 @@ SIZES = [(1, 8, 1), (1, 64, 300), (2, 72, 256), (5, 72, 257), (48, 512, 1000), (
 
 @pytest.mark.parametrize("tiles", [0, 7], ids=["large", "small"])
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("kept", [True, False], ids=["kept", "again"])
 @pytest.mark.parametrize("n,d,v", SIZES)
-def test_cross_entropy(n, d, v, dt, tiles, monkeypatch):
+def test_cross_entropy(n, d, v, dt, kept, tiles, monkeypatch):
     from triton_kubernetes_amd.ops import loss
     from triton_kubernetes_amd.ops.loss import linear_cross_entropy
 
     monkeypatch.setattr(loss, "small_products", lambda *a: tiles)
+    monkeypatch.setattr(loss, "keeps", lambda *a: kept)
     gen = _gen(n, d, v)
     x, w, t = _inputs(n, d, v, dt, gen)
     for reduction in ("none", "mean"):
         _against(lambda x, w: linear_cross_entropy(x, w, t, reduction=reduction), x, w, *ref.targets_of(t, -100, n, v),
-                 reduction=reduction, gen=gen)
+                 reduction=reduction, gen=gen, kept=kept)
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+@pytest.mark.parametrize("kept", [True, False], ids=["kept", "again"])
 @pytest.mark.parametrize("n,d,v,k,temp", [(1, 64, 300, 1, 1.0), (7, 72, 257, 5, 2.0), (130, 264, 1111, 64, 0.7),
                                           (40, 77, 5003, 130, 2.0), (300, 512, 999, 33, 1.0)])
 @pytest.mark.parametrize("tiles", [0, 7], ids=["large", "small"])
-def test_distill(n, d, v, k, temp, dt, tiles, monkeypatch):
+def test_distill(n, d, v, k, temp, dt, kept, tiles, monkeypatch):
     from triton_kubernetes_amd.ops import loss
     from triton_kubernetes_amd.ops.loss import linear_distill
 
     monkeypatch.setattr(loss, "small_products", lambda *a: tiles)
+    monkeypatch.setattr(loss, "keeps", lambda *a: kept)
     gen = _gen(n, d, v, k)
     x, w, _ = _inputs(n, d, v, dt, gen)
     ids = torch.randint(0, v, (n, k), device="cuda", generator=gen)  # the same id twice among them
@@ -86,7 +90,7 @@ def test_distill(n, d, v, k, temp, dt, tiles, monkeypatch):
         logits[1] = -float("inf")
     for reduction in ("none", "sum"):
         _against(lambda x, w: linear_distill(x, w, ids, logits, temperature=temp, reduction=reduction), x, w,
-                 *ref.teacher_of(ids, logits, temp), t=temp, reduction=reduction, gen=gen)
+                 *ref.teacher_of(ids, logits, temp), t=temp, reduction=reduction, gen=gen, kept=kept)
 
 
 def test_one_id_listed_many_times():
@@ -551,3 +555,34 @@ print("same")
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert done.returncode == 0 and done.stdout.strip().endswith("same"), done.stderr[-2000:]
+
+
+def test_keep_logits_decides_what_stays_between_the_passes():
+    from triton_kubernetes_amd.ops.loss import linear_cross_entropy, linear_distill
+
+    n, d, v = 300, 64, 20_000
+    gen = _gen(27)
+    x, w, t = _inputs(n, d, v, torch.bfloat16, gen)
+    x.requires_grad_()
+    logits = torch.zeros((n, 1), device="cuda")
+    for call in (lambda **k: linear_cross_entropy(x, w, t, **k), lambda **k: linear_distill(x, w, t[:, None], logits, **k)):
+        held, losses, grads = [], [], []
+        for keep in (False, True, None):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            loss = call(keep_logits=keep)
+            held.append(torch.cuda.memory_allocated() - before)
+            first = torch.autograd.grad(loss, x, retain_graph=True)[0]
+            assert torch.equal(first, torch.autograd.grad(loss, x)[0])  # the kept logits stay as they are
+            losses.append(loss.detach())
+            grads.append(first.float())
+            del loss
+        assert held[0] < 2 * n * v <= held[1] == held[2]
+        assert torch.equal(losses[0], losses[1]) and torch.equal(grads[1], grads[2])
+        # both round the derivative to 16 bits; one half step 2^-8 of each, and the result's
+        size = (torch.softmax(x.detach().float() @ w.float().T, 1).abs() @ w.float().abs() + w[t].float().abs()) / n
+        assert bool(((grads[0] - grads[1]).abs() <= 4 * 2.0 ** -8 * size).all())
+        with torch.no_grad():
+            before = torch.cuda.memory_allocated()
+            loss = call(keep_logits=True)  # without a backward pass nothing is kept
+            assert torch.cuda.memory_allocated() - before < 2 * n * v

@@ -37,7 +37,7 @@ def test_pieces_cover_the_vocabulary_within_the_workspace(n, v):
 
 
 FIELDS = ("n", "d", "v", "k", "ldx", "ldw", "ldg", "ignore", "piece", "fill", "dev", "f16", "distill", "reduction",
-          "temperature", "want", "small", "x", "w", "ids", "teacher", "grad", "loss", "kept", "room", "wc", "dx", "dw",
+          "temperature", "want", "small", "x", "w", "ids", "teacher", "grad", "loss", "kept", "room", "codes", "wc", "dx", "dw",
           "stream")
 
 

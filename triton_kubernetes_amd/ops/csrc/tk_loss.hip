@@ -1,5 +1,5 @@
 // Losses of a language model's output head on MI355X (gfx950): the logits z = X W^T of N tokens
-// over a vocabulary of V are never stored.
+// over a vocabulary of V leave the kernel that multiplies only as sums, or in 16 bits.
 //
 // Both losses compare the softmax q of a row's logits (at a temperature T) with K sparse
 // targets (id_k, p_k), sum_k p_k = 1:
@@ -13,10 +13,9 @@
 // Forward: one matrix product whose epilogue reduces every tile of the vocabulary to a maximum
 // and a sum per token (k_logits<LSE>), a dot product per target, and a join over the tiles
 // (k_loss, which also forms a cross entropy's dot products; k_dots those of a teacher's lists).
-// Backward, in pieces of the vocabulary: the logits of the piece are computed again, and the
-// epilogue turns them into their 16-bit derivative dl (k_logits<DL>; a teacher's targets are
-// put in by k_fix); then dX += dl W and dW = dl^T X, two matrix products that read dl while
-// the last-level cache still holds it.
+// Backward, in pieces of the vocabulary: the logits' 16-bit derivative dl, from codes that the
+// forward pass kept (k_dl, struct Codes), or from the same product again (k_logits<DL>); a
+// teacher's targets are put in by k_fix; then dX += dl W and dW = dl^T X.
 //
 // dl is rounded to 16 bits, which costs each product about as much as the rounding of its result.
 // Most of a row's derivative is at its target, though, and few numbers' roundings do not average
@@ -69,6 +68,7 @@ struct tkl_args {
   const void *x, *w, *ids, *teacher, *grad;
   void *loss, *kept;           // kept: from forward to backward (struct Kept)
   void *room;                  // forward: the tiles' maxima and sums; backward: dl, sums of dX, factors
+  void *codes;                 // from forward to backward: the logits in 16 bits (struct Codes), or null
   void *wc;                    // a padded copy of w, where w's rows are not 16-byte aligned; forward makes it
   void *dx, *dw;
   void* stream;
@@ -86,7 +86,7 @@ constexpr int FEW_ROWS = 512;
 // row(mf) + (lane / 16) * 4 + 0..3 and column col(nf) + lane % 16 of fragment (mf, nf).
 struct Big {  // 8 waves, the schedule of product_big
   static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2,
-                       LDS = 256 * (256 * 2 + 16);  // of the tile on its way out; the steps take 128 KiB
+                       LDS = 256 * (256 * 2 + 16) + 4096;  // the tile on its way out and sums; steps take 128 KiB
   static __device__ __forceinline__ int wave_m(int wid) { return wid >> 2; }
   static __device__ __forceinline__ int row(int mf, int wid) { return (mf >> 2) * 128 + (wid >> 2) * 64 + (mf & 3) * 16; }
   static __device__ __forceinline__ int col(int nf, int wid) { return (nf >> 1) * 128 + (wid & 3) * 32 + (nf & 1) * 16; }
@@ -473,9 +473,13 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
 template <class Tile, typename T>
 struct Outgoing {
   static constexpr int STRIDE = Tile::BM * 2 + 16, PER = Tile::BM / 8;
-  static_assert(Tile::BN * STRIDE <= Tile::LDS, "the tile fits");
+  static constexpr int BYTES = Tile::BN * STRIDE;
+  static_assert(BYTES + Tile::WAVES_M * Tile::BN * 8 <= Tile::LDS, "the tile and its sums fit");
+  static __device__ __forceinline__ void put(char* smem, int col, int row, unsigned ab, unsigned cd) {
+    *reinterpret_cast<u32x2*>(smem + col * STRIDE + row * 2) = u32x2{ab, cd};
+  }
   static __device__ __forceinline__ void put(char* smem, int col, int row, float a, float b, float c, float d) {
-    *reinterpret_cast<u32x2*>(smem + col * STRIDE + row * 2) = u32x2{pack2<T>(a, b), pack2<T>(c, d)};
+    put(smem, col, row, pack2<T>(a, b), pack2<T>(c, d));
   }
   // rows first .. first + count of `out`, from column c0 on, `width` of them
   static __device__ __forceinline__ void store(const char* smem, T* out, long long ld, long long first, int count, int c0,
@@ -525,18 +529,42 @@ struct Upstream {
   }
 };
 
+// A logit z (times log2(e) / T) in 16 bits, as its distance from the maximum M of its row within
+// its tile: steps of 2^-12 down to M - 8, of 2^-10 to M - 24, of 2^-7 to M - 152, below which
+// exp2 is 0 in fp32.  What a step's half is of q = exp2(z - lse), 8.5e-5, 3.4e-4 and 2.7e-3 of its
+// value, joins the rounding of dl to bf16, 3.9e-3, or to fp16, 4.9e-4, whose numbers run out at
+// 2^-29 of the largest (struct Upstream).
+struct Codes {
+  static __device__ __forceinline__ unsigned pack(float a, float b) {  // distances
+    auto code = [](float d) {  // the least of the three lines, of 65535
+      constexpr float S = 4096.f / 65535.f;
+      return fminf(fminf(d * S, __builtin_fmaf(d, S / 4, 24576.f / 65535.f)), __builtin_fmaf(d, S / 32, 46080.f / 65535.f));
+    };
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(code(a), code(b)));
+  }
+  static __device__ __forceinline__ float distance(unsigned code) {
+    constexpr float S = 1.f / 4096.f;
+    const float c = (float)code;
+    return fmaxf(fmaxf(c * S, __builtin_fmaf(c, 4 * S, -98304.f * S)), __builtin_fmaf(c, 32 * S, -1474560.f * S));
+  }
+  // [n][stride] codes, then [tiles][n] maxima and sums
+  static __host__ __device__ long long stride(long long v) { return (v + 255) / 256 * 256; }
+};
+
 // z^T of Tile::BM vocabulary entries (A = W) by Tile::BN tokens (B = Xc), so that a lane holds
 // many entries of few tokens and the softmax's sums need two shuffles a token.
-// LSE: writes part[tile][token] = (max, sum).  DL: writes f (q - p) in 16 bits, with a cross
-// entropy's p; `targets` is null for a teacher's lists.  sc = log2(e) / T.
-template <class Tile, bool F16, bool DL>
+// LSE: writes part[tile][token] = (max, sum); KEEP: and the logits' codes to `out`.  DL: writes
+// f (q - p) in 16 bits to `out`, with a cross entropy's p; `targets` is null for a teacher's
+// lists.  sc = log2(e) / T.
+enum Mode { LSE, KEEP, DL };
+template <class Tile, bool F16, Mode MODE>
 __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict__ w, long long ldw,
                                                           const void* __restrict__ xc, long long ldxc, int v0,
                                                           int vend, int d, const int* __restrict__ count, int n,
                                                           float sc, float2* __restrict__ part,
                                                           const float* __restrict__ lse, Upstream<F16> up,
-                                                          const int* __restrict__ targets, void* __restrict__ dl,
-                                                          long long lddl, float* __restrict__ lost) {
+                                                          const int* __restrict__ targets, void* __restrict__ out,
+                                                          long long ldout, float* __restrict__ lost) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
   const int rows = count[0];
@@ -554,9 +582,10 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
   const int vb = tv * Tile::BM + fq * 4;  // the lane's entries are vb + row(i) + 0..3, in the piece
   const int vn = vend - v0;
   const bool whole = (tv + 1) * Tile::BM <= vn;
-  if constexpr (!DL) {
+  const int first = tn * Tile::BN, here = min(Tile::BN, rows - first);
+  if constexpr (MODE != DL) {
     barrier();  // LDS has been read
-    float2* sums = reinterpret_cast<float2*>(smem);  // [WAVES_M][BN]
+    float2* sums = reinterpret_cast<float2*>(smem + Outgoing<Tile, T>::BYTES);  // [WAVES_M][BN]
 #pragma unroll
     for (int j = 0; j < Tile::NF; ++j) {
       float m = -INFINITY, s = 0.f;
@@ -582,12 +611,29 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
       if (fq == 0) sums[Tile::wave_m(wid) * Tile::BN + Tile::col(j, wid) + fr] = float2{m, s};
     }
     __syncthreads();
-    const int token = tn * Tile::BN + tid;
-    if (tid < Tile::BN && token < rows) {
+    if (tid < here) {
       float2 c = sums[tid];
 #pragma unroll
       for (int o = 1; o < Tile::WAVES_M; ++o) merge(c.x, c.y, sums[o * Tile::BN + tid].x, sums[o * Tile::BN + tid].y);
-      part[(size_t)tv * n + token] = c;
+      part[(size_t)tv * n + first + tid] = c;
+    }
+    if constexpr (MODE == KEEP) {
+#pragma unroll
+      for (int j = 0; j < Tile::NF; ++j) {
+        const int col = Tile::col(j, wid) + fr;
+        float m = sums[col].x;
+#pragma unroll
+        for (int o = 1; o < Tile::WAVES_M; ++o) m = fmaxf(m, sums[o * Tile::BN + col].x);
+#pragma unroll
+        for (int i = 0; i < Tile::MF; ++i) {
+          float d[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = __builtin_fmaf(acc[i][j][e], -sc, m);
+          Outgoing<Tile, T>::put(smem, col, Tile::row(i, wid) + fq * 4, Codes::pack(d[0], d[1]), Codes::pack(d[2], d[3]));
+        }
+      }
+      __syncthreads();
+      Outgoing<Tile, T>::store(smem, static_cast<T*>(out), ldout, first, here, tv * Tile::BM, Tile::BM, tid);
     }
   } else {
     __syncthreads();  // LDS has been read
@@ -620,9 +666,44 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
       }
     }
     __syncthreads();
-    Outgoing<Tile, T>::store(smem, static_cast<T*>(dl), lddl, tn * Tile::BN, min(Tile::BN, rows - tn * Tile::BN),
-                             tv * Tile::BM, Tile::BM, tid);
+    Outgoing<Tile, T>::store(smem, static_cast<T*>(out), ldout, first, here, tv * Tile::BM, Tile::BM, tid);
   }
+}
+
+// The kept logits' codes of a piece -> f (q - p) in 16 bits, as k_logits<DL> writes it.  A block
+// takes 2048 entries of a row, 8 a thread; `at` and `zt` are the target and its logit of a cross
+// entropy's row, whose q - 1 has to be better than a code is.  zeros pad the piece.
+template <class Tile, bool F16>
+__global__ __launch_bounds__(256) void k_dl(const unsigned short* __restrict__ codes, long long ldc,
+                                            const float2* __restrict__ part, int n, int v0, int vn, float sc,
+                                            const float* __restrict__ lse, Upstream<F16> up, const int* __restrict__ at,
+                                            const float* __restrict__ zt, void* __restrict__ dl, long long lddl,
+                                            float* __restrict__ lost) {
+  using T = typename Type<F16>::T;
+  const int per_row = (int)((lddl + 2047) / 2048), pos = blockIdx.x / per_row;
+  const int c = ((blockIdx.x - pos * per_row) * 256 + threadIdx.x) * 8;
+  if (pos >= up.count[0] || c >= lddl) return;
+  u32x4 out = {0, 0, 0, 0};
+  if (c < vn) {
+    const u32x4 in = *reinterpret_cast<const u32x4*>(codes + pos * ldc + v0 + c);
+    const float f = up.of(pos), ls = lse[pos], m = part[(size_t)((v0 + c) / Tile::BM) * n + pos].x - ls;
+    const int target = (at ? at[pos] : -1) - v0 - c;
+    float g[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = Codes::distance(in[e / 2] >> (e % 2 * 16) & 0xffffu);
+      g[e] = c + e < vn ? f * __builtin_amdgcn_exp2f(m - d) : 0.f;
+    }
+    if ((unsigned)target < 8u) {
+      const float t = f * (__builtin_amdgcn_exp2f(__builtin_fmaf(zt[pos], sc, -ls)) - 1.f);
+      lost[pos] = t - (float)(T)t;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = e == target ? t : g[e];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = pack2<T>(g[2 * i], g[2 * i + 1]);
+  }
+  *reinterpret_cast<u32x4*>(static_cast<T*>(dl) + pos * lddl + c) = out;
 }
 
 // Into how many parts the vocabulary is split for dX of `rows` packed rows: as many as `fill`
@@ -943,7 +1024,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, int parts, int n,
                                               const T* __restrict__ xc, int dp, const T* __restrict__ w, long long ldw,
                                               int dk, const long long* __restrict__ ids, long long v,
-                                              const float* __restrict__ zk, const float* __restrict__ p, int k,
+                                              float* __restrict__ zk, const float* __restrict__ p, int k,
                                               const int* __restrict__ rowmap, const int* __restrict__ count, float sc,
                                               float t2, float* __restrict__ lse, float* __restrict__ rowloss,
                                               float* __restrict__ loss, int reduction, int* __restrict__ at_out,
@@ -956,7 +1037,7 @@ __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, i
       const long long id = ids[rowmap[at]];
       const float z = dot(xc + (size_t)at * dp, w, ldw, dk, id, v, threadIdx.x & 31, 32);
       if ((threadIdx.x & 31) == 0) {
-        sz[own] = z;
+        sz[own] = zk[at] = z;
         at_out[at] = id >= 0 && id < v ? (int)id : -1;
       }
     }
@@ -1141,12 +1222,12 @@ int padded(long long d) { return (int)((d + 63) / 64 * 64); }
 
 int residuals(const tkl_args& a) { return a.distill ? RESIDUALS : 1; }
 
-// What the forward pass keeps, in one buffer.  Without a teacher zk, p and flag are not there.
+// What the forward pass keeps, in one buffer.  Without a teacher p and flag are not there.
 struct Kept {
   char* xc;                        // [n][dp], the packed rows
   float *lse, *rowloss;            // by packed row
   int *rowmap, *posof, *count;     // packed row -> token and back; count[0] packed rows, count[1] k_loss's
-  float *zk, *p;                   // [packed row][k] logits of the targets, [token][k] probabilities
+  float *zk, *p;                   // [packed row][k] logits of the targets; a teacher's [token][k] probabilities
   int* flag;                       // by token: whether it has a target
   int* at;                         // [packed row][residuals] vocabulary entries, -1: none
   long long bytes;
@@ -1166,7 +1247,7 @@ Kept kept_of(const tkl_args& a) {
   r.rowmap = reinterpret_cast<int*>(take(4 * n));
   r.posof = reinterpret_cast<int*>(take(4 * n));
   r.count = reinterpret_cast<int*>(take(8));
-  r.zk = a.distill ? reinterpret_cast<float*>(take(4 * lists)) : nullptr;
+  r.zk = reinterpret_cast<float*>(take(4 * (a.distill ? lists : n)));
   r.p = a.distill ? reinterpret_cast<float*>(take(4 * lists)) : nullptr;
   r.flag = a.distill ? reinterpret_cast<int*>(take(4 * n)) : nullptr;
   r.at = reinterpret_cast<int*>(take(4 * n * residuals(a)));
@@ -1236,8 +1317,9 @@ hipError_t allow(Kernel* k, int lds) {
 }
 template <class Tile, bool F16>
 hipError_t allow_all() {
-  hipError_t e = allow(&k_logits<Tile, F16, false>, Tile::LDS);
-  if (e == hipSuccess) e = allow(&k_logits<Tile, F16, true>, Tile::LDS);
+  hipError_t e = allow(&k_logits<Tile, F16, LSE>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_logits<Tile, F16, DL>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_logits<Tile, F16, KEEP>, Tile::LDS);
   if (e == hipSuccess) e = allow(&k_dx<Tile, F16>, Tile::LDS);
   if (e == hipSuccess) e = allow(&k_dw<Tile, F16>, Tile::LDS);
   return e;
@@ -1267,19 +1349,36 @@ void pad(const tkl_args& a, int dp, hipStream_t s) {
         static_cast<const T*>(a.w), a.ldw, a.v, (int)a.d, dp, static_cast<T*>(a.wc));
 }
 
-template <class Tile, bool F16, bool DL>
-void logits_as(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
-            float* lost, hipStream_t s) {
-  k_logits<Tile, F16, DL><<<blocks(vn, Tile::BM) * blocks(a.n, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
-      w.at, w.ldb, kept.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, kept.count, (int)a.n, LOG2E / a.temperature,
-      static_cast<float2*>(a.room), kept.lse, up, a.distill ? nullptr : kept.at, a.room, a.piece, lost);
+// Where the forward pass puts the tiles' maxima and sums: behind the codes, if they are kept.
+float2* part_of(const tkl_args& a) {
+  return reinterpret_cast<float2*>(a.codes ? static_cast<char*>(a.codes) + 2 * a.n * Codes::stride(a.v)
+                                           : static_cast<char*>(a.room));
 }
 
-template <bool F16, bool DL>
-void logits(const tkl_args& a, const Kept& q, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
-            float* lost, hipStream_t s) {
-  if (a.small & 1) logits_as<Small, F16, DL>(a, q, w, dp, v0, vn, up, lost, s);
-  else logits_as<Big, F16, DL>(a, q, w, dp, v0, vn, up, lost, s);
+template <class Tile, bool F16, Mode MODE>
+void logits_as(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
+               void* out, long long ldout, float* lost, hipStream_t s) {
+  k_logits<Tile, F16, MODE><<<blocks(vn, Tile::BM) * blocks(a.n, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
+      w.at, w.ldb, kept.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, kept.count, (int)a.n, LOG2E / a.temperature,
+      part_of(a), kept.lse, up, a.distill ? nullptr : kept.at, out, ldout, lost);
+}
+
+template <class Tile, bool F16>
+void all_logits(const tkl_args& a, const Kept& q, const Weight& w, int dp, hipStream_t s) {
+  if (a.codes) logits_as<Tile, F16, KEEP>(a, q, w, dp, 0, (int)a.v, {}, a.codes, Codes::stride(a.v), nullptr, s);
+  else logits_as<Tile, F16, LSE>(a, q, w, dp, 0, (int)a.v, {}, nullptr, 0, nullptr, s);
+}
+
+// dl of a piece, out of the kept logits or by computing them again
+template <class Tile, bool F16>
+void derivative(const tkl_args& a, const Kept& q, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
+                const Room& r, hipStream_t s) {
+  if (a.codes)
+    k_dl<Tile, F16><<<blocks(a.piece, 2048) * (unsigned)a.n, 256, 0, s>>>(
+        static_cast<const unsigned short*>(a.codes), Codes::stride(a.v), part_of(a), (int)a.n, (int)v0, vn,
+        LOG2E / a.temperature, q.lse, up, a.distill ? nullptr : q.at, q.zk, r.dl, a.piece, r.lost);
+  else
+    logits_as<Tile, F16, DL>(a, q, w, dp, v0, vn, up, r.dl, a.piece, r.lost, s);
 }
 
 template <bool F16>
@@ -1299,11 +1398,12 @@ hipError_t forward(const tkl_args& a) {
   pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
   const T* wt = static_cast<const T*>(w.at);
-  logits<F16, false>(a, q, w, dp, 0, (int)a.v, {}, nullptr, s);
+  if (a.small & 1) all_logits<Small, F16>(a, q, w, dp, s);
+  else all_logits<Big, F16>(a, q, w, dp, s);
   if (a.distill)
     k_dots<T><<<(unsigned)std::min<long long>(((long long)n * k + 3) / 4, 1 << 22), 256, 0, s>>>(
         xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count, q.zk);
-  k_loss<T><<<blocks(n, 8), 256, 0, s>>>(static_cast<const float2*>(a.room),
+  k_loss<T><<<blocks(n, 8), 256, 0, s>>>(part_of(a),
                                          (int)blocks(a.v, a.small & 1 ? Small::BM : Big::BM), n, xc, dp, wt, w.ldb / 2,
                                          w.dk, ids, a.v, q.zk, q.p, k, q.rowmap, q.count, LOG2E / t, t * t, q.lse,
                                          q.rowloss, loss, a.reduction, q.at, a.reduction && n <= 512 ? q.count + 1 : nullptr);
@@ -1338,7 +1438,8 @@ hipError_t backward(const tkl_args& a) {
   const Weight w = weight_of(a, dp);
   for (long long v0 = 0; v0 < a.v; v0 += a.piece) {
     const int vn = (int)std::min(a.piece, a.v - v0);
-    logits<F16, true>(a, q, w, dp, v0, vn, up, r.lost, s);
+    if (a.small & 1) derivative<Small, F16>(a, q, w, dp, v0, vn, up, r, s);
+    else derivative<Big, F16>(a, q, w, dp, v0, vn, up, r, s);
     if (a.distill)
       k_fix<F16><<<blocks(n, 4), 256, 0, s>>>(static_cast<const long long*>(a.ids), q.p, k, a.v, q.zk, q.lse, up,
                                               LOG2E / a.temperature, v0, vn, r.dl, a.piece, q.at, r.lost);

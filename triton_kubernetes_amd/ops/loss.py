@@ -2,9 +2,10 @@
 
 ``linear_cross_entropy(x, w, target)`` is the softmax cross entropy of the logits ``x @ w.T``,
 and ``linear_distill(x, w, ids, logits)`` their divergence from a teacher's top logits; both
-with their gradients (torch autograd), and without the ``[tokens, vocabulary]`` logits ever
-being stored: the forward pass keeps a few numbers a token, and the backward pass computes
-the logits again, a piece of the vocabulary at a time.  Like ``gemm.gemm_bt`` they take torch
+with their gradients (torch autograd).  The ``[tokens, vocabulary]`` logits are never stored in
+full: the forward pass keeps a few numbers a token and, up to ``KEEP_BYTES`` of them, the
+logits in 16 bits for the backward pass, which otherwise computes them again; the backward
+pass works on a piece of the vocabulary at a time.  Like ``gemm.gemm_bt`` they take torch
 tensors on the GPU and queue their work on torch's current stream of that device; nothing
 waits for it here, and both directions can be captured into a graph.
 
@@ -18,12 +19,14 @@ first, or capture with leaves made in the capture (``x.detach().requires_grad_()
 import ctypes
 import math
 import struct
+from typing import Optional
 
 from .native import NativeUnavailable, load
 
 TILE = 256  # vocabulary entries and tokens of a large tile
 SMALL_M, SMALL_N = 128, 64  # of a small one
 DL_BYTES = 512 << 20  # the backward pass' 16-bit derivative of the logits, per piece
+KEEP_BYTES = 4 << 30  # of logits in 16 bits, kept from the forward to the backward pass
 MAX_TARGETS = 1024  # ids of a token's list
 MAX_TOKENS = 1 << 20
 MAX_WIDTH = 1 << 16
@@ -36,8 +39,9 @@ class LossError(RuntimeError):
 
 
 # struct tkl_args of csrc/tk_loss.hip: n d v k ldx ldw ldg ignore piece fill, dev f16 distill
-# reduction, temperature, want small, x w ids teacher grad loss kept room wc dx dw stream
-_ARGS = struct.Struct("@10q4if2i12P")
+# reduction, temperature, want small, x w ids teacher grad loss kept room codes wc dx
+# dw stream
+_ARGS = struct.Struct("@10q4if2i13P")
 
 _loaded = None
 
@@ -87,6 +91,15 @@ def small_products(n: int, d: int, v: int) -> int:
     return logits | dx << 1 | (tiles(d, v) <= 128) << 2
 
 
+def keeps(n: int, d: int, v: int) -> bool:
+    """Whether the forward pass keeps the logits, in 16 bits, for the backward pass, which otherwise
+    computes them again (``keep_logits`` decides for a single call).  A short product is cheaper than two passes over its result.  A step at
+    bf16, kept and again, in us: 4096 x 4096 x 32768 2740 and 3430, 512 x 32768 561 and 586,
+    384 530 and 534, 256 478 and 458; few tokens read the weight once less (16 x 4096 x 131072 841
+    and 1006, 512 x 256 x 32000 105 both)."""
+    return (d >= 384 or n <= 512) and 2 * n * v <= KEEP_BYTES
+
+
 def fill(small: bool) -> int:
     """Workgroups for x's gradient, among which the vocabulary is split where there are fewer tiles:
     a large tile for each of the 256 compute units (more only cost joining: 2048 x 2048 x 65536,
@@ -96,7 +109,16 @@ def fill(small: bool) -> int:
 
 def kept_bytes(n: int, d: int, lists: int) -> int:
     """Of what the forward pass keeps for the backward pass; ``lists`` entries of a teacher."""
-    return 2 * n * _up(d, 64) + 20 * n + 8 + (8 * lists + 16 * n if lists else 0)
+    return 2 * n * _up(d, 64) + 8 + (8 * lists + 36 * n if lists else 24 * n)
+
+
+def codes_bytes(n: int, v: int, small: bool) -> int:
+    """Of the logits kept for the backward pass: 2 bytes each, and a tile's maxima and sums."""
+    return 2 * n * _up(v, 256) + part_bytes(n, v, small)
+
+
+def part_bytes(n: int, v: int, small: bool) -> int:
+    return 8 * n * -(-v // (SMALL_M if small else TILE))
 
 
 def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, lists: int) -> int:
@@ -147,7 +169,7 @@ def _apply(x, w, ids, teacher, plan):
 class _Plan:
     """The sizes and settings of a call, from its forward to its backward pass."""
 
-    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore", "f16", "small", "lead")
+    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore", "f16", "small", "lead", "keep")
 
 
 _function = None
@@ -180,15 +202,16 @@ def _autograd():
             plain = _row_strided(w)
             copy = _room_for_copy(plain)
             kept = torch.empty(kept_bytes(n, d, n * k if plan.distill else 0), dtype=torch.uint8, device=dev)
-            room = torch.empty(8 * n * -(-v // (SMALL_M if plan.small & 1 else TILE)), dtype=torch.uint8, device=dev)
+            small = bool(plan.small & 1)
+            room = torch.empty((codes_bytes if plan.keep else part_bytes)(n, v, small), dtype=torch.uint8, device=dev)
             args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
                               plan.distill, plan.reduction, plan.temperature, 0, plan.small, x.data_ptr(),
                               plain.data_ptr(), ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0,
-                              loss.data_ptr(), kept.data_ptr(), room.data_ptr(), 0 if copy is None else copy.data_ptr(),
-                              0, 0, stream_of(dev.index))
+                              loss.data_ptr(), kept.data_ptr(), room.data_ptr(), room.data_ptr() if plan.keep else 0,
+                              0 if copy is None else copy.data_ptr(), 0, 0, stream_of(dev.index))
             if _lib().tkl_forward(args) != 0:
                 raise LossError(_lib().tkl_last_error().decode())
-            ctx.save_for_backward(w, ids, kept, *(() if copy is None else (copy,)))
+            ctx.save_for_backward(w, ids, kept, room if plan.keep else None, copy)
             return loss
 
         @staticmethod
@@ -202,13 +225,13 @@ def _autograd():
                 x, w = ctx.saved_tensors
                 return (torch.zeros_like(x) if want & 1 else None, torch.zeros_like(w) if want & 2 else None, None, None,
                         None)
-            w, ids, kept, *copy = ctx.saved_tensors
+            w, ids, kept, codes, copy = ctx.saved_tensors
             dev = w.device
             if not plan.reduction:
                 grad = grad.reshape(-1)
             if grad.dtype != torch.float32:
                 grad = grad.float()
-            plain = copy[0] if copy else _row_strided(w)
+            plain = _row_strided(w) if copy is None else copy
             piece = pieces(n, v)
             groups = fill(bool(plan.small & 2))
             room = torch.empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill),
@@ -218,7 +241,8 @@ def _autograd():
             args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
                               piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
                               want, plan.small, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
-                              kept.data_ptr(), room.data_ptr(), copy[0].data_ptr() if copy else 0,
+                              kept.data_ptr(), room.data_ptr(), 0 if codes is None else codes.data_ptr(),
+                              0 if copy is None else copy.data_ptr(),
                               0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
                               stream_of(dev.index))
             if want and _lib().tkl_backward(args) != 0:
@@ -231,7 +255,7 @@ def _autograd():
     return _function
 
 
-def _check(what: str, x, w, reduction: str) -> _Plan:
+def _check(what: str, x, w, reduction: str, keep: Optional[bool]) -> _Plan:
     import torch
 
     dtype = x.dtype
@@ -250,6 +274,8 @@ def _check(what: str, x, w, reduction: str) -> _Plan:
     plan.n = plan.lead.numel()
     plan.reduction = REDUCTIONS[reduction]
     plan.f16 = dtype is torch.float16
+    plan.keep = (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+                 and (keeps(plan.n, plan.d, plan.v) if keep is None else bool(keep)))
     if not (1 <= plan.d <= MAX_WIDTH and 1 <= plan.v <= MAX_VOCAB and plan.n <= MAX_TOKENS):
         raise LossError(f"{what}: {plan.n} tokens of width {plan.d} over {plan.v} entries (at most {MAX_TOKENS}, "
                         f"{MAX_WIDTH}, {MAX_VOCAB})")
@@ -270,7 +296,8 @@ def _ids(what: str, name: str, ids, x, dims: int):
     return ids.to(torch.int64).contiguous()
 
 
-def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: str = "mean"):
+def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: str = "mean",
+                         keep_logits: Optional[bool] = None):
     """Softmax cross entropy of the logits ``x @ w.T`` against ``target``, in fp32.
 
     ``x [..., D]`` and ``w [V, D]`` are both bf16 or both fp16, of any strides (rows that are
@@ -278,14 +305,18 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
     target is ``ignore_index`` has loss 0 and takes part in no sum, whatever its row of ``x``
     holds; a target outside the vocabulary gives that token a NaN loss (and NaN gradients).
     ``reduction`` is ``mean`` over the tokens that count (0 if none does), ``sum``, or
-    ``none`` for a loss per token.  Gradients flow to ``x`` and ``w``, once."""
-    plan = _check("linear_cross_entropy", x, w, reduction)
+    ``none`` for a loss per token.  Gradients flow to ``x`` and ``w``, once.
+
+    Between the passes 2 bytes a logit are kept where :func:`keeps` finds that faster;
+    ``keep_logits=False`` saves that memory, ``True`` spends it whatever the size."""
+    plan = _check("linear_cross_entropy", x, w, reduction, keep_logits)
     ids = _ids("linear_cross_entropy", "target", target, x, 0)
     plan.k, plan.distill, plan.temperature, plan.ignore = 1, 0, 1.0, int(ignore_index)
     return _apply(x, w, ids, None, plan)
 
 
-def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean"):
+def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean",
+                   keep_logits: Optional[bool] = None):
     """Divergence of the softmax of ``x @ w.T / temperature`` from a teacher's, times
     ``temperature ** 2``, in fp32: per token ``sum_k p_k (log p_k - log q_k)`` over the listed
     entries, with ``p`` the softmax of ``logits / temperature`` over them.
@@ -294,12 +325,12 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     (fp32, bf16 or fp16; no gradient).  An id below 0 is no entry, so lists may differ in
     length; a token without any entry (or with logits of -inf alone) has loss 0 and takes part
     in no sum.  An entry listed twice counts twice.  An id past the vocabulary makes the
-    token's loss NaN.  ``x``, ``w`` and ``reduction`` are those of
+    token's loss NaN.  ``x``, ``w``, ``reduction`` and ``keep_logits`` are those of
     :func:`linear_cross_entropy`."""
     import torch
 
     what = "linear_distill"
-    plan = _check(what, x, w, reduction)
+    plan = _check(what, x, w, reduction, keep_logits)
     ids = _ids(what, "ids", ids, x, 1)
     if not logits.is_floating_point() or logits.device != x.device or logits.shape != ids.shape:
         raise LossError(f"{what} wants logits as numbers of ids' shape on x's device, not {logits.dtype} "
