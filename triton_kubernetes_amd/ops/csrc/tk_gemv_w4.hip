@@ -42,6 +42,10 @@ struct Type<false> {
   using T = __bf16;
   static constexpr unsigned MASK = 0x00780078u, SIXTEEN = 0x41804180u, ONES = 0x3f803f80u;  // mantissa bits 3-6
   static constexpr int LOW = 3;
+  static __device__ __forceinline__ float sum2(unsigned v, float c) {  // c + both numbers
+    typedef __attribute__((ext_vector_type(2))) __bf16 t2;
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, v), __builtin_bit_cast(t2, ONES), c, false);
+  }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
@@ -52,6 +56,10 @@ struct Type<true> {
   using T = _Float16;
   static constexpr unsigned MASK = 0x03c003c0u, SIXTEEN = 0x4c004c00u, ONES = 0x3c003c00u;  // mantissa bits 6-9
   static constexpr int LOW = 6;
+  static __device__ __forceinline__ float sum2(unsigned v, float c) {
+    typedef __attribute__((ext_vector_type(2))) _Float16 t2;
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, v), __builtin_bit_cast(t2, ONES), c, false);
+  }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
@@ -161,8 +169,9 @@ struct Scales {
   __device__ __forceinline__ float scale(int q) const {
     return (float)__builtin_bit_cast(T, (uint16_t)(G ? s[q / 2] >> (q % 2 * 16) : s[q]));
   }
+  static constexpr float OFFSET = 16.f + 8.f;             // without zeros
   __device__ __forceinline__ float offset(int q) const {  // of the number that a code of zero unpacks to
-    return 16.f + (ZEROS ? (float)(G ? z[0] >> (q * 8) & 255 : z[q]) : 8.f);
+    return ZEROS ? 16.f + (float)(G ? z[0] >> (q * 8) & 255 : z[q]) : OFFSET;
   }
 };
 
@@ -358,6 +367,13 @@ hipError_t one(const void* x, long long ldx, const uint8_t* codes, const void* s
 // of W a workgroup for more than 16 rows of x keep that to as much as the codes.  The columns
 // are split over blockIdx.y: each split writes its own fp32 sums (`part`), which k_join adds in
 // order; a single split writes y.
+template <int SPC, int MT>
+constexpr int XBytes = 32 * 16 * MT * 16 + 2 * SPC * 16 * MT * 4;  // a stage of x, and its sums
+template <int CTRL>
+__device__ __forceinline__ float add_lanes(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 15, 15, true));
+}
+
 template <bool F16, int G, bool ZEROS, int MT, int RT>
 __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, const uint8_t* codes, const void* scales,
                                                const uint8_t* zeros, void* y, long long ldy, int m, int n, int k,
@@ -365,13 +381,13 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
   using Y = Type<F16>;
   using T = typename Y::T;
   using Sc = Scales<F16, G, ZEROS>;
-  constexpr int STEPS = 4 / Sc::SPC, ROWS = 16 * MT, SLOT = RT * 2048, COPIES = 2 * RT;
+  constexpr int STEPS = 4 / Sc::SPC, ROWS = 16 * MT, SLOT = RT * 2048, COPIES = 2 * RT, XB = XBytes<Sc::SPC, MT>, AHEAD = 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane >> 4, r = lane & 15;
   const int row0 = (blockIdx.x * 8 + wave) * 16 * RT, groups = k / group, per_group = group / CHUNK;
   const int chunks = (k + CHUNK - 1) / CHUNK, c0 = blockIdx.y * per, c1 = min(chunks, c0 + per);
-  char* mine = smem + 2 * 32 * ROWS * 16 + wave * 3 * SLOT;
+  char* mine = smem + 2 * XB + wave * AHEAD * SLOT;
   const uint64_t at0 = reinterpret_cast<uint64_t>(codes) + (uint64_t)min(row0, n - 1) * (k / 2);
   const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((unsigned)(at0 >> 32)) << 32 |
                         (unsigned)__builtin_amdgcn_readfirstlane((unsigned)at0);
@@ -409,8 +425,18 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
   auto store_x = [&](int c, char* xb) {
     const bool there = c * CHUNK + (tid & 31) * 8 < k;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-      *reinterpret_cast<u32x4*>(xb + to + i * 256) = there ? pairs(xr[i]) : u32x4{0, 0, 0, 0};
+    for (int i = 0; i < MT; ++i) {
+      const u32x4 v = there ? pairs(xr[i]) : u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(xb + to + i * 256) = v;
+      // the sum of x over the 4 units of each column block of 32, or over all of a scale's
+      float s = Y::sum2(v[0], Y::sum2(v[1], Y::sum2(v[2], Y::sum2(v[3], 0.f))));
+      s = add_lanes<0xb1>(s);                              // 1 lane apart
+      s = add_lanes<0x4e>(s);                              // 2
+      if constexpr (Sc::SPC < 4) s = add_lanes<0x141>(s);  // the other 4 of 8
+      if constexpr (Sc::SPC < 2) s = add_lanes<0x140>(s);  // the other 8 of 16
+      if (tid % (16 / Sc::SPC) == 0)
+        reinterpret_cast<float*>(xb + 32 * ROWS * 16)[(tid & 31) / (16 / Sc::SPC) * ROWS + (tid >> 5) + i * 16] = s;
+    }
   };
 
   f32x4 total[RT][MT];
@@ -418,12 +444,11 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
   for (int a = 0; a < RT; ++a)
 #pragma unroll
     for (int t = 0; t < MT; ++t) total[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const u32x4 ones = {Y::ONES, Y::ONES, Y::ONES, Y::ONES};
   const int lane_at = r * 128 + (r >> 1 & 7) * 16 + j * 4;
 
   const int stages = (c1 - c0 + 1) / 2;
   auto chunk_of = [&](int i) { return i < stages ? c0 + 2 * i : 1 << 20; };  // past the last stage nothing is read
-  Sc f[3];
+  Sc f[AHEAD];
   copy(chunk_of(0), 0);
   f[0] = fetch(chunk_of(0));
   load_x(min(chunk_of(0), chunks - 1));
@@ -431,34 +456,21 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
   copy(chunk_of(1), 1);
   f[1] = fetch(chunk_of(1));
   int buf = 0;
-  for (int i = 0; i < stages; i += 3) {
+  for (int i = 0; i < stages; i += AHEAD) {
 #pragma unroll
-    for (int slot = 0; slot < 3; ++slot) {
+    for (int slot = 0; slot < AHEAD; ++slot) {
       if (i + slot >= stages) break;
       const int at = chunk_of(i + slot);
       // loads return in order: the codes of this stage are older than its x, and of what is in
       // flight only the next stage's codes and scales are younger
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES + Sc::LOADS) : "memory");
-      char* xb = smem + buf * 32 * ROWS * 16;
+      char* xb = smem + buf * XB;
       store_x(at, xb);
       load_x(min(chunk_of(i + slot + 1), chunks - 1));
-      asm volatile("" ::: "memory");
-      const Sc now = f[slot];
-      copy(chunk_of(i + slot + 2), (slot + 2) % 3);
-      f[(slot + 2) % 3] = fetch(chunk_of(i + slot + 2));
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");  // the barrier alone does not hold the compiler's loads back
-      const char* img = mine + slot * SLOT;
       // all codes of the stage, and x one step ahead of the matrix instructions: left to itself
       // the compiler reads right before each use and waits every time
+      const char* img = mine + slot * SLOT;
       unsigned w[2][4][RT];
-      u32x4 xa[2][MT];
-      auto read_x = [&](int u, int s, u32x4* to) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          to[t] = *reinterpret_cast<const u32x4*>(xb + from[s] + u * 16 * ROWS * 16 + t * 256);
-      };
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -466,12 +478,26 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
 #pragma unroll
           for (int a = 0; a < RT; ++a)
             w[u][s][a] = *reinterpret_cast<const unsigned*>(img + a * 2048 + (lane_at ^ ((u * 4 + s) * 16)));
+      const Sc now = f[slot];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // x is written, and the codes' slot has been read
+      copy(chunk_of(i + slot + AHEAD), slot);
+      f[slot] = fetch(chunk_of(i + slot + AHEAD));
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");  // the barrier alone does not hold the compiler's loads back
+      u32x4 xa[2][MT];
+      auto read_x = [&](int u, int s, u32x4* to) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          to[t] = *reinterpret_cast<const u32x4*>(xb + from[s] + u * 16 * ROWS * 16 + t * 256);
+      };
       read_x(0, 0, xa[0]);
       Sc v[2][RT];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int a = 0; a < RT; ++a) v[u][a] = now.of(((a * 2 + u) * 16 + r) * 4, min(at + u, chunks - 1), groups);
+      const float* xsum = reinterpret_cast<const float*>(xb + 32 * ROWS * 16) + j * 4;
       f32x4 part[RT][MT], sum[MT];
 #pragma unroll
       for (int us = 0; us < 8; ++us) {  // a chunk past the row's end has zeros in x
@@ -485,11 +511,12 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
         for (int t = 0; t < MT; ++t) {
           const u32x4 x8 = xa[us & 1][t];
           if (s % STEPS == 0) {
-            sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            // without zeros every code's offset is the same, so the sums can start at it
+            sum[t] = *reinterpret_cast<const f32x4*>(xsum + us / STEPS * ROWS + t * 16);
+            if constexpr (!ZEROS) sum[t] *= -Sc::OFFSET;
 #pragma unroll
-            for (int a = 0; a < RT; ++a) part[a][t] = sum[t];
+            for (int a = 0; a < RT; ++a) part[a][t] = ZEROS ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[t];
           }
-          sum[t] = Y::mfma(x8, ones, sum[t]);
 #pragma unroll
           for (int a = 0; a < RT; ++a) part[a][t] = Y::mfma(x8, b[a], part[a][t]);
         }
@@ -501,7 +528,8 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) total[a][t][e] += sc * (part[a][t][e] - off * sum[t][e]);
+              for (int e = 0; e < 4; ++e)
+                total[a][t][e] += sc * (ZEROS ? part[a][t][e] - off * sum[t][e] : part[a][t][e]);
           }
         }
       }
@@ -539,7 +567,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
 template <bool F16, int G, bool ZEROS, int MT, int RT>
 hipError_t batch_as(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros,
                     void* y, long long ldy, int m, int n, int k, int group, int splits, float* part, hipStream_t s) {
-  constexpr size_t lds = 2 * 32 * 16 * MT * 16 + 8 * 3 * RT * 2048;
+  constexpr size_t lds = 2 * XBytes<Scales<F16, G, ZEROS>::SPC, MT> + 8 * 2 * RT * 2048;
   const int chunks = (k + CHUNK - 1) / CHUNK, per = ((chunks + splits - 1) / splits + 1) / 2 * 2;
   const dim3 grid((n + 128 * RT - 1) / (128 * RT), splits);
   k_batch<F16, G, ZEROS, MT, RT><<<grid, 512, lds, s>>>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, per,
