@@ -423,19 +423,24 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
 #pragma unroll
   for (int s = 0; s < 4; ++s) from[s] = ((s * 4 + j) * ROWS + (r ^ (s * 4 + j))) * 16;
   auto store_x = [&](int c, char* xb) {
-    const bool there = c * CHUNK + (tid & 31) * 8 < k;
+    if (c * CHUNK + 2 * CHUNK > k && c * CHUNK + (tid & 31) * 8 >= k) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xr[i] = u32x4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const u32x4 v = there ? pairs(xr[i]) : u32x4{0, 0, 0, 0};
+      const u32x4 v = pairs(xr[i]);
       *reinterpret_cast<u32x4*>(xb + to + i * 256) = v;
-      // the sum of x over the 4 units of each column block of 32, or over all of a scale's
+      // the sum of x over a scale's columns: units of 8 lie in neighbouring lanes.  Without zeros
+      // every code has the same offset, and the matrix instructions start at -offset sum x
       float s = Y::sum2(v[0], Y::sum2(v[1], Y::sum2(v[2], Y::sum2(v[3], 0.f))));
       s = add_lanes<0xb1>(s);                              // 1 lane apart
       s = add_lanes<0x4e>(s);                              // 2
       if constexpr (Sc::SPC < 4) s = add_lanes<0x141>(s);  // the other 4 of 8
       if constexpr (Sc::SPC < 2) s = add_lanes<0x140>(s);  // the other 8 of 16
       if (tid % (16 / Sc::SPC) == 0)
-        reinterpret_cast<float*>(xb + 32 * ROWS * 16)[(tid & 31) / (16 / Sc::SPC) * ROWS + (tid >> 5) + i * 16] = s;
+        reinterpret_cast<float*>(xb + 32 * ROWS * 16)[(tid & 31) / (16 / Sc::SPC) * ROWS + (tid >> 5) + i * 16] =
+            ZEROS ? s : s * -Sc::OFFSET;
     }
   };
 
@@ -485,54 +490,66 @@ __global__ __launch_bounds__(512) void k_batch(const void* x, long long ldx, con
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");  // the barrier alone does not hold the compiler's loads back
-      u32x4 xa[2][MT];
+      u32x4 xa[2][MT], b[2][RT];
       auto read_x = [&](int u, int s, u32x4* to) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
           to[t] = *reinterpret_cast<const u32x4*>(xb + from[s] + u * 16 * ROWS * 16 + t * 256);
       };
       read_x(0, 0, xa[0]);
+#pragma unroll
+      for (int a = 0; a < RT; ++a) b[0][a] = unpack<F16>(w[0][0][a]);
       Sc v[2][RT];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int a = 0; a < RT; ++a) v[u][a] = now.of(((a * 2 + u) * 16 + r) * 4, min(at + u, chunks - 1), groups);
       const float* xsum = reinterpret_cast<const float*>(xb + 32 * ROWS * 16) + j * 4;
-      f32x4 part[RT][MT], sum[MT];
+      f32x4 part[2][RT][MT], sum[2][MT];
+      // the sums of group g (of a scale's columns) for x's tile t, into the result
+      auto finish = [&](int g, int t) {
+#pragma unroll
+        for (int a = 0; a < RT; ++a) {
+          const float sc = v[g / Sc::SPC][a].scale(g % Sc::SPC), off = v[g / Sc::SPC][a].offset(g % Sc::SPC);
+          const f32x4 p = part[g & 1][a][t];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) total[a][t][e] += sc * (ZEROS ? p[e] - off * sum[g & 1][t][e] : p[e]);
+        }
+      };
 #pragma unroll
       for (int us = 0; us < 8; ++us) {  // a chunk past the row's end has zeros in x
-        const int u = us / 4, s = us % 4;
-        if (us < 7) read_x((us + 1) / 4, (us + 1) % 4, xa[(us + 1) & 1]);
+        const int g = us / STEPS, step = us % STEPS;
         __builtin_amdgcn_sched_barrier(0);
-        u32x4 b[RT];
-#pragma unroll
-        for (int a = 0; a < RT; ++a) b[a] = unpack<F16>(w[u][s][a]);
+        if (us < 7) read_x((us + 1) / 4, (us + 1) % 4, xa[(us + 1) & 1]);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          const u32x4 x8 = xa[us & 1][t];
-          if (s % STEPS == 0) {
-            // without zeros every code's offset is the same, so the sums can start at it
-            sum[t] = *reinterpret_cast<const f32x4*>(xsum + us / STEPS * ROWS + t * 16);
-            if constexpr (!ZEROS) sum[t] *= -Sc::OFFSET;
+          if (step == 0) {
+            sum[g & 1][t] = *reinterpret_cast<const f32x4*>(xsum + g * ROWS + t * 16);
 #pragma unroll
-            for (int a = 0; a < RT; ++a) part[a][t] = ZEROS ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[t];
+            for (int a = 0; a < RT; ++a) part[g & 1][a][t] = ZEROS ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[g & 1][t];
           }
 #pragma unroll
-          for (int a = 0; a < RT; ++a) part[a][t] = Y::mfma(x8, b[a], part[a][t]);
+          for (int a = 0; a < RT; ++a) part[g & 1][a][t] = Y::mfma(xa[us & 1][t], b[us & 1][a], part[g & 1][a][t]);
         }
-        if ((s + 1) % STEPS == 0) {
-          const int q = s / STEPS;
+        // meanwhile the vector unit unpacks the next step's codes and scales the last group's sums
+        if (us < 7) {
 #pragma unroll
-          for (int a = 0; a < RT; ++a) {
-            const float sc = v[u][a].scale(q), off = v[u][a].offset(q);
+          for (int a = 0; a < RT; ++a) b[(us + 1) & 1][a] = unpack<F16>(w[(us + 1) / 4][(us + 1) % 4][a]);
+        }
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < MT; ++t)
+          if (g && t * STEPS / MT == step) finish(g - 1, t);
+        if constexpr (MT * RT >= 4) {
+          __builtin_amdgcn_sched_group_barrier(0x100, MT, 0);  // reads of LDS
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                total[a][t][e] += sc * (ZEROS ? part[a][t][e] - off * sum[t][e] : part[a][t][e]);
+          for (int i = 0; i < MT * RT; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                          // a matrix instruction,
+            __builtin_amdgcn_sched_group_barrier(0x002, (RT * 8 + MT * RT) / (MT * RT) + 1, 0);  // vector ones
           }
         }
       }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) finish(2 * Sc::SPC - 1, t);
       buf ^= 1;
     }
   }
