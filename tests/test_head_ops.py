@@ -103,8 +103,15 @@ def test_gemv_refuses_inputs():
     (1, 4, 64, 64, 32, 4, 4096, 4096), (1, 4, 64, 64, 68, 4, 4096, 4096), (1, 4, 64, 64, 64, 4, 4098, 4096),
     (1, 4, 64, 64, 64, 4, 4096, 4104), (1, 4, 64, 64, 64, 3, 4096, 4096)])
 def test_the_gemv_c_entry_checks_before_the_gpu(m, n, k, group, ldx, ldy, x, codes):
-    assert gemv._lib().tkv_gemv_w4(0, 0, x, ldx, codes, 4096, None, 4096, ldy, m, n, k, group, 1, None, None) == -1
-    assert gemv._lib().tkv_last_error()
+    lib = gemv._lib()
+    assert lib.tkv_gemv_w4(gemv._ARGS.pack(0, 0, m, n, k, group, 1, ldx, ldy, x, codes, 4096, 0, 4096, 0, 0)) == -1
+    assert lib.tkv_last_error()
+
+
+def test_the_gemv_c_entry_checks_its_splits():
+    for splits in (-1, 2, 65):  # 2 without room for the sums
+        assert gemv._lib().tkv_gemv_w4(gemv._ARGS.pack(0, 0, 1, 4, 64, 64, splits, 64, 4, 4096, 4096, 4096, 0, 4096, 0, 0)) == -1
+        assert b"splits" in gemv._lib().tkv_last_error()
 
 
 def test_pack_and_quantize_refuse():

@@ -624,14 +624,26 @@ int refuse(const char* why) {
 
 }  // namespace
 
-// y[m][n] = x[m][k] W^T, queued on `stream` of device `dev`; nothing waits for it.  codes
-// [n][k/2] (the lower half of a byte first), scales [n][k/group] of x's type, zeros
-// [n][k/group] bytes or null for 8.  splits 0: each row of x by itself, k_one; else together,
-// k_batch, the columns split, and `part` holds splits x m x n fp32 sums.  0, or -1 / a HIP error
-// with tkv_last_error() set.
-extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const void* codes, const void* scales,
-                           const void* zeros, void* y, long long ldy, int m, int n, int k, int group, int splits,
-                           void* part, void* stream) {
+// One call's tensors and sizes (ops/gemv.py packs the same fields in the same order).
+struct tkv_args {
+  int dev, f16, m, n, k, group;
+  int splits;            // 0: each row of x by itself, k_one; else together, k_batch, the columns split
+  long long ldx, ldy;    // row strides, elements
+  const void *x, *codes, *scales;  // codes [n][k/2], the lower half of a byte first; scales [n][k/group] of x's type
+  const void* zeros;     // [n][k/group] bytes, or null for 8
+  void *y, *part;        // part: splits x m x n fp32 sums
+  void* stream;
+};
+
+extern "C" int tkv_args_size() { return (int)sizeof(tkv_args); }
+
+// y[m][n] = x[m][k] W^T, queued on a->stream; nothing waits for it.  0, or -1 / a HIP error with
+// tkv_last_error() set.
+extern "C" int tkv_gemv_w4(const tkv_args* a) {
+  const int dev = a->dev, m = a->m, n = a->n, k = a->k, group = a->group, splits = a->splits;
+  const long long ldx = a->ldx, ldy = a->ldy;
+  const void *x = a->x, *codes = a->codes, *scales = a->scales, *zeros = a->zeros;
+  void *y = a->y, *part = a->part;
   if (m < 1 || m > 64) return refuse("1 to 64 rows of x");
   if (n < 1 || n > (1 << 24)) return refuse("1 to 2^24 rows of weights");
   if (group < 32 || group % 32 || k < group || k % group || k > (1 << 20))
@@ -644,11 +656,11 @@ extern "C" int tkv_gemv_w4(int dev, int f16, const void* x, long long ldx, const
   hipError_t e = hipGetDevice(&prev);
   if (e == hipSuccess && prev != dev) e = hipSetDevice(dev);
   if (e == hipSuccess) {
-    const auto s = static_cast<hipStream_t>(stream);
+    const auto s = static_cast<hipStream_t>(a->stream);
     const auto *c = static_cast<const uint8_t*>(codes), *z = static_cast<const uint8_t*>(zeros);
     float* p = static_cast<float*>(part);
-    e = f16 ? launch<true>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, splits == 0, s)
-            : launch<false>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, splits == 0, s);
+    e = a->f16 ? launch<true>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, splits == 0, s)
+               : launch<false>(x, ldx, c, scales, z, y, ldy, m, n, k, group, splits, p, splits == 0, s);
     if (prev != dev) {
       const hipError_t back = hipSetDevice(prev);
       if (e == hipSuccess) e = back;

@@ -10,9 +10,10 @@ and undo them, on any device.
 
 import ctypes
 import math
+import struct
 from typing import Any, Optional, Tuple
 
-from .native import load
+from .native import NativeUnavailable, load
 
 MAX_ROWS = 64
 MAX_OUT = 1 << 24
@@ -23,6 +24,10 @@ SYMMETRIC_ZERO = 8  # the zero of weights without zeros
 class GemvError(RuntimeError):
     pass
 
+
+# struct tkv_args of csrc/tk_gemv_w4.hip: dev f16 m n k group splits, ldx ldy, x codes scales zeros
+# y part stream
+_ARGS = struct.Struct("@7i2q7P")
 
 _loaded = None
 
@@ -35,8 +40,9 @@ def _lib():
         require_torch_first()
         lib = load("libtk_gemv.so")
         lib.tkv_last_error.restype = ctypes.c_char_p
-        i, ll, p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
-        lib.tkv_gemv_w4.argtypes = [i, i, p, ll, p, p, p, p, ll, i, i, i, i, i, p, p]
+        lib.tkv_gemv_w4.argtypes = [ctypes.c_char_p]
+        if lib.tkv_args_size() != _ARGS.size:
+            raise NativeUnavailable("libtk_gemv.so does not match ops/gemv.py: run `python -m triton_kubernetes_amd.ops.build`")
         _loaded = lib
     return _loaded
 
@@ -45,13 +51,15 @@ def _check_weight(codes, scales, zeros) -> Tuple[int, int, int]:
     """``(n, k, group)`` of a packed weight."""
     import torch
 
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0]:
+    shape, by = codes.shape, scales.shape
+    if codes.dtype is not torch.uint8 or len(shape) != 2 or len(by) != 2 or by[0] != shape[0]:
         raise GemvError(f"wants codes uint8 [N, K/2] and scales [N, K/group], not {codes.dtype} {list(codes.shape)} "
                         f"and {list(scales.shape)}")
-    n, k, groups = codes.shape[0], codes.shape[1] * 2, scales.shape[1]
-    if not groups or not k or k % groups or (k // groups) % 32:
+    n, half = shape
+    k, groups = half * 2, by[1]
+    if not groups or not k or k % groups or k // groups % 32:
         raise GemvError(f"{groups} groups do not divide {k} columns into groups of a multiple of 32")
-    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+    if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != by):
         raise GemvError(f"wants zeros uint8 {list(scales.shape)}, not {zeros.dtype} {list(zeros.shape)}")
     return n, k, k // groups
 
@@ -92,10 +100,10 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
     ``codes`` is uint8 ``[N, K/2]``, two codes to a byte, the lower half first; ``scales``
     ``[N, K/group]`` has ``x``'s type, ``zeros`` (uint8, the same shape) may be left out for
     symmetric weights, whose zero is 8.  The weight's tensors are contiguous; ``group`` is a
-    multiple of 32.  Sums are fp32 and rounded once; they are of ``(16 + code) * x``, so an infinite
-    ``x`` gives NaN.  The result (``out``, if given: contiguous,
-    ``[..., N]``) has ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that
-    wants one is refused."""
+    multiple of 32.  Sums are fp32 and rounded once; they are of ``(16 + code) * x``, so an
+    infinite ``x`` gives NaN.  The result (``out``, if given: contiguous, ``[..., N]``) has
+    ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that wants one is
+    refused."""
     import torch
 
     dtype = x.dtype
@@ -107,20 +115,21 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
         raise GemvError(f"x {list(shape)} does not go with {k} columns")
     if n > MAX_OUT or k > MAX_IN:
         raise GemvError(f"a weight of {n} x {k} (at most {MAX_OUT} x {MAX_IN})")
-    dev = x.device
-    if not x.is_cuda or codes.device != dev or scales.device != dev or (zeros is not None and zeros.device != dev):
+    dev = x.get_device()
+    if dev < 0 or codes.get_device() != dev or scales.get_device() != dev or (zeros is not None and zeros.get_device() != dev):
         raise GemvError("gemv_w4 wants CUDA tensors on one device")
-    if not (codes.is_contiguous() and scales.is_contiguous() and (zeros is None or zeros.is_contiguous())) \
-            or codes.data_ptr() % 16:
+    at = codes.data_ptr()
+    if at % 16 or not (codes.is_contiguous() and scales.is_contiguous() and (zeros is None or zeros.is_contiguous())):
         raise GemvError("gemv_w4 wants a contiguous weight, its codes 16-byte aligned")
     if (x.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
         raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
-    m = x.numel() // k
+    flat = len(shape) == 2
+    m = shape[0] if flat else x.numel() // k
     if m > MAX_ROWS:
         raise GemvError(f"{m} rows of x (at most {MAX_ROWS}): dequantize_w4 and a matrix product serve more")
     if out is None:
-        out = torch.empty((*shape[:-1], n), dtype=dtype, device=dev)
-    elif out.shape != (*shape[:-1], n) or out.dtype is not dtype or out.device != dev or not out.is_contiguous():
+        out = x.new_empty((m, n) if flat else (*shape[:-1], n))
+    elif out.shape != (*shape[:-1], n) or out.dtype is not dtype or out.device != x.device or not out.is_contiguous():
         raise GemvError(f"out must be contiguous {dtype} {[*shape[:-1], n]} on x's device")
     elif any(_overlap(out, t) for t in (x, codes, scales, zeros) if t is not None):
         raise GemvError("out must not share memory with x or the weight")
@@ -128,19 +137,22 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
         raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
     if m == 0 or n == 0:
         return out
-    if len(shape) != 2:
+    if not flat:
         x = x.reshape(m, k)
-    ldx = x.stride(0)
-    if x.stride(1) != 1 or ldx < k or ldx % 8 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
+    ldx, step = x.stride()
+    if m == 1:
         ldx = k
+    from_x = x.data_ptr()
+    if step != 1 or ldx < k or ldx % 8 or from_x % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        ldx, from_x = k, x.data_ptr()
     parts = splits(m, n, k)
-    room = torch.empty((parts, m, n), dtype=torch.float32, device=dev) if parts > 1 else None
-    rc = _lib().tkv_gemv_w4(dev.index, dtype is torch.float16, x.data_ptr(), ldx, codes.data_ptr(), scales.data_ptr(),
-                            None if zeros is None else zeros.data_ptr(), out.data_ptr(), n, m, n, k, group, parts,
-                            None if room is None else room.data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
-    if rc != 0:
-        raise GemvError(_lib().tkv_last_error().decode())
+    room = x.new_empty((parts, m, n), dtype=torch.float32) if parts > 1 else None
+    lib = _loaded or _lib()
+    if lib.tkv_gemv_w4(_ARGS.pack(dev, dtype is torch.float16, m, n, k, group, parts, ldx, n, from_x, at, scales.data_ptr(),
+                                  0 if zeros is None else zeros.data_ptr(), out.data_ptr(),
+                                  0 if room is None else room.data_ptr(), torch._C._cuda_getCurrentRawStream(dev))) != 0:
+        raise GemvError(lib.tkv_last_error().decode())
     return out
 
 
