@@ -190,7 +190,7 @@ def _autograd():
             dev = x.device
             n, d, v, k = plan.n, plan.d, plan.v, plan.k
             ctx.plan = plan
-            loss = torch.empty(() if plan.reduction else plan.lead, dtype=torch.float32, device=dev)
+            loss = x.new_empty(() if plan.reduction else plan.lead, dtype=torch.float32)
             if n == 0 or k == 0:  # nothing has a loss
                 ctx.save_for_backward(x, w)
                 return loss.zero_()
@@ -201,9 +201,9 @@ def _autograd():
             plan.small = small_products(n, d, v)
             plain = _row_strided(w)
             copy = _room_for_copy(plain)
-            kept = torch.empty(kept_bytes(n, d, n * k if plan.distill else 0), dtype=torch.uint8, device=dev)
+            kept = x.new_empty(kept_bytes(n, d, n * k if plan.distill else 0), dtype=torch.uint8)
             small = bool(plan.small & 1)
-            room = torch.empty((codes_bytes if plan.keep else part_bytes)(n, v, small), dtype=torch.uint8, device=dev)
+            room = x.new_empty((codes_bytes if plan.keep else part_bytes)(n, v, small), dtype=torch.uint8)
             args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
                               plan.distill, plan.reduction, plan.temperature, 0, plan.small, x.data_ptr(),
                               plain.data_ptr(), ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0,
@@ -234,10 +234,9 @@ def _autograd():
             plain = _row_strided(w) if copy is None else copy
             piece = pieces(n, v)
             groups = fill(bool(plan.small & 2))
-            room = torch.empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill),
-                               dtype=torch.uint8, device=dev)
-            dx = torch.empty((n, d), dtype=w.dtype, device=dev) if want & 1 else None
-            dw = torch.empty((v, d), dtype=w.dtype, device=dev) if want & 2 else None
+            room = kept.new_empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill))
+            dx = w.new_empty((n, d)) if want & 1 else None
+            dw = w.new_empty((v, d)) if want & 2 else None
             args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
                               piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
                               want, plan.small, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
@@ -293,7 +292,7 @@ def _ids(what: str, name: str, ids, x, dims: int):
     lead = x.shape[:-1]
     if ids.dim() != len(lead) + dims or ids.shape[:len(lead)] != lead:
         raise LossError(f"{what}: {name} {list(ids.shape)} does not go with x {list(x.shape)}")
-    return ids.to(torch.int64).contiguous()
+    return ids if ids.dtype is torch.int64 and ids.is_contiguous() else ids.to(torch.int64).contiguous()
 
 
 def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: str = "mean",
