@@ -87,6 +87,8 @@ constexpr int FEW_ROWS = 512;
 struct Big {  // 8 waves, the schedule of product_big
   static constexpr int BM = 256, BN = 256, THREADS = 512, MF = 8, NF = 4, WAVES_M = 2,
                        LDS = 256 * (256 * 2 + 16) + 4096;  // the tile on its way out and sums; steps take 128 KiB
+  static constexpr int SLOTS = 256;         // workgroups at a time
+  static constexpr float SUM_COST = 4.3f;  // of a tile's sums: 116 ns, to 27 ns for a K step of 1
   static __device__ __forceinline__ int wave_m(int wid) { return wid >> 2; }
   static __device__ __forceinline__ int row(int mf, int wid) { return (mf >> 2) * 128 + (wid >> 2) * 64 + (mf & 3) * 16; }
   static __device__ __forceinline__ int col(int nf, int wid) { return (nf >> 1) * 128 + (wid & 3) * 32 + (nf & 1) * 16; }
@@ -95,6 +97,8 @@ struct Big {  // 8 waves, the schedule of product_big
 struct Small {  // 4 waves, STEPS steps in LDS, two workgroups to a compute unit: for few tokens
   static constexpr int BM = 128, BN = 64, THREADS = 256, MF = 2, NF = 4, WAVES_M = 4, STEPS = 3,
                        LDS = STEPS * (BM + BN) * KT * 2;
+  static constexpr int SLOTS = 512;
+  static constexpr float SUM_COST = 1.f;
   static __device__ __forceinline__ int wave_m(int wid) { return wid; }
   static __device__ __forceinline__ int row(int mf, int wid) { return wid * 32 + mf * 16; }
   static __device__ __forceinline__ int col(int nf, int) { return nf * 16; }
@@ -535,10 +539,10 @@ struct Upstream {
 // value, joins the rounding of dl to bf16, 3.9e-3, or to fp16, 4.9e-4, whose numbers run out at
 // 2^-29 of the largest (struct Upstream).
 struct Codes {
-  static __device__ __forceinline__ unsigned pack(float a, float b) {  // distances
-    auto code = [](float d) {  // the least of the three lines, of 65535
-      constexpr float S = 4096.f / 65535.f;
-      return fminf(fminf(d * S, __builtin_fmaf(d, S / 4, 24576.f / 65535.f)), __builtin_fmaf(d, S / 32, 46080.f / 65535.f));
+  static constexpr float UNIT = 4096.f / 65535.f;  // a distance of 1, of the largest code
+  static __device__ __forceinline__ unsigned pack(float a, float b) {  // distances, in UNITs
+    auto code = [](float d) {  // the least of the three lines
+      return fminf(fminf(d, __builtin_fmaf(d, 1.f / 4, 24576.f / 65535.f)), __builtin_fmaf(d, 1.f / 32, 46080.f / 65535.f));
     };
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(code(a), code(b)));
   }
@@ -624,11 +628,12 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
         float m = sums[col].x;
 #pragma unroll
         for (int o = 1; o < Tile::WAVES_M; ++o) m = fmaxf(m, sums[o * Tile::BN + col].x);
+        m *= Codes::UNIT;
 #pragma unroll
         for (int i = 0; i < Tile::MF; ++i) {
           float d[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[e] = __builtin_fmaf(acc[i][j][e], -sc, m);
+          for (int e = 0; e < 4; ++e) d[e] = __builtin_fmaf(acc[i][j][e], -sc * Codes::UNIT, m);
           Outgoing<Tile, T>::put(smem, col, Tile::row(i, wid) + fq * 4, Codes::pack(d[0], d[1]), Codes::pack(d[2], d[3]));
         }
       }
@@ -706,13 +711,25 @@ __global__ __launch_bounds__(256) void k_dl(const unsigned short* __restrict__ c
   *reinterpret_cast<u32x4*>(static_cast<T*>(dl) + pos * lddl + c) = out;
 }
 
-// Into how many parts the vocabulary is split for dX of `rows` packed rows: as many as `fill`
-// workgroups have tiles for, at least 512 entries of a piece each.  Only the device knows `rows`.
+// Into how many parts the vocabulary is split for dX of `rows` packed rows, so that the last round
+// of tiles over the compute units is as full as the others: of the most parts that 1, 2 or 3 rounds
+// hold (`fill` workgroups at most, 512 entries of a piece or more each) those that cost least, a
+// round's products and a tile's fp32 sums, written and read once more.  Only the device knows `rows`.
 template <class Tile>
-__host__ __device__ __forceinline__ int splits_of(int rows, int d, int fill, int piece) {
+__device__ __forceinline__ int splits_of(int rows, int d, int fill, int piece) {
   const int tiles = ((d + Tile::BM - 1) / Tile::BM) * ((rows + Tile::BN - 1) / Tile::BN);
-  const int s = tiles ? fill / tiles : 1, most = piece / 512;
-  return s < 1 || most < 1 ? 1 : s < most ? s : most;
+  const int most = tiles ? min(fill / tiles, piece / 512) : 1;
+  int best = 1;
+  float least = INFINITY;
+  for (int round = 1; round <= 3; ++round) {
+    const int s = max(1, min(round * Tile::SLOTS / max(tiles, 1), most));
+    const float cost = (float)((tiles * s + Tile::SLOTS - 1) / Tile::SLOTS) * piece / s + Tile::SUM_COST * tiles * s;
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 // dX^T tile: A = W (K = vocabulary, down the rows), B = dl (K along the rows).  Each split owns

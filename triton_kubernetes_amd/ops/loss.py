@@ -101,10 +101,10 @@ def keeps(n: int, d: int, v: int) -> bool:
 
 
 def fill(small: bool) -> int:
-    """Workgroups for x's gradient, among which the vocabulary is split where there are fewer tiles:
-    a large tile for each of the 256 compute units (more only cost joining: 2048 x 2048 x 65536,
-    472 us with 256, 516 with 512), or two small ones."""
-    return 512 if small else 256
+    """Most workgroups for x's gradient, among which the vocabulary is split: 3 rounds of a large
+    tile for each of the 256 compute units (a step of 5000 x 4000 x 32768, 320 tiles: 3906 us with
+    one round, 3517 with 3, 3472 with 5), or one of two small ones."""
+    return 512 if small else 768
 
 
 def kept_bytes(n: int, d: int, lists: int) -> int:
