@@ -586,3 +586,21 @@ def test_keep_logits_decides_what_stays_between_the_passes():
             before = torch.cuda.memory_allocated()
             loss = call(keep_logits=True)  # without a backward pass nothing is kept
             assert torch.cuda.memory_allocated() - before < 2 * n * v
+
+
+@pytest.mark.parametrize("n,d,v,masked", [(300, 136, 70, 0.0), (2049, 72, 300, 0.0), (1500, 77, 130, 0.7),
+                                          (1500, 77, 130, 1.0), (4096, 256, 64, 0.98)])
+@pytest.mark.parametrize("dt", DTYPES, ids=NAMES.get)
+def test_weight_gradient_in_parts(n, d, v, masked, dt, monkeypatch):
+    """Tokens split for w's gradient, parts without any token among them."""
+    from triton_kubernetes_amd.ops import loss
+
+    gen = _gen(28, n, d)
+    x, w, t = _inputs(n, d, v, dt, gen)
+    t[torch.rand(n, device="cuda", generator=gen) < masked] = -100
+    call = lambda x, w: loss.linear_cross_entropy(x, w, t, reduction="none")  # noqa: E731
+    monkeypatch.setattr(loss, "small_products", lambda *a: 7)
+    assert n < 512 or loss.weight_parts(n, d, v) > 1
+    for parts in (loss.weight_parts(n, d, v), 2, 64):
+        monkeypatch.setattr(loss, "weight_parts", lambda *a, parts=parts: parts)
+        _against(call, x, w, *ref.targets_of(t, -100, n, v), gen=gen)

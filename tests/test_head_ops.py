@@ -37,7 +37,7 @@ def test_pieces_cover_the_vocabulary_within_the_workspace(n, v):
 
 
 FIELDS = ("n", "d", "v", "k", "ldx", "ldw", "ldg", "ignore", "piece", "fill", "dev", "f16", "distill", "reduction",
-          "temperature", "want", "small", "x", "w", "ids", "teacher", "grad", "loss", "kept", "room", "codes", "wc", "dx", "dw",
+          "temperature", "want", "small", "parts", "x", "w", "ids", "teacher", "grad", "loss", "kept", "room", "codes", "wc", "dx", "dw",
           "stream")
 
 
@@ -51,10 +51,12 @@ def test_buffers_have_the_sizes_that_the_kernels_take(n, d, k):
     lib = loss._lib()
     for distill in (0, 1):
         assert lib.tkl_kept_bytes(_args(n=n, d=d, k=k, distill=distill)) == loss.kept_bytes(n, d, n * k * distill)
-        for want, groups, small, piece in ((3, 256, 0, 512), (1, 512, 2, 4096), (2, 256, 0, 256), (1, 1, 0, 32768),
-                                           (3, 4096, 7, 256)):
-            args = _args(n=n, d=d, k=k, want=want, piece=piece, fill=groups, small=small, distill=distill)
-            assert lib.tkl_room_bytes(args) == loss.room_bytes(n, d, piece, groups, bool(small & 2), want, distill)
+        for want, groups, small, piece, parts in ((3, 256, 0, 512, 1), (1, 512, 2, 4096, 0), (2, 256, 0, 256, 3),
+                                                  (1, 1, 0, 32768, 1), (3, 4096, 7, 256, 64)):
+            args = _args(n=n, d=d, v=200, k=k, want=want, piece=piece, fill=groups, small=small, distill=distill,
+                         parts=parts)
+            assert lib.tkl_room_bytes(args) == loss.room_bytes(n, d, piece, groups, bool(small & 2), want, distill,
+                                                               parts * 200 if parts > 1 else 0)
 
 
 @pytest.mark.parametrize("fields,message", [
@@ -73,7 +75,8 @@ def test_the_c_entries_check_before_the_gpu(fields, message):
 
 
 @pytest.mark.parametrize("fields", [dict(piece=0), dict(piece=255), dict(piece=1 << 25), dict(fill=0), dict(fill=4097),
-                                    dict(n=300, piece=1 << 21)])
+                                    dict(n=300, piece=1 << 21), dict(parts=65), dict(parts=-1),
+                                    dict(parts=2, v=300)])
 def test_the_c_backward_checks_its_pieces(fields):
     assert loss._lib().tkl_backward(_args(**fields)) == -1
 

@@ -65,6 +65,7 @@ struct tkl_args {
   float temperature;
   int want;                    // backward: 1 dX, 2 dW, 3 both
   int small;                   // products in small tiles: 1 the logits, 2 dX, 4 dW
+  int parts;                   // backward: of the tokens for dW; more than 1 only where there is one piece
   const void *x, *w, *ids, *teacher, *grad;
   void *loss, *kept;           // kept: from forward to backward (struct Kept)
   void *room;                  // forward: the tiles' maxima and sums; backward: dl, sums of dX, factors
@@ -771,29 +772,33 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w
   }
 }
 
-// dW^T tile: A = Xc (K = tokens, down the rows), B = dl (K = tokens, down the rows).
+// dW^T tile: A = Xc (K = tokens, down the rows), B = dl (K = tokens, down the rows).  Where dW has
+// few tiles the tokens are split over blockIdx.y, and each part writes its fp32 sums [v][dp], which
+// k_dw_out adds in order (8192 x 512 x 1000, 128 tiles: 86 us whole, 26 in 4 parts).
 template <class Tile, bool F16>
 __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ xc, long long ldxc,
                                                       const void* __restrict__ dl, long long lddl, int v0, int vn,
                                                       int d, const int* __restrict__ count, Upstream<F16> up,
                                                       const int* __restrict__ at, const float* __restrict__ lost,
-                                                      int residuals, void* __restrict__ dw, int lddw) {
+                                                      int residuals, void* __restrict__ dw, int lddw,
+                                                      float* __restrict__ sums) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
-  const int rows = count[0];
+  const int rows = count[0], per = ((rows + KT - 1) / KT + gridDim.y - 1) / gridDim.y * KT;
+  const int k0 = blockIdx.y * per, k = max(0, min(rows - k0, per));
   const int tiles_d = (d + Tile::BM - 1) / Tile::BM, tiles_v = (vn + Tile::BN - 1) / Tile::BN;
   int td, tv;
   tile_of(run_of(blockIdx.x, tiles_d * tiles_v), tiles_d, tiles_v, &td, &tv);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const PanelA<Tile, false> pa(xc, ldxc, td * Tile::BM, (int)(ldxc / 2), 0, rows, tid);
-  const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), 0, rows, tid);
+  const PanelA<Tile, false> pa(xc, ldxc, td * Tile::BM, (int)(ldxc / 2), k0, k, tid);
+  const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), k0, k, tid);
   Acc<Tile> acc;
-  multiply<Tile, F16, false, false>(acc, smem, pa, pb, (rows + KT - 1) / KT, tid);
+  multiply<Tile, F16, false, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
 
   // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
   // share of the packed rows, in order; beyond ROOM of them a sum has so many targets that their
   // roundings average out.  Their rows of Xc come through LDS, 64 at a time.
-  if (rows <= FEW_ROWS) {
+  if (rows <= FEW_ROWS && blockIdx.y == 0) {
     constexpr int WAVES = Tile::THREADS / 64, ROOM = 32, PER = Tile::BM / 8;
     struct Hit {
       int pos, col;
@@ -856,6 +861,20 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
       }
     }
   }
+  if (gridDim.y > 1) {
+    const int dp = (int)(ldxc / 2);
+    sums += (size_t)blockIdx.y * vn * dp;
+#pragma unroll
+    for (int j = 0; j < Tile::NF; ++j) {
+      const int v = tv * Tile::BN + Tile::col(j, wid) + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < Tile::MF; ++i) {
+        const int c = td * Tile::BM + Tile::row(i, wid) + (lane >> 4) * 4;
+        if (v < vn && c < dp) *reinterpret_cast<f32x4*>(sums + (size_t)v * dp + c) = acc[i][j];
+      }
+    }
+    return;
+  }
   const float sc = up.scale();
   __syncthreads();  // LDS has been read
 #pragma unroll
@@ -869,6 +888,24 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
   __syncthreads();
   Outgoing<Tile, T>::store(smem, static_cast<T*>(dw), lddw, v0 + tv * Tile::BN, min(Tile::BN, vn - tv * Tile::BN),
                            td * Tile::BM, d - td * Tile::BM, tid);
+}
+
+// Joins the parts of dW: 4 columns of a row a thread.
+template <bool F16>
+__global__ __launch_bounds__(256) void k_dw_out(const float* __restrict__ sums, int parts, long long v, int d, int dp,
+                                                Upstream<F16> up, void* __restrict__ dw) {
+  using T = typename Type<F16>::T;
+  const long long item = (long long)blockIdx.x * 256 + threadIdx.x, row = item / (dp / 4);
+  const int c = (int)(item - row * (dp / 4)) * 4;
+  if (row >= v || c >= d) return;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (up.count[0]) {
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) s += *reinterpret_cast<const f32x4*>(sums + (i * v + row) * dp + c);
+    s *= up.scale();
+  }
+  T* out = static_cast<T*>(dw) + row * d + c;
+  for (int e = 0; e < 4 && c + e < d; ++e) out[e] = (T)s[e];
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -1292,6 +1329,7 @@ struct Room {
   float* sums;    // [splits][packed rows][dp] of dX: n dp, or what `fill` tiles hold
   float* factor;  // [n + 1]
   float* lost;    // [packed row][residuals] what dl's rounding took
+  float* parts;   // [parts][v][dp] of dW, where there are more than one
   long long bytes;
 };
 Room room_of(const tkl_args& a) {
@@ -1305,7 +1343,11 @@ Room room_of(const tkl_args& a) {
   r.factor = reinterpret_cast<float*>(at);
   at += 4 * (a.n + 1);
   r.lost = reinterpret_cast<float*>(at);
-  r.bytes = at + 4 * a.n * residuals(a) - static_cast<char*>(a.room);
+  at += 4 * a.n * residuals(a);
+  at += -(at - static_cast<char*>(a.room)) & 15;
+  r.parts = reinterpret_cast<float*>(at);
+  if (a.parts > 1) at += 4 * a.parts * a.v * padded(a.d);
+  r.bytes = at - static_cast<char*>(a.room);
   return r;
 }
 
@@ -1453,8 +1495,11 @@ void dx(const tkl_args& a, const Kept& q, const Room& r, const Weight& w, int dp
 template <class Tile, bool F16>
 void dw(const tkl_args& a, const Kept& q, const Room& r, int dp, long long v0, int vn, const Upstream<F16>& up,
         hipStream_t s) {
-  k_dw<Tile, F16><<<blocks(a.d, Tile::BM) * blocks(vn, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
-      q.xc, (long long)dp * 2, r.dl, a.piece * 2, (int)v0, vn, (int)a.d, q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d);
+  const dim3 grid(blocks(a.d, Tile::BM) * blocks(vn, Tile::BN), std::max(1, a.parts));
+  k_dw<Tile, F16><<<grid, Tile::THREADS, Tile::LDS, s>>>(q.xc, (long long)dp * 2, r.dl, a.piece * 2, (int)v0, vn, (int)a.d,
+                                                         q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d, r.parts);
+  if (a.parts > 1)
+    k_dw_out<F16><<<blocks(a.v * (dp / 4), 256), 256, 0, s>>>(r.parts, a.parts, a.v, (int)a.d, dp, up, a.dw);
 }
 
 template <bool F16>
@@ -1518,6 +1563,10 @@ extern "C" long long tkl_room_bytes(const tkl_args* a) { return room_of(*a).byte
 extern "C" int tkl_forward(const tkl_args* a) { return on_device(a, a->f16 ? forward<true> : forward<false>); }
 
 extern "C" int tkl_backward(const tkl_args* a) {
+  if (a->parts < 0 || a->parts > 64 || (a->parts > 1 && a->piece < a->v)) {
+    snprintf(g_err, sizeof(g_err), "dW in %d parts: at most 64, of one piece", a->parts);
+    return -1;
+  }
   // (a tile's rows of dl are addressed below FAR)
   if (a->piece < Big::BM || a->piece % Big::BM || a->piece > (1 << 24) || a->fill < 1 || a->fill > 4096 ||
       std::min<long long>(a->n, Big::BN) * a->piece > (1 << 28)) {

@@ -39,9 +39,9 @@ class LossError(RuntimeError):
 
 
 # struct tkl_args of csrc/tk_loss.hip: n d v k ldx ldw ldg ignore piece fill, dev f16 distill
-# reduction, temperature, want small, x w ids teacher grad loss kept room codes wc dx
+# reduction, temperature, want small parts, x w ids teacher grad loss kept room codes wc dx
 # dw stream
-_ARGS = struct.Struct("@10q4if2i13P")
+_ARGS = struct.Struct("@10q4if3i13P")
 
 _loaded = None
 
@@ -107,6 +107,13 @@ def fill(small: bool) -> int:
     return 512 if small else 768
 
 
+def weight_parts(n: int, d: int, v: int) -> int:
+    """Into how many parts the tokens are split for w's gradient in small tiles: two workgroups for
+    each of the 256 compute units, 4 steps of 64 tokens or more each."""
+    tiles = -(-d // SMALL_M) * -(-v // SMALL_N)
+    return max(1, min(512 // tiles, n // 256, 64))
+
+
 def kept_bytes(n: int, d: int, lists: int) -> int:
     """Of what the forward pass keeps for the backward pass; ``lists`` entries of a teacher."""
     return 2 * n * _up(d, 64) + 8 + (8 * lists + 36 * n if lists else 24 * n)
@@ -121,14 +128,15 @@ def part_bytes(n: int, v: int, small: bool) -> int:
     return 8 * n * -(-v // (SMALL_M if small else TILE))
 
 
-def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, lists: int) -> int:
+def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, lists: int,
+               weight: int = 0) -> int:
     """Of the backward pass' workspace: the derivative of a piece's logits, fp32 sums of x's
-    gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors and
-    residuals."""
+    gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors,
+    residuals and fp32 sums of w's gradient (``weight`` rows of them)."""
     once = n * _up(d, 64)
     tiles = groups * (SMALL_M * SMALL_N if small else TILE * TILE)
     sums = max(once, min(piece // 512 * once, tiles)) if want & 1 else 0
-    return 2 * n * piece + 4 * sums + 4 * (n + 1) + (16 * n if lists else 4 * n)
+    return _up(2 * n * piece + 4 * sums + 4 * (n + 1) + (16 * n if lists else 4 * n), 16) + 4 * weight * _up(d, 64)
 
 
 def _row_strided(w):
@@ -205,7 +213,7 @@ def _autograd():
             small = bool(plan.small & 1)
             room = x.new_empty((codes_bytes if plan.keep else part_bytes)(n, v, small), dtype=torch.uint8)
             args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
-                              plan.distill, plan.reduction, plan.temperature, 0, plan.small, x.data_ptr(),
+                              plan.distill, plan.reduction, plan.temperature, 0, plan.small, 1, x.data_ptr(),
                               plain.data_ptr(), ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0,
                               loss.data_ptr(), kept.data_ptr(), room.data_ptr(), room.data_ptr() if plan.keep else 0,
                               0 if copy is None else copy.data_ptr(), 0, 0, stream_of(dev.index))
@@ -234,12 +242,14 @@ def _autograd():
             plain = _row_strided(w) if copy is None else copy
             piece = pieces(n, v)
             groups = fill(bool(plan.small & 2))
-            room = kept.new_empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill))
+            parts = weight_parts(n, d, v) if want & 2 and plan.small & 4 and piece >= v else 1
+            room = kept.new_empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill,
+                                             parts * v if parts > 1 else 0))
             dx = w.new_empty((n, d)) if want & 1 else None
             dw = w.new_empty((v, d)) if want & 2 else None
             args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
                               piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
-                              want, plan.small, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
+                              want, plan.small, parts, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
                               kept.data_ptr(), room.data_ptr(), 0 if codes is None else codes.data_ptr(),
                               0 if copy is None else copy.data_ptr(),
                               0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
