@@ -344,8 +344,10 @@ __device__ __forceinline__ void product_small(f32x4 (&acc)[2][4], char* smem, co
 // The schedule is the one of tk_gemm_screen.hip's k_gemm8: LDS holds half-tiles of two steps,
 // a step is two phases of 32 matrix instructions per wave, and the wave groups wr = 0 and 1
 // run one barrier apart, so that on every SIMD one wave feeds the matrix pipe while the other
-// reads LDS and issues copies.
-template <bool F16, bool AA, bool BA>
+// reads LDS and issues copies.  A wave reads twice as much of A as of B, so a panel down the rows,
+// whose reads take twice as long, is better B; FLIP gives the tile transposed for that, with the
+// lanes' 4 numbers along B.
+template <bool F16, bool AA, bool BA, bool FLIP>
 __device__ __forceinline__ void product_big(Acc<Big>& acc, char* smem, const PanelA<Big, AA>& pa,
                                         const PanelB<Big, BA>& pb, int nk, int tid) {
   constexpr int HBYTES = 128 * KT * 2;
@@ -381,7 +383,8 @@ __device__ __forceinline__ void product_big(Acc<Big>& acc, char* smem, const Pan
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
-          acc[mh * 4 + i][nh * 2 + j] = Type<F16>::mfma(a[i][kk], b[nh][j][kk], acc[mh * 4 + i][nh * 2 + j]);
+          acc[mh * 4 + i][nh * 2 + j] = FLIP ? Type<F16>::mfma(b[nh][j][kk], a[i][kk], acc[mh * 4 + i][nh * 2 + j])
+                                             : Type<F16>::mfma(a[i][kk], b[nh][j][kk], acc[mh * 4 + i][nh * 2 + j]);
     __builtin_amdgcn_s_setprio(0);
   };
   // keep every matrix instruction between its phase's two barriers
@@ -456,10 +459,10 @@ __device__ __forceinline__ void product_big(Acc<Big>& acc, char* smem, const Pan
   if (wr == 0) barrier();  // the other group's extra barrier
 }
 
-template <class Tile, bool F16, bool AA, bool BA>
+template <class Tile, bool F16, bool AA, bool BA, bool FLIP = false>
 __device__ __forceinline__ void multiply(Acc<Tile>& acc, char* smem, const PanelA<Tile, AA>& pa,
                                          const PanelB<Tile, BA>& pb, int nk, int tid) {
-  if constexpr (Tile::BM == 256) product_big<F16, AA, BA>(acc, smem, pa, pb, nk, tid);
+  if constexpr (Tile::BM == 256) product_big<F16, AA, BA, FLIP>(acc, smem, pa, pb, nk, tid);
   else product_small<F16, AA, BA>(acc, smem, pa, pb, nk, tid);
 }
 
@@ -733,7 +736,7 @@ __device__ __forceinline__ int splits_of(int rows, int d, int fill, int piece) {
   return best;
 }
 
-// dX^T tile: A = W (K = vocabulary, down the rows), B = dl (K along the rows).  Each split owns
+// dX^T tile of W (K = vocabulary, down the rows) and dl (K along the rows).  Each split owns
 // its own fp32 sums [rows][dp], added to from piece to piece, so the order of every sum is fixed.
 template <class Tile, bool F16>
 __global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w, long long ldw,
@@ -751,19 +754,26 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int per_split = ((vn + KT - 1) / KT + splits - 1) / splits * KT;
   const int k0 = split * per_split, k = max(0, min(vn - k0, per_split));
-  const PanelA<Tile, false> pa(w, ldw, td * Tile::BM, d, v0 + k0, k, tid);
-  const PanelB<Tile, true> pb(dl, lddl, tn * Tile::BN, rows, k0, (k + 7) & ~7, tid);  // dl is padded with zeros
+  constexpr bool BIG = Tile::BM == Tile::BN;  // W as B (8192 x 4096 x 32768: 1684 us, 1837 with it as A)
   Acc<Tile> acc;
-  multiply<Tile, F16, false, true>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  if constexpr (BIG) {
+    const PanelA<Tile, true> pa(dl, lddl, tn * Tile::BM, rows, k0, (k + 7) & ~7, tid);  // dl is padded with zeros
+    const PanelB<Tile, false> pb(w, ldw, td * Tile::BN, d, v0 + k0, k, tid);
+    multiply<Tile, F16, true, false, true>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  } else {
+    const PanelA<Tile, false> pa(w, ldw, td * Tile::BM, d, v0 + k0, k, tid);
+    const PanelB<Tile, true> pb(dl, lddl, tn * Tile::BN, rows, k0, (k + 7) & ~7, tid);
+    multiply<Tile, F16, false, true>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  }
   out += (size_t)split * rows * dp;
 #pragma unroll
   for (int j = 0; j < Tile::NF; ++j) {
-    const int token = tn * Tile::BN + Tile::col(j, wid) + (lane & 15);
-    if (token >= rows) continue;
 #pragma unroll
     for (int i = 0; i < Tile::MF; ++i) {
-      const int c = td * Tile::BM + Tile::row(i, wid) + (lane >> 4) * 4;
-      if (c >= dp) continue;
+      const int of_a = Tile::row(i, wid), of_b = Tile::col(j, wid);
+      const int token = tn * Tile::BN + (BIG ? of_a : of_b) + (lane & 15);
+      const int c = td * Tile::BM + (BIG ? of_b : of_a) + (lane >> 4) * 4;
+      if (token >= rows || c >= dp) continue;
       f32x4* at = reinterpret_cast<f32x4*>(out + (size_t)token * dp + c);
       f32x4 r = acc[i][j];
       if (!first) r += *at;
@@ -772,13 +782,39 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w
   }
 }
 
-// dW^T tile: A = Xc (K = tokens, down the rows), B = dl (K = tokens, down the rows).  Where dW has
-// few tiles the tokens are split over blockIdx.y, and each part writes its fp32 sums [v][dp], which
-// k_dw_out adds in order (8192 x 512 x 1000, 128 tiles: 86 us whole, 26 in 4 parts).
+// Xc^T [dp][np] of the packed rows, zeros behind them up to the next 64, in tiles of 64 x 64.
+template <typename T>
+__global__ __launch_bounds__(256) void k_transpose(const T* __restrict__ xc, int dp, const int* __restrict__ count,
+                                                   T* __restrict__ xt, int np) {
+  __shared__ __attribute__((aligned(16))) T tile[64][72];
+  typedef __attribute__((ext_vector_type(8))) T t8;
+  const int rows = count[0], c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, at = threadIdx.x >> 3, unit = (threadIdx.x & 7) * 8;
+  if (r0 >= rows) return;
+#pragma unroll
+  for (int h = 0; h < 64; h += 32) {
+    u32x4 v = {0, 0, 0, 0};
+    if (r0 + at + h < rows) v = *reinterpret_cast<const u32x4*>(xc + (size_t)(r0 + at + h) * dp + c0 + unit);
+    *reinterpret_cast<u32x4*>(&tile[at + h][unit]) = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 64; h += 32) {
+    t8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[unit + i][at + h];
+    *reinterpret_cast<t8*>(xt + (size_t)(c0 + at + h) * np + r0 + unit) = v;
+  }
+}
+
+// dW^T tile: A = Xc^T (K = tokens along the rows), B = dl (K = tokens, down the rows).  (With A down
+// the rows of Xc every fragment has to be transposed on its way out of LDS, which takes twice the
+// time of a plain read: 8192 x 4096 x 32768 1724 us, 1950 so.)  Where dW has few tiles the tokens are split over blockIdx.y, and each
+// part writes its fp32 sums [v][dp], which k_dw_out adds in order (8192 x 512 x 1000, 128 tiles: 86
+// us whole, 26 in 4 parts).
 template <class Tile, bool F16>
-__global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ xc, long long ldxc,
-                                                      const void* __restrict__ dl, long long lddl, int v0, int vn,
-                                                      int d, const int* __restrict__ count, Upstream<F16> up,
+__global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ xt, long long ldxt,
+                                                      const void* __restrict__ xc, int dp, const void* __restrict__ dl,
+                                                      long long lddl, int v0, int vn, int d, const int* __restrict__ count, Upstream<F16> up,
                                                       const int* __restrict__ at, const float* __restrict__ lost,
                                                       int residuals, void* __restrict__ dw, int lddw,
                                                       float* __restrict__ sums) {
@@ -790,10 +826,10 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
   int td, tv;
   tile_of(run_of(blockIdx.x, tiles_d * tiles_v), tiles_d, tiles_v, &td, &tv);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const PanelA<Tile, false> pa(xc, ldxc, td * Tile::BM, (int)(ldxc / 2), k0, k, tid);
+  const PanelA<Tile, true> pa(xt, ldxt, td * Tile::BM, dp, k0, (k + 7) & ~7, tid);
   const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), k0, k, tid);
   Acc<Tile> acc;
-  multiply<Tile, F16, false, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  multiply<Tile, F16, true, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
 
   // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
   // share of the packed rows, in order; beyond ROOM of them a sum has so many targets that their
@@ -836,9 +872,8 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
       if (b) __syncthreads();
       for (int i = tid; i < here * PER; i += Tile::THREADS) {
         const int c = td * Tile::BM + i % PER * 8;
-        xrows[i] = c < (int)(ldxc / 2) ? *reinterpret_cast<const u32x4*>(static_cast<const T*>(xc) +
-                                                                       (size_t)all[b + i / PER].pos * (ldxc / 2) + c)
-                                       : u32x4{0, 0, 0, 0};
+        xrows[i] = c < dp ? *reinterpret_cast<const u32x4*>(static_cast<const T*>(xc) + (size_t)all[b + i / PER].pos * dp + c)
+                          : u32x4{0, 0, 0, 0};
       }
       __syncthreads();
       const Hit own = lane < here ? all[b + lane] : Hit{0, 0, 0.f};
@@ -862,7 +897,6 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
     }
   }
   if (gridDim.y > 1) {
-    const int dp = (int)(ldxc / 2);
     sums += (size_t)blockIdx.y * vn * dp;
 #pragma unroll
     for (int j = 0; j < Tile::NF; ++j) {
@@ -1330,6 +1364,7 @@ struct Room {
   float* factor;  // [n + 1]
   float* lost;    // [packed row][residuals] what dl's rounding took
   float* parts;   // [parts][v][dp] of dW, where there are more than one
+  void* xt;       // Xc^T [dp][n up to 64], for dW
   long long bytes;
 };
 Room room_of(const tkl_args& a) {
@@ -1347,6 +1382,8 @@ Room room_of(const tkl_args& a) {
   at += -(at - static_cast<char*>(a.room)) & 15;
   r.parts = reinterpret_cast<float*>(at);
   if (a.parts > 1) at += 4 * a.parts * a.v * padded(a.d);
+  r.xt = at;
+  if (a.want & 2) at += 2 * padded(a.d) * (long long)padded(a.n);
   r.bytes = at - static_cast<char*>(a.room);
   return r;
 }
@@ -1496,8 +1533,9 @@ template <class Tile, bool F16>
 void dw(const tkl_args& a, const Kept& q, const Room& r, int dp, long long v0, int vn, const Upstream<F16>& up,
         hipStream_t s) {
   const dim3 grid(blocks(a.d, Tile::BM) * blocks(vn, Tile::BN), std::max(1, a.parts));
-  k_dw<Tile, F16><<<grid, Tile::THREADS, Tile::LDS, s>>>(q.xc, (long long)dp * 2, r.dl, a.piece * 2, (int)v0, vn, (int)a.d,
-                                                         q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d, r.parts);
+  k_dw<Tile, F16><<<grid, Tile::THREADS, Tile::LDS, s>>>(r.xt, 2 * padded(a.n), q.xc, dp, r.dl, a.piece * 2, (int)v0, vn,
+                                                         (int)a.d, q.count, up, q.at, r.lost, residuals(a), a.dw,
+                                                         (int)a.d, r.parts);
   if (a.parts > 1)
     k_dw_out<F16><<<blocks(a.v * (dp / 4), 256), 256, 0, s>>>(r.parts, a.parts, a.v, (int)a.d, dp, up, a.dw);
 }
@@ -1512,6 +1550,10 @@ hipError_t backward(const tkl_args& a) {
                             n, a.temperature};
   if (F16 && a.reduction == 0)
     k_factor<<<1, 1024, 0, s>>>(up.grad, up.ldg, up.rowmap, up.count, n, a.temperature, Upstream<F16>::SPAN, r.factor);
+  using T = typename Type<F16>::T;
+  if (a.want & 2)
+    k_transpose<T><<<dim3(dp / 64, blocks(n, 64)), 256, 0, s>>>(reinterpret_cast<const T*>(q.xc), dp, q.count,
+                                                                static_cast<T*>(r.xt), padded(n));
   const Weight w = weight_of(a, dp);
   for (long long v0 = 0; v0 < a.v; v0 += a.piece) {
     const int vn = (int)std::min(a.piece, a.v - v0);
