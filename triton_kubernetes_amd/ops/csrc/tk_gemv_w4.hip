@@ -12,9 +12,10 @@
 // Nothing is rounded to 16 bits on the way but the result.
 //
 // Measured (device time, weights out of HBM): one row, 131072 x 4096 with groups of 64 and
-// zeros, 64 us, 4.6 TB/s; 8192 x 8192 12 us; 64 rows, 16384 x 16384 70 us.  One row is bound by
-// the reads and the instructions that unpack and scale; many rows by the matrix and the vector
-// instructions together, which two waves on a SIMD do not overlap wholly.
+// zeros, 65 us, 4.5 TB/s; 8192 x 8192 12 us; 64 rows, 16384 x 16384 63 us.  One row is bound by
+// the reads and the instructions that unpack and scale; many rows by LDS, the matrix and the
+// vector instructions together (49 us of loads alone, 55 of the rest alone), which two waves on a
+// SIMD do not overlap wholly.
 //
 // C ABI for ctypes: triton_kubernetes_amd/ops/gemv.py.
 
@@ -351,7 +352,7 @@ hipError_t one(const void* x, long long ldx, const uint8_t* codes, const void* s
   const int tiles = (n + 15) / 16 * m;  // over all rows of x
   const int chunks = (k + CHUNK - 1) / CHUNK;
   // Enough tiles for every compute unit: one wave a tile, and 4 tiles share what is read of x
-  // (32768 x 4096: 17.4 us, 20.2 with 4 waves a tile).  Fewer: 4 waves a tile (4096 x 4096: 6.0
+  // (32768 x 4096: 17 us, 20 with 4 waves a tile).  Fewer: 4 waves a tile (4096 x 4096: 5.6
   // and 9.9 us), or 8 where the columns are long (4096 x 16384: 12.2 us, 13.5 with 4).
   if (tiles >= 2048) return one_as<F16, G, ZEROS, 4, 1>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, s);
   if (tiles > 256 || chunks < 96) return one_as<F16, G, ZEROS, 1, 4>(x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, s);
@@ -362,7 +363,9 @@ hipError_t one(const void* x, long long ldx, const uint8_t* codes, const void* s
 // on the same columns: a stage is 2 chunks.  Codes come as in k_one, two stages ahead, images of
 // 16 rows x 128 bytes with unit u of row r at u ^ (r/2 & 7); x comes through registers, one stage
 // ahead, into LDS [32 units][16 MT rows], row i of unit u at i ^ (u & 15), in the order that the
-// codes unpack to.  A wave reads x out of LDS for RT tiles at once (8 rows of x are 4 KiB a
+// codes unpack to, with the sums over each scale's columns, which every tile needs.  While the
+// matrix instructions of a step run, the codes of the next are unpacked and the sums of the last
+// group scaled.  A wave reads x out of LDS for RT tiles at once (8 rows of x are 4 KiB a
 // chunk, a tile's codes 1 KiB), and the whole workgroup reads it out of memory once: 256 rows
 // of W a workgroup for more than 16 rows of x keep that to as much as the codes.  The columns
 // are split over blockIdx.y: each split writes its own fp32 sums (`part`), which k_join adds in

@@ -68,10 +68,10 @@ def splits(m: int, n: int, k: int) -> int:
     """How the product is run: 0, each row of ``x`` by itself, or into how many parts ``k`` is split.
 
     A row by itself is one launch and no join, and small weights come out of the cache for every
-    row (4 x 1024 x 4096: 5.6 us, 8.8 together; 16 rows 9.5 both ways; 4 x 4096 x 4096 10.6 and
-    10.3).  Together a workgroup takes 128 rows of the weight (256 for more than 16 rows of
+    row (4 x 1024 x 4096: 5.0 us, 8.5 together; 16 rows 8.5 and 8.7; 4 x 4096 x 4096 9.2 and 9.4;
+    2 x 8192 x 8192 17.0 and 16.2).  Together a workgroup takes 128 rows of the weight (256 for more than 16 rows of
     ``x``), and one for each of the 256 compute units is best (64 rows of ``x``, 16384 x 16384:
-    70 us; 104 with 128 of them, 84 with 512, whose sums cost more to join); a part has at least
+    64 us; 99 with 128 of them, 76 with 512, whose sums cost more to join); a part has at least
     4 chunks of 128 columns."""
     if m == 1 or m * n * k <= 1 << 26:
         return 0

@@ -79,16 +79,17 @@ def small_products(n: int, d: int, v: int) -> int:
 
     A large tile multiplies faster, a small one wastes less on few tokens and fills more
     compute units.  Measured gain of a small tile over a large one, in us of a whole step at
-    bf16 (n x d x v), where the rules turn: logits, n 64 x 4096 x 32000 61, 128 37, 192 -2, 256 -26;
-    1024 x 512 x 1000 24.  x's gradient, 64 x 4096 x 32000 26, 128 7, 128 x 4096 x 131072 -70.
-    w's, 1024 x 512 x 1000 (8 large tiles) 22, 128 x 2048 x 32000 (1000) -7."""
+    bf16 (n x d x v), where the rules turn: logits, 128 x 4096 x 32000 12 of 298, 192 -7, 256 -23;
+    4096 x 512 x 1000 10 of 87, 8192 2.  x's gradient, 64 x 4096 x 32000 9, 128 1, 192 -19, 128 x
+    4096 x 131072 -77; 2048 x 1024 x 4000 10, 512 x 1024 x 32000 0, 4096 x 512 x 8000 -7.  w's, 1024 x
+    512 x 8000 (64 large tiles) 11, 1024 x 1024 x 6000 (96) 3, 4096 x 1024 x 8000 (128) -13."""
 
     def tiles(a, b):
         return -(-a // TILE) * -(-b // TILE)
 
     logits = n <= SMALL_N or tiles(n, v) <= 64 or (tiles(n, v) <= 128 and n <= 2 * SMALL_N)
-    dx = n <= SMALL_N or n * d * v <= 1 << 34
-    return logits | dx << 1 | (tiles(d, v) <= 128) << 2
+    dx = n <= SMALL_N or n * d * v <= 3 << 32
+    return logits | dx << 1 | (tiles(d, v) <= 96) << 2
 
 
 def keeps(n: int, d: int, v: int) -> bool:
