@@ -245,3 +245,20 @@ def test_an_infinite_x_shows_in_its_row_alone(monkeypatch):
         monkeypatch.setattr(gemv, "splits", lambda *a, parts=parts: parts)
         want, got = (gemv.gemv_w4(a, packed, scales, zero) for a in (x, bad))
         assert torch.equal(got[keep], want[keep]) and bool(got[7].isnan().all())
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1, 5, 1 << 20, 32), (3, 5, 1 << 20, 1 << 20), (33, 3, 1 << 19, 64),
+                                         (1, 1 << 24, 32, 32), (2, 1 << 22, 64, 64), (20, 1 << 22, 32, 32)])
+def test_largest_sizes(m, n, k, group):
+    """x of one column that counts, per row another: the products are exact."""
+    from triton_kubernetes_amd.ops import gemv
+
+    gen = _gen(10, m, k)
+    codes, scales, zero = _weight(n, k, group, torch.bfloat16, True, gen, exact=True)
+    packed = gemv.pack_w4(codes)
+    at = torch.randint(0, k, (m,), device="cuda", generator=gen)
+    at[0] = k - 1
+    x = torch.zeros((m, k), device="cuda", dtype=torch.bfloat16)
+    x[torch.arange(m, device="cuda"), at] = 3.0
+    want = (codes[:, at].float() - zero[:, at // group].float()) * scales[:, at // group].float() * 3
+    assert torch.equal(gemv.gemv_w4(x, packed, scales, zero), want.t().bfloat16())

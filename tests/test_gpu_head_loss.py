@@ -604,3 +604,30 @@ def test_weight_gradient_in_parts(n, d, v, masked, dt, monkeypatch):
     for parts in (loss.weight_parts(n, d, v), 2, 64):
         monkeypatch.setattr(loss, "weight_parts", lambda *a, parts=parts: parts)
         _against(call, x, w, *ref.targets_of(t, -100, n, v), gen=gen)
+
+
+@pytest.mark.parametrize("n,d,v,dt", [(3, 65536, 300, torch.bfloat16), (3, 65535, 300, torch.float16),
+                                      (1 << 20, 8, 16, torch.bfloat16), (2, 8, 1 << 24, torch.float16),
+                                      (17, 9, 1 << 22, torch.bfloat16)])
+def test_largest_sizes(n, d, v, dt):
+    from triton_kubernetes_amd.ops.loss import linear_cross_entropy
+
+    gen = _gen(29, n, d)
+    x, w, t = _inputs(n, d, v, dt, gen)
+    for keep in (True, False):
+        _against(lambda x, w: linear_cross_entropy(x, w, t, reduction="none", keep_logits=keep), x, w,
+                 *ref.targets_of(t, -100, n, v), gen=gen, kept=keep)
+        torch.cuda.empty_cache()
+
+
+def test_sizes_past_a_launch_are_refused():
+    from triton_kubernetes_amd.ops.loss import LossError, linear_cross_entropy
+
+    x = torch.zeros((1, 16), device="cuda", dtype=torch.bfloat16).expand(1 << 20, 16)
+    t = torch.zeros(1, device="cuda", dtype=torch.int64).expand(1 << 20)
+    w = torch.zeros((1 << 19, 16), device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(LossError, match="tokens x vocabulary"):
+        linear_cross_entropy(x, w, t)
+    wide = torch.zeros((1, 16384), device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(LossError, match="tokens x width"):
+        linear_cross_entropy(wide.expand(1 << 20, 16384), wide, t)

@@ -290,6 +290,9 @@ def _check(what: str, x, w, reduction: str, keep: Optional[bool]) -> _Plan:
     if not (1 <= plan.d <= MAX_WIDTH and 1 <= plan.v <= MAX_VOCAB and plan.n <= MAX_TOKENS):
         raise LossError(f"{what}: {plan.n} tokens of width {plan.d} over {plan.v} entries (at most {MAX_TOKENS}, "
                         f"{MAX_WIDTH}, {MAX_VOCAB})")
+    if -(-plan.v // TILE) * -(-plan.n // TILE) >= 1 << 23 or -(-plan.d // 1024) * plan.n >= 1 << 24:
+        raise LossError(f"{what}: {plan.n} tokens of width {plan.d} over {plan.v} entries: tokens x vocabulary must be below "
+                        "2^39, tokens x width below 2^34")
     return plan
 
 
