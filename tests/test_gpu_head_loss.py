@@ -631,3 +631,23 @@ def test_sizes_past_a_launch_are_refused():
     wide = torch.zeros((1, 16384), device="cuda", dtype=torch.bfloat16)
     with pytest.raises(LossError, match="tokens x width"):
         linear_cross_entropy(wide.expand(1 << 20, 16384), wide, t)
+
+
+def test_a_second_derivative_is_refused():
+    from triton_kubernetes_amd.ops.loss import LossError, linear_cross_entropy
+
+    x, w, t = _inputs(20, 64, 300, torch.bfloat16, _gen(30))
+    x.requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(x, w, t), x)[0]
+    dx = torch.autograd.grad(linear_cross_entropy(x, w, t), x, create_graph=True)[0]
+    assert torch.equal(dx, want)
+    with pytest.raises(RuntimeError):  # torch's own: x is nothing that dx was made from
+        torch.autograd.grad(dx.float().sum(), x)
+    w.requires_grad_()
+    dw = torch.autograd.grad(linear_cross_entropy(x, w, t), w, create_graph=True)[0]
+    with pytest.raises(LossError, match="second derivative"):
+        torch.autograd.grad(dw.float().sum(), w)
+    loss = linear_cross_entropy(x, w, t)  # a penalty of the gradient would have none otherwise, silently
+    dx = torch.autograd.grad(loss, x, create_graph=True)[0]
+    with pytest.raises(LossError, match="second derivative"):
+        (loss + dx.float().norm()).backward()

@@ -179,7 +179,7 @@ def _apply(x, w, ids, teacher, plan):
 class _Plan:
     """The sizes and settings of a call, from its forward to its backward pass."""
 
-    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore", "f16", "small", "lead", "keep")
+    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore", "f16", "small", "lead", "keep", "codes")
 
 
 _function = None
@@ -193,6 +193,53 @@ def _autograd():
     import torch
 
     stream_of = torch._C._cuda_getCurrentRawStream
+
+    def gradients(ctx, grad):
+        plan = ctx.plan
+        need = ctx.needs_input_grad
+        want = (1 if need[0] else 0) | (2 if need[1] else 0)
+        n, d, v, k = plan.n, plan.d, plan.v, plan.k
+        if n == 0 or k == 0:
+            x, w = ctx.saved_tensors
+            return (torch.zeros_like(x) if want & 1 else None, torch.zeros_like(w) if want & 2 else None, None, None,
+                    None)
+        w, kept, copy, ids = ctx.saved_tensors
+        dev, at = w.device, kept.data_ptr()
+        if not plan.reduction:
+            grad = grad.reshape(-1)
+        if grad.dtype != torch.float32:
+            grad = grad.float()
+        plain = _row_strided(w) if copy is None else copy
+        piece = pieces(n, v)
+        groups = fill(bool(plan.small & 2))
+        parts = weight_parts(n, d, v) if want & 2 and plan.small & 4 and piece >= v else 1
+        room = kept.new_empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill,
+                                         parts * v if parts > 1 else 0))
+        dx = w.new_empty((n, d)) if want & 1 else None
+        dw = w.new_empty((v, d)) if want & 2 else None
+        args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
+                          piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
+                          want, plan.small, parts, 0, plain.data_ptr(), 0 if ids is None else ids.data_ptr(), 0,
+                          grad.data_ptr(), 0, at, room.data_ptr(), at + plan.codes if plan.codes else 0,
+                          0 if copy is None else copy.data_ptr(),
+                          0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                          stream_of(dev.index))
+        if want and _lib().tkl_backward(args) != 0:
+            raise LossError(_lib().tkl_last_error().decode())
+        if dx is not None and plan.lead != (n,):
+            dx = dx.view(*plan.lead, d)
+        return dx, dw, None, None, None
+
+    class Once(torch.autograd.Function):
+        """A gradient that was made with create_graph: to differentiate it again is an error."""
+
+        @staticmethod
+        def forward(ctx, g, w):
+            return g.view_as(g)
+
+        @staticmethod
+        def backward(ctx, grad):
+            raise LossError("the head's losses have no second derivative")
 
     class HeadLoss(torch.autograd.Function):
         @staticmethod
@@ -211,56 +258,35 @@ def _autograd():
             plan.small = small_products(n, d, v)
             plain = _row_strided(w)
             copy = _room_for_copy(plain)
-            kept = x.new_empty(kept_bytes(n, d, n * k if plan.distill else 0), dtype=torch.uint8)
+            size = _up(kept_bytes(n, d, n * k if plan.distill else 0), 256)
             small = bool(plan.small & 1)
-            room = x.new_empty((codes_bytes if plan.keep else part_bytes)(n, v, small), dtype=torch.uint8)
+            if plan.keep:  # the logits behind the rest
+                plan.codes = size
+                kept = x.new_empty(size + codes_bytes(n, v, small), dtype=torch.uint8)
+                at = kept.data_ptr()
+                room = codes = at + size
+            else:
+                plan.codes = 0
+                kept = x.new_empty(size, dtype=torch.uint8)
+                sums = x.new_empty(part_bytes(n, v, small), dtype=torch.uint8)
+                at, room, codes = kept.data_ptr(), sums.data_ptr(), 0
             args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
                               plan.distill, plan.reduction, plan.temperature, 0, plan.small, 1, x.data_ptr(),
                               plain.data_ptr(), ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0,
-                              loss.data_ptr(), kept.data_ptr(), room.data_ptr(), room.data_ptr() if plan.keep else 0,
-                              0 if copy is None else copy.data_ptr(), 0, 0, stream_of(dev.index))
+                              loss.data_ptr(), at, room, codes, 0 if copy is None else copy.data_ptr(), 0, 0,
+                              stream_of(dev.index))
             if _lib().tkl_forward(args) != 0:
                 raise LossError(_lib().tkl_last_error().decode())
-            ctx.save_for_backward(w, ids, kept, room if plan.keep else None, copy)
+            ctx.save_for_backward(w, kept, copy, ids if plan.distill else None)  # (kept has the targets)
             return loss
 
         @staticmethod
-        @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
-            plan = ctx.plan
-            need = ctx.needs_input_grad
-            want = (1 if need[0] else 0) | (2 if need[1] else 0)
-            n, d, v, k = plan.n, plan.d, plan.v, plan.k
-            if n == 0 or k == 0:
-                x, w = ctx.saved_tensors
-                return (torch.zeros_like(x) if want & 1 else None, torch.zeros_like(w) if want & 2 else None, None, None,
-                        None)
-            w, ids, kept, codes, copy = ctx.saved_tensors
-            dev = w.device
-            if not plan.reduction:
-                grad = grad.reshape(-1)
-            if grad.dtype != torch.float32:
-                grad = grad.float()
-            plain = _row_strided(w) if copy is None else copy
-            piece = pieces(n, v)
-            groups = fill(bool(plan.small & 2))
-            parts = weight_parts(n, d, v) if want & 2 and plan.small & 4 and piece >= v else 1
-            room = kept.new_empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill,
-                                             parts * v if parts > 1 else 0))
-            dx = w.new_empty((n, d)) if want & 1 else None
-            dw = w.new_empty((v, d)) if want & 2 else None
-            args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
-                              piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
-                              want, plan.small, parts, 0, plain.data_ptr(), ids.data_ptr(), 0, grad.data_ptr(), 0,
-                              kept.data_ptr(), room.data_ptr(), 0 if codes is None else codes.data_ptr(),
-                              0 if copy is None else copy.data_ptr(),
-                              0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
-                              stream_of(dev.index))
-            if want and _lib().tkl_backward(args) != 0:
-                raise LossError(_lib().tkl_last_error().decode())
-            if dx is not None and plan.lead != (n,):
-                dx = dx.view(*plan.lead, d)
-            return dx, dw, None, None, None
+            if not torch.is_grad_enabled():
+                return gradients(ctx, grad)
+            with torch.no_grad():
+                grads = gradients(ctx, grad)
+            return tuple(None if g is None else Once.apply(g.requires_grad_(), ctx.saved_tensors[0]) for g in grads)
 
     _function = HeadLoss
     return _function
