@@ -153,6 +153,8 @@ std::string hex64(uint64_t v) {
   return b;
 }
 
+void read_power_cap(const std::string& dev, GpuInfo* g);
+
 // ---------------------------------------------------------------- amd_smi --
 #ifdef TK_TOPO_AMDSMI
 const char* link_name(amdsmi_link_type_t t) {
@@ -237,6 +239,8 @@ Topology collect_amdsmi() {
     if (amdsmi_get_power_cap_info(h, 0, &pc) == AMDSMI_STATUS_SUCCESS && pc.power_cap > 0) {  // uW on bare metal
       g.power_cap_w = static_cast<int64_t>((pc.power_cap + 500000) / 1000000);
       if (pc.default_power_cap > 0) g.power_cap_default_w = static_cast<int64_t>((pc.default_power_cap + 500000) / 1000000);
+    } else {  // amd_smi wants the cap's whole range, of which a container may show the cap alone
+      read_power_cap("/sys/class/drm/renderD" + std::to_string(g.drm_render) + "/device", &g);
     }
     amdsmi_vbios_info_t vb{};
     // sysfs vbios_version is amd_smi's part_number ("113-M355-01-1K1-020F" on the box);
@@ -324,6 +328,23 @@ bool read_file(const std::string& path, std::string* out) {
   fclose(f);
   while (!out->empty() && (out->back() == '\n' || out->back() == ' ')) out->pop_back();
   return true;
+}
+
+// board power cap (hwmon of the PCI function, microwatts)
+void read_power_cap(const std::string& dev, GpuInfo* g) {
+  DIR* hw = opendir((dev + "/hwmon").c_str());
+  if (!hw) return;
+  std::string s;
+  while (dirent* e = readdir(hw)) {
+    if (strncmp(e->d_name, "hwmon", 5) != 0) continue;
+    const std::string hd = dev + "/hwmon/" + e->d_name;
+    if (read_file(hd + "/power1_cap", &s) && isdigit((unsigned char)s[0]))
+      g->power_cap_w = static_cast<int64_t>((strtoull(s.c_str(), nullptr, 10) + 500000) / 1000000);
+    if (read_file(hd + "/power1_cap_default", &s) && isdigit((unsigned char)s[0]))
+      g->power_cap_default_w = static_cast<int64_t>((strtoull(s.c_str(), nullptr, 10) + 500000) / 1000000);
+    break;
+  }
+  closedir(hw);
 }
 
 // "key value" lines (KFD properties files).
@@ -456,19 +477,7 @@ Topology collect_sysfs(const std::string& root) {
     if (read_file(dev + "/numa_node", &s)) g.numa_node = std::max<int64_t>(0, atoll(s.c_str()));
     if (read_file(dev + "/product_name", &s) && !s.empty()) g.market_name = s;
     if (read_file(dev + "/vbios_version", &s)) g.vbios = s;
-    // board power cap (hwmon of the PCI function, microwatts)
-    if (DIR* hw = opendir((dev + "/hwmon").c_str())) {
-      while (dirent* e = readdir(hw)) {
-        if (strncmp(e->d_name, "hwmon", 5) != 0) continue;
-        const std::string hd = dev + "/hwmon/" + e->d_name;
-        if (read_file(hd + "/power1_cap", &s) && isdigit((unsigned char)s[0]))
-          g.power_cap_w = static_cast<int64_t>((strtoull(s.c_str(), nullptr, 10) + 500000) / 1000000);
-        if (read_file(hd + "/power1_cap_default", &s) && isdigit((unsigned char)s[0]))
-          g.power_cap_default_w = static_cast<int64_t>((strtoull(s.c_str(), nullptr, 10) + 500000) / 1000000);
-        break;
-      }
-      closedir(hw);
-    }
+    read_power_cap(dev, &g);
     // PCIe link (the PCI function's attributes, e.g. "32.0 GT/s PCIe" and "16")
     if (read_file(dev + "/current_link_width", &s) && isdigit((unsigned char)s[0])) g.pcie_width = atoll(s.c_str());
     if (read_file(dev + "/max_link_width", &s) && isdigit((unsigned char)s[0])) g.pcie_max_width = atoll(s.c_str());
