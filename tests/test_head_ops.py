@@ -31,7 +31,8 @@ def test_losses_refuse_inputs(x, w, message):
 def test_pieces_cover_the_vocabulary_within_the_workspace(n, v):
     piece = loss.pieces(n, v)
     assert piece % loss.TILE == 0 and piece >= loss.TILE
-    assert piece == loss.TILE or piece * n * 2 <= loss.DL_BYTES
+    assert piece == loss.TILE or (piece - loss.TILE) * n * 2 <= 1.5 * loss.DL_BYTES
+    assert min(n, loss.TILE) * piece < 1 << 29  # what the C entry takes
     count = -(-v // piece)
     assert (count - 1) * piece < v  # no empty piece
 

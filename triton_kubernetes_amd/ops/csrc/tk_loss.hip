@@ -1616,8 +1616,8 @@ extern "C" int tkl_backward(const tkl_args* a) {
   }
   // (a tile's rows of dl are addressed below FAR)
   if (a->piece < Big::BM || a->piece % Big::BM || a->piece > (1 << 24) || a->fill < 1 || a->fill > 4096 ||
-      std::min<long long>(a->n, Big::BN) * a->piece > (1 << 28)) {
-    snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, at most 2^28 over 256 tokens; fill %lld 1 to 4096",
+      std::min<long long>(a->n, Big::BN) * a->piece >= (1 << 29)) {
+    snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, below 2^29 over 256 tokens; fill %lld 1 to 4096",
              a->piece, Big::BM, a->fill);
     return -1;
   }
