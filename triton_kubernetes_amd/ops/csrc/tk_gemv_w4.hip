@@ -13,9 +13,9 @@
 //
 // Measured (device time, weights out of HBM): one row, 131072 x 4096 with groups of 64 and
 // zeros, 65 us, 4.5 TB/s; 8192 x 8192 12 us; 64 rows, 16384 x 16384 63 us.  One row is bound by
-// the reads and the instructions that unpack and scale; many rows by LDS, the matrix and the
-// vector instructions together (49 us of loads alone, 55 of the rest alone), which two waves on a
-// SIMD do not overlap wholly.
+// the reads and the instructions that unpack and scale; many rows by the vector and the matrix
+// instructions, 23 and 14 us, which hardly overlap (42 us without loads, barriers and x's way
+// through LDS, 54 without the loads, 49 with nothing but loads).
 //
 // C ABI for ctypes: triton_kubernetes_amd/ops/gemv.py.
 
