@@ -17,6 +17,7 @@ first, or capture with leaves made in the capture (``x.detach().requires_grad_()
 """
 
 import ctypes
+import functools
 import math
 import struct
 from typing import Optional
@@ -164,14 +165,15 @@ def _apply(x, w, ids, teacher, plan):
     import torch
 
     loss = _autograd().apply(x, w, ids, teacher, plan)
-    if loss.grad_fn is not None:
-        stream = torch._C._cuda_getCurrentRawStream(x.device.index)
-        for node, _ in loss.grad_fn.next_functions[:2]:
+    made = loss.grad_fn
+    if made is not None:
+        stream = torch._C._cuda_getCurrentRawStream(plan.device)
+        for node, _ in made.next_functions[:2]:
             # (kept by the node itself, as long as a graph holds it)
             if node is not None and node.metadata.setdefault("tk_loss_stream", stream) != stream:
                 with torch.cuda.device(x.device):
                     if torch.cuda.is_current_stream_capturing():
-                        del loss, node  # or the error's traceback keeps them
+                        del loss, made, node  # or the error's traceback keeps them
                         raise LossError("captured while an eager graph of the same x or w lives: its gradient cannot be "
                                         "captured (drop the earlier loss, or detach x and w in the capture)")
     return loss
@@ -180,7 +182,86 @@ def _apply(x, w, ids, teacher, plan):
 class _Plan:
     """The sizes and settings of a call, from its forward to its backward pass."""
 
-    __slots__ = ("n", "d", "v", "k", "distill", "reduction", "temperature", "ignore", "f16", "small", "lead", "keep", "codes")
+    __slots__ = ("n", "d", "v", "k", "lead", "distill", "reduction", "temperature", "ignore", "f16", "device", "small", "keep",
+                 "kept", "codes", "sums", "piece", "groups", "parts", "room")
+
+
+_INTEGERS = ("torch.int64", "torch.int32", "torch.int16", "torch.uint8", "torch.int8")
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, rules) -> _Plan:
+    """The plan of a call whose tensors have these ``(shape, dtype, device)``; calls alike share one
+    (``rules``: what else the sizes come from)."""
+    (shape, dtype, device), (by, w_type, w_device) = x, w
+    if str(dtype) not in ("torch.bfloat16", "torch.float16") or w_type is not dtype:
+        raise LossError(f"{what} wants x and w both bf16 or both fp16, not {dtype} and {w_type}")
+    if len(shape) < 1 or len(by) != 2 or shape[-1] != by[1]:
+        raise LossError(f"{what} wants x [..., D] and w [V, D], not {list(shape)} and {list(by)}")
+    if device.type != "cuda" or device != w_device:
+        raise LossError(f"{what} wants CUDA tensors on one device, not {device} and {w_device}")
+    if reduction not in REDUCTIONS:
+        raise LossError(f"unknown reduction '{reduction}' ({' | '.join(REDUCTIONS)})")
+    p = _Plan()
+    (p.v, p.d), p.lead = by, shape[:-1]
+    p.n = n = p.lead.numel()
+    d, v = p.d, p.v
+    if not (1 <= d <= MAX_WIDTH and 1 <= v <= MAX_VOCAB and n <= MAX_TOKENS):
+        raise LossError(f"{what}: {n} tokens of width {d} over {v} entries (at most {MAX_TOKENS}, {MAX_WIDTH}, {MAX_VOCAB})")
+    if -(-v // TILE) * -(-n // TILE) >= 1 << 23 or -(-d // 1024) * n >= 1 << 24:
+        raise LossError(f"{what}: {n} tokens of width {d} over {v} entries: tokens x vocabulary must be below 2^39, "
+                        "tokens x width below 2^34")
+    id_shape, id_type, id_device = ids
+    name = "target" if logits is None else "ids"
+    if str(id_type) not in _INTEGERS or id_device != device:
+        raise LossError(f"{what} wants {name} as integers on x's device, not {id_type} on {id_device}")
+    if (id_shape if logits is None else id_shape[:-1]) != p.lead or (logits is not None and len(id_shape) == 0):
+        raise LossError(f"{what}: {name} {list(id_shape)} does not go with x {list(shape)}")
+    p.k, p.distill = 1, 0
+    if logits is not None:
+        if not logits[1].is_floating_point or logits[2] != device or logits[0] != id_shape:
+            raise LossError(f"{what} wants logits as numbers of ids' shape on x's device, not {logits[1]} {list(logits[0])} "
+                            f"on {logits[2]}")
+        p.k, p.distill = id_shape[-1], 1
+        if p.k > MAX_TARGETS:
+            raise LossError(f"{what}: {p.k} entries a token (at most {MAX_TARGETS})")
+        if not (math.isfinite(temperature) and temperature > 0):
+            raise LossError(f"{what}: the temperature must be above 0, not {temperature}")
+    if not -(1 << 63) <= ignore < 1 << 63:
+        raise LossError(f"{what}: no target can be {ignore}")
+    p.reduction, p.temperature, p.ignore = REDUCTIONS[reduction], temperature, ignore
+    p.f16, p.device = str(dtype) == "torch.float16", device.index
+    if n and p.k:
+        p.small = small_products(n, d, v)
+        p.keep = grads and (keeps(n, d, v) if keep is None else bool(keep))
+        p.kept = _up(kept_bytes(n, d, n * p.k if p.distill else 0), 256)
+        p.codes = p.kept if p.keep else 0  # the logits lie behind the rest
+        p.sums = part_bytes(n, v, bool(p.small & 1))
+        if p.keep:
+            p.kept += codes_bytes(n, v, bool(p.small & 1))
+        p.piece = pieces(n, v)
+        p.groups = fill(bool(p.small & 2))
+        parts = weight_parts(n, d, v) if p.small & 4 and p.piece >= v else 1
+        p.parts = (1, 1, parts, parts)  # by the gradients that are wanted
+        p.room = tuple(room_bytes(n, d, p.piece, p.groups, bool(p.small & 2), want, p.distill,
+                                  p.parts[want] * v if p.parts[want] > 1 else 0) for want in range(4))
+    return p
+
+
+def _planned(what, x, w, ids, logits, reduction, temperature, ignore, keep):
+    import torch
+
+    grads = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    rules = (small_products, keeps, pieces, fill, weight_parts, DL_BYTES, KEEP_BYTES)
+    return _plan(what, (x.shape, x.dtype, x.device), (w.shape, w.dtype, w.device), (ids.shape, ids.dtype, ids.device),
+                 None if logits is None else (logits.shape, logits.dtype, logits.device), reduction, temperature, ignore,
+                 keep, grads, rules)
+
+
+def _ids(ids):
+    import torch
+
+    return ids if ids.dtype is torch.int64 and ids.is_contiguous() else ids.to(torch.int64).contiguous()
 
 
 _function = None
@@ -193,7 +274,7 @@ def _autograd():
         return _function
     import torch
 
-    stream_of = torch._C._cuda_getCurrentRawStream
+    lib, stream_of = _lib(), torch._C._cuda_getCurrentRawStream
 
     def gradients(ctx, grad):
         plan = ctx.plan
@@ -205,29 +286,24 @@ def _autograd():
             return (torch.zeros_like(x) if want & 1 else None, torch.zeros_like(w) if want & 2 else None, None, None,
                     None)
         w, kept, copy, ids = ctx.saved_tensors
-        dev, at = w.device, kept.data_ptr()
         if not plan.reduction:
             grad = grad.reshape(-1)
-        if grad.dtype != torch.float32:
+        if grad.dtype is not torch.float32:
             grad = grad.float()
         plain = _row_strided(w) if copy is None else copy
-        piece = pieces(n, v)
-        groups = fill(bool(plan.small & 2))
-        parts = weight_parts(n, d, v) if want & 2 and plan.small & 4 and piece >= v else 1
-        room = kept.new_empty(room_bytes(n, d, piece, groups, bool(plan.small & 2), want, plan.distill,
-                                         parts * v if parts > 1 else 0))
+        room = kept.new_empty(plan.room[want])
         dx = w.new_empty((n, d)) if want & 1 else None
         dw = w.new_empty((v, d)) if want & 2 else None
+        at = kept.data_ptr()
         args = _ARGS.pack(n, d, v, k, 0, plain.stride(0), 0 if plan.reduction else grad.stride(0), plan.ignore,
-                          piece, groups, dev.index, plan.f16, plan.distill, plan.reduction, plan.temperature,
-                          want, plan.small, parts, 0, plain.data_ptr(), 0 if ids is None else ids.data_ptr(), 0,
+                          plan.piece, plan.groups, plan.device, plan.f16, plan.distill, plan.reduction, plan.temperature,
+                          want, plan.small, plan.parts[want], 0, plain.data_ptr(), 0 if ids is None else ids.data_ptr(), 0,
                           grad.data_ptr(), 0, at, room.data_ptr(), at + plan.codes if plan.codes else 0,
-                          0 if copy is None else copy.data_ptr(),
-                          0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
-                          stream_of(dev.index))
-        if want and _lib().tkl_backward(args) != 0:
-            raise LossError(_lib().tkl_last_error().decode())
-        if dx is not None and plan.lead != (n,):
+                          0 if copy is None else copy.data_ptr(), 0 if dx is None else dx.data_ptr(),
+                          0 if dw is None else dw.data_ptr(), stream_of(plan.device))
+        if want and lib.tkl_backward(args) != 0:
+            raise LossError(lib.tkl_last_error().decode())
+        if dx is not None and len(plan.lead) != 1:
             dx = dx.view(*plan.lead, d)
         return dx, dw, None, None, None
 
@@ -245,39 +321,33 @@ def _autograd():
     class HeadLoss(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, w, ids, teacher, plan):
-            dev = x.device
             n, d, v, k = plan.n, plan.d, plan.v, plan.k
             ctx.plan = plan
             loss = x.new_empty(() if plan.reduction else plan.lead, dtype=torch.float32)
             if n == 0 or k == 0:  # nothing has a loss
                 ctx.save_for_backward(x, w)
                 return loss.zero_()
-            if x.dim() != 2:
+            if len(plan.lead) != 1:
                 x = x.reshape(n, d)
-            if x.stride(1) != 1:
+            ldx, step = x.stride()
+            if step != 1:
                 x = x.contiguous()
-            plan.small = small_products(n, d, v)
+                ldx = x.stride(0)
             plain = _row_strided(w)
             copy = _room_for_copy(plain)
-            size = _up(kept_bytes(n, d, n * k if plan.distill else 0), 256)
-            small = bool(plan.small & 1)
-            if plan.keep:  # the logits behind the rest
-                plan.codes = size
-                kept = x.new_empty(size + codes_bytes(n, v, small), dtype=torch.uint8)
-                at = kept.data_ptr()
-                room = codes = at + size
+            kept = x.new_empty(plan.kept, dtype=torch.uint8)
+            at = kept.data_ptr()
+            if plan.keep:
+                sums, codes = None, at + plan.codes
             else:
-                plan.codes = 0
-                kept = x.new_empty(size, dtype=torch.uint8)
-                sums = x.new_empty(part_bytes(n, v, small), dtype=torch.uint8)
-                at, room, codes = kept.data_ptr(), sums.data_ptr(), 0
-            args = _ARGS.pack(n, d, v, k, x.stride(0), plain.stride(0), 0, plan.ignore, 0, 0, dev.index, plan.f16,
-                              plan.distill, plan.reduction, plan.temperature, 0, plan.small, 1, x.data_ptr(),
-                              plain.data_ptr(), ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0,
-                              loss.data_ptr(), at, room, codes, 0 if copy is None else copy.data_ptr(), 0, 0,
-                              stream_of(dev.index))
-            if _lib().tkl_forward(args) != 0:
-                raise LossError(_lib().tkl_last_error().decode())
+                sums, codes = x.new_empty(plan.sums, dtype=torch.uint8), 0
+            args = _ARGS.pack(n, d, v, k, ldx, plain.stride(0), 0, plan.ignore, 0, 0, plan.device, plan.f16, plan.distill,
+                              plan.reduction, plan.temperature, 0, plan.small, 1, x.data_ptr(), plain.data_ptr(),
+                              ids.data_ptr(), 0 if teacher is None else teacher.data_ptr(), 0, loss.data_ptr(), at,
+                              codes or sums.data_ptr(), codes, 0 if copy is None else copy.data_ptr(), 0, 0,
+                              stream_of(plan.device))
+            if lib.tkl_forward(args) != 0:
+                raise LossError(lib.tkl_last_error().decode())
             ctx.save_for_backward(w, kept, copy, ids if plan.distill else None)  # (kept has the targets)
             return loss
 
@@ -293,50 +363,6 @@ def _autograd():
     return _function
 
 
-def _check(what: str, x, w, reduction: str, keep: Optional[bool]) -> _Plan:
-    import torch
-
-    dtype = x.dtype
-    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or w.dtype is not dtype:
-        raise LossError(f"{what} wants x and w both bf16 or both fp16, not {x.dtype} and {w.dtype}")
-    shape = x.shape
-    if len(shape) < 1 or w.dim() != 2 or shape[-1] != w.shape[1]:
-        raise LossError(f"{what} wants x [..., D] and w [V, D], not {list(x.shape)} and {list(w.shape)}")
-    if not x.is_cuda or x.device != w.device:
-        raise LossError(f"{what} wants CUDA tensors on one device, not {x.device} and {w.device}")
-    if reduction not in REDUCTIONS:
-        raise LossError(f"unknown reduction '{reduction}' ({' | '.join(REDUCTIONS)})")
-    plan = _Plan()
-    plan.v, plan.d = w.shape
-    plan.lead = shape[:-1]
-    plan.n = plan.lead.numel()
-    plan.reduction = REDUCTIONS[reduction]
-    plan.f16 = dtype is torch.float16
-    plan.keep = (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
-                 and (keeps(plan.n, plan.d, plan.v) if keep is None else bool(keep)))
-    if not (1 <= plan.d <= MAX_WIDTH and 1 <= plan.v <= MAX_VOCAB and plan.n <= MAX_TOKENS):
-        raise LossError(f"{what}: {plan.n} tokens of width {plan.d} over {plan.v} entries (at most {MAX_TOKENS}, "
-                        f"{MAX_WIDTH}, {MAX_VOCAB})")
-    if -(-plan.v // TILE) * -(-plan.n // TILE) >= 1 << 23 or -(-plan.d // 1024) * plan.n >= 1 << 24:
-        raise LossError(f"{what}: {plan.n} tokens of width {plan.d} over {plan.v} entries: tokens x vocabulary must be below "
-                        "2^39, tokens x width below 2^34")
-    return plan
-
-
-_INTEGERS = ("torch.int64", "torch.int32", "torch.int16", "torch.uint8", "torch.int8")
-
-
-def _ids(what: str, name: str, ids, x, dims: int):
-    import torch
-
-    if ids.dtype is not torch.int64 and str(ids.dtype) not in _INTEGERS or ids.device != x.device:
-        raise LossError(f"{what} wants {name} as integers on x's device, not {ids.dtype} on {ids.device}")
-    lead = x.shape[:-1]
-    if ids.dim() != len(lead) + dims or ids.shape[:len(lead)] != lead:
-        raise LossError(f"{what}: {name} {list(ids.shape)} does not go with x {list(x.shape)}")
-    return ids if ids.dtype is torch.int64 and ids.is_contiguous() else ids.to(torch.int64).contiguous()
-
-
 def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: str = "mean",
                          keep_logits: Optional[bool] = None):
     """Softmax cross entropy of the logits ``x @ w.T`` against ``target``, in fp32.
@@ -350,10 +376,8 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
 
     Between the passes 2 bytes a logit are kept where :func:`keeps` finds that faster;
     ``keep_logits=False`` saves that memory, ``True`` spends it whatever the size."""
-    plan = _check("linear_cross_entropy", x, w, reduction, keep_logits)
-    ids = _ids("linear_cross_entropy", "target", target, x, 0)
-    plan.k, plan.distill, plan.temperature, plan.ignore = 1, 0, 1.0, int(ignore_index)
-    return _apply(x, w, ids, None, plan)
+    plan = _planned("linear_cross_entropy", x, w, target, None, reduction, 1.0, int(ignore_index), keep_logits)
+    return _apply(x, w, _ids(target), None, plan)
 
 
 def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean",
@@ -370,18 +394,7 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     :func:`linear_cross_entropy`."""
     import torch
 
-    what = "linear_distill"
-    plan = _check(what, x, w, reduction, keep_logits)
-    ids = _ids(what, "ids", ids, x, 1)
-    if not logits.is_floating_point() or logits.device != x.device or logits.shape != ids.shape:
-        raise LossError(f"{what} wants logits as numbers of ids' shape on x's device, not {logits.dtype} "
-                        f"{list(logits.shape)} on {logits.device}")
+    plan = _planned("linear_distill", x, w, ids, logits, reduction, float(temperature), 0, keep_logits)
     if logits.requires_grad and torch.is_grad_enabled():
-        raise LossError(f"{what} gives the teacher's logits no gradient: detach them")
-    if ids.shape[-1] > MAX_TARGETS:
-        raise LossError(f"{what}: {ids.shape[-1]} entries a token (at most {MAX_TARGETS})")
-    temperature = float(temperature)
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise LossError(f"{what}: the temperature must be above 0, not {temperature}")
-    plan.k, plan.distill, plan.temperature, plan.ignore = ids.shape[-1], 1, temperature, 0
-    return _apply(x, w, ids, logits.detach().float().contiguous(), plan)
+        raise LossError("linear_distill gives the teacher's logits no gradient: detach them")
+    return _apply(x, w, _ids(ids), logits.detach().float().contiguous(), plan)
