@@ -56,7 +56,7 @@ def test_buffers_have_the_sizes_that_the_kernels_take(n, d, k):
                                                   (1, 1, 0, 32768, 1), (3, 4096, 7, 256, 64)):
             args = _args(n=n, d=d, v=200, k=k, want=want, piece=piece, fill=groups, small=small, distill=distill,
                          parts=parts)
-            assert lib.tkl_room_bytes(args) == loss.room_bytes(n, d, piece, groups, bool(small & 2), want, distill,
+            assert lib.tkl_room_bytes(args) == loss.room_bytes(n, d, piece, groups, small, want, distill,
                                                                parts * 200 if parts > 1 else 0)
 
 

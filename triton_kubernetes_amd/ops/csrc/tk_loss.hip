@@ -813,9 +813,10 @@ __global__ __launch_bounds__(256) void k_transpose(const T* __restrict__ xc, int
 
 // dW^T tile: A = Xc^T (K = tokens along the rows), B = dl (K = tokens, down the rows).  (With A down
 // the rows of Xc its fragments have to be transposed on their way out of LDS too, which takes twice
-// the time of a plain read: 1950 us for 1724 at 8192 x 4096 x 32768.)  Where dW has few tiles the
-// tokens are split over blockIdx.y, and each part writes its fp32 sums [v][dp], which k_dw_out adds
-// in order (8192 x 512 x 1000, 128 tiles: 86 us whole, 26 in 4 parts).
+// the time of a plain read: 1950 us for 1724 at 8192 x 4096 x 32768.  Small tiles do that, and save a
+// launch: 21 us both ways at 8192 x 512 x 1000.)  Where dW has few tiles the tokens are split over
+// blockIdx.y, and each part writes its fp32 sums [v][dp], which k_dw_out adds in order (8192 x 512 x
+// 1000, 128 tiles: 86 us whole, 26 in 4 parts).
 template <class Tile, bool F16>
 __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ xt, long long ldxt,
                                                       const void* __restrict__ xc, int dp, const void* __restrict__ dl,
@@ -831,10 +832,15 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
   int td, tv;
   tile_of(run_of(blockIdx.x, tiles_d * tiles_v), tiles_d, tiles_v, &td, &tv);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const PanelA<Tile, true> pa(xt, ldxt, td * Tile::BM, dp, k0, (k + 7) & ~7, tid);
   const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), k0, k, tid);
   Acc<Tile> acc;
-  multiply<Tile, F16, true, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  if constexpr (Tile::BM == Tile::BN) {
+    const PanelA<Tile, true> pa(xt, ldxt, td * Tile::BM, dp, k0, (k + 7) & ~7, tid);
+    multiply<Tile, F16, true, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  } else {
+    const PanelA<Tile, false> pa(xc, 2 * dp, td * Tile::BM, dp, k0, k, tid);
+    multiply<Tile, F16, false, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+  }
 
   // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
   // share of the packed rows, in order; beyond ROOM of them a sum has so many targets that their
@@ -1369,7 +1375,7 @@ struct Room {
   float* factor;  // [n + 1]
   float* lost;    // [packed row][residuals] what dl's rounding took
   float* parts;   // [parts][v][dp] of dW, where there are more than one
-  void* xt;       // Xc^T [dp][n up to 64], for dW
+  void* xt;       // Xc^T [dp][n up to 64], for dW in large tiles
   long long bytes;
 };
 Room room_of(const tkl_args& a) {
@@ -1388,7 +1394,7 @@ Room room_of(const tkl_args& a) {
   r.parts = reinterpret_cast<float*>(at);
   if (a.parts > 1) at += 4 * a.parts * a.v * padded(a.d);
   r.xt = at;
-  if (a.want & 2) at += 2 * padded(a.d) * (long long)padded(a.n);
+  if ((a.want & 2) && !(a.small & 4)) at += 2 * padded(a.d) * (long long)padded(a.n);
   r.bytes = at - static_cast<char*>(a.room);
   return r;
 }
@@ -1556,7 +1562,7 @@ hipError_t backward(const tkl_args& a) {
   if (F16 && a.reduction == 0)
     k_factor<<<1, 1024, 0, s>>>(up.grad, up.ldg, up.rowmap, up.count, n, a.temperature, Upstream<F16>::SPAN, r.factor);
   using T = typename Type<F16>::T;
-  if (a.want & 2)
+  if ((a.want & 2) && !(a.small & 4))
     k_transpose<T><<<dim3(dp / 64, blocks(n, 64)), 256, 0, s>>>(reinterpret_cast<const T*>(q.xc), dp, q.count,
                                                                 static_cast<T*>(r.xt), padded(n));
   const Weight w = weight_of(a, dp);

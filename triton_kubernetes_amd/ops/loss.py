@@ -131,16 +131,17 @@ def part_bytes(n: int, v: int, small: bool) -> int:
     return 8 * n * -(-v // (SMALL_M if small else TILE))
 
 
-def room_bytes(n: int, d: int, piece: int, groups: int, small: bool, want: int, lists: int,
+def room_bytes(n: int, d: int, piece: int, groups: int, small: int, want: int, lists: int,
                weight: int = 0) -> int:
     """Of the backward pass' workspace: the derivative of a piece's logits, fp32 sums of x's
     gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors,
-    residuals, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``)."""
+    residuals, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``,
+    unless ``small & 4``)."""
     once = n * _up(d, 64)
-    tiles = groups * (SMALL_M * SMALL_N if small else TILE * TILE)
+    tiles = groups * (SMALL_M * SMALL_N if small & 2 else TILE * TILE)
     sums = max(once, min(piece // 512 * once, tiles)) if want & 1 else 0
     return _up(2 * n * piece + 4 * sums + 4 * (n + 1) + (16 * n if lists else 4 * n), 16) \
-        + 4 * weight * _up(d, 64) + (2 * _up(d, 64) * _up(n, 64) if want & 2 else 0)
+        + 4 * weight * _up(d, 64) + (2 * _up(d, 64) * _up(n, 64) if want & 2 and not small & 4 else 0)
 
 
 def _row_strided(w):
@@ -243,7 +244,7 @@ def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, 
         p.groups = fill(bool(p.small & 2))
         parts = weight_parts(n, d, v) if p.small & 4 and p.piece >= v else 1
         p.parts = (1, 1, parts, parts)  # by the gradients that are wanted
-        p.room = tuple(room_bytes(n, d, p.piece, p.groups, bool(p.small & 2), want, p.distill,
+        p.room = tuple(room_bytes(n, d, p.piece, p.groups, p.small, want, p.distill,
                                   p.parts[want] * v if p.parts[want] > 1 else 0) for want in range(4))
     return p
 
