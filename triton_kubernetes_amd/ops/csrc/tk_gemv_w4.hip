@@ -579,8 +579,16 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
                                               T* __restrict__ y, long long ldy) {
   const int row = blockIdx.x * 256 + threadIdx.x, xrow = blockIdx.y;
   if (row >= n) return;
+  const float* from = part + (size_t)xrow * n + row;
+  const size_t step = (size_t)m * n;
   float s = 0.f;
-  for (int i = 0; i < splits; ++i) s += part[((size_t)i * m + xrow) * n + row];
+  for (int i = 0; i < splits; i += 8) {  // 8 loads in flight (8 x 1024 x 16384, 32 splits: 9.5 us for 16.9)
+    float v[8];
+#pragma unroll
+    for (int o = 0; o < 8; ++o) v[o] = i + o < splits ? from[(i + o) * step] : 0.f;
+#pragma unroll
+    for (int o = 0; o < 8; ++o) s += v[o];
+  }
   y[xrow * ldy + row] = (T)s;
 }
 

@@ -68,16 +68,16 @@ def splits(m: int, n: int, k: int) -> int:
     """How the product is run: 0, each row of ``x`` by itself, or into how many parts ``k`` is split.
 
     A row by itself is one launch and no join, and small weights come out of the cache for every
-    row (4 x 1024 x 4096: 5.0 us, 8.5 together; 16 rows 8.5 and 8.7; 4 x 4096 x 4096 9.2 and 9.4;
-    2 x 8192 x 8192 17.0 and 16.2).  Together a workgroup takes 128 rows of the weight (256 for more than 16 rows of
-    ``x``), and one for each of the 256 compute units is best (64 rows of ``x``, 16384 x 16384:
-    64 us; 99 with 128 of them, 76 with 512, whose sums cost more to join); a part has at least
-    4 chunks of 128 columns."""
-    if m == 1 or m * n * k <= 1 << 26:
+    row (4 x 1024 x 4096: 5.7 us, 6.9 together; 8 rows 7.2 and 7.0; 2 x 4096 x 4096 7.9 and 7.7,
+    4 rows 10.3 and 7.9; 64 x 1024 x 512 6.2 and 9.2).  Together a workgroup takes 128 rows of the
+    weight (256 for more than 16 rows of ``x``), and one for each of the 256 compute units is best
+    (64 rows of ``x``, 16384 x 16384: 64 us; 99 with 128 of them, 75 with 512, whose sums cost more
+    to join); a part has at least 2 chunks of 128 columns, a stage."""
+    if m == 1 or m * n * k < 1 << 25:
         return 0
     blocks = -(-n // (128 if m <= 16 else 256))
     chunks = -(-k // 128)
-    want = max(1, min(256 // blocks, chunks // 4, 64))
+    want = max(1, min(256 // blocks, chunks // 2, 64))
     per = _up(-(-chunks // want), 2)
     return -(-chunks // per)  # no part is empty
 
