@@ -1098,19 +1098,45 @@ __device__ __forceinline__ float dot(const T* x, const T* w, long long ldw, int 
   return s;
 }
 
-// A teacher's lists: zk[pos][j] = x . w[id], one wave a target.  An id below 0 is no entry.
+// A teacher's lists: zk[pos][j] = x . w[id], one wave for 4 entries of a token, which share its x
+// (2048 tokens x 64 entries of 2048: 92 us one by one, 82 so, 6.5 TB/s).  An id below 0 is no entry.
 template <typename T>
 __global__ __launch_bounds__(256) void k_dots(const T* __restrict__ xc, int dp, const T* __restrict__ w,
                                               long long ldw, int dk, const long long* __restrict__ ids, int k,
                                               long long v, const int* __restrict__ rowmap,
                                               const int* __restrict__ count, float* __restrict__ zk) {
-  const long long items = (long long)count[0] * k;
-  const int lane = threadIdx.x & 63;
+  constexpr int SHARE = 4;
+  typedef __attribute__((ext_vector_type(8))) T t8;
+  const int per_row = (k + SHARE - 1) / SHARE, lane = threadIdx.x & 63;
+  const long long items = (long long)count[0] * per_row;
   for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += (long long)gridDim.x * 4) {
-    const int pos = (int)(i / k), j = (int)(i - (long long)pos * k);
-    const long long id = ids[(size_t)rowmap[pos] * k + j];
-    const float s = id < 0 ? 0.f : dot(xc + (size_t)pos * dp, w, ldw, dk, id, v, lane, 64);
-    if (lane == 0) zk[i] = s;
+    const int pos = (int)(i / per_row), j = (int)(i - (long long)pos * per_row) * SHARE;
+    const long long* row = ids + (size_t)rowmap[pos] * k;
+    long long id[SHARE];
+    const T* from[SHARE];
+    float s[SHARE] = {};
+#pragma unroll
+    for (int o = 0; o < SHARE; ++o) {
+      id[o] = j + o < k ? row[j + o] : -1;
+      from[o] = w + (id[o] >= 0 && id[o] < v ? id[o] : 0) * ldw;
+    }
+    const T* x = xc + (size_t)pos * dp;
+#pragma unroll 2
+    for (int e = lane * 8; e < dk; e += 512) {
+      const t8 p = *reinterpret_cast<const t8*>(x + e);
+      t8 q[SHARE];
+#pragma unroll
+      for (int o = 0; o < SHARE; ++o) q[o] = *reinterpret_cast<const t8*>(from[o] + e);
+#pragma unroll
+      for (int o = 0; o < SHARE; ++o)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) s[o] += (float)p[c] * (float)q[o][c];
+    }
+#pragma unroll
+    for (int o = 0; o < SHARE; ++o) {
+      s[o] = wave_sum(s[o]);
+      if (lane == 0 && j + o < k) zk[(size_t)pos * k + j + o] = id[o] < 0 ? 0.f : id[o] < v ? s[o] : NAN;
+    }
   }
 }
 
@@ -1523,7 +1549,7 @@ hipError_t forward(const tkl_args& a) {
   if (a.small & 1) all_logits<Small, F16>(a, q, w, dp, s);
   else all_logits<Big, F16>(a, q, w, dp, s);
   if (a.distill)
-    k_dots<T><<<(unsigned)std::min<long long>(((long long)n * k + 3) / 4, 1 << 22), 256, 0, s>>>(
+    k_dots<T><<<(unsigned)std::min<long long>((n * ((k + 3ll) / 4) + 3) / 4, 1 << 22), 256, 0, s>>>(
         xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count, q.zk);
   k_loss<T><<<blocks(n, 8), 256, 0, s>>>(part_of(a),
                                          (int)blocks(a.v, a.small & 1 ? Small::BM : Big::BM), n, xc, dp, wt, w.ldb / 2,
