@@ -1008,8 +1008,10 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
   const int row0 = blockIdx.x * 4 * per, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c = 0;
   if (flag) {
+#pragma unroll 8
     for (int r = tid; r < row0; r += 256) c += flag[r] != 0;
   } else {
+#pragma unroll 8
     for (int r = tid; r < row0; r += 256) c += target[r] != ignore;
   }
 #pragma unroll
@@ -1040,7 +1042,7 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
     }
     T* out = xc + (size_t)pos * dp;
     const T* in = x + (long long)r * ldx;
-#pragma unroll 4
+#pragma unroll 8
     for (int e = lane * 8; e + 8 <= d; e += 512) {
       u32x4 v;
       __builtin_memcpy(&v, in + e, 16);  // at any alignment
@@ -1226,6 +1228,7 @@ __global__ __launch_bounds__(1024) void k_reduce(const float* __restrict__ rowlo
   __shared__ double sum[16];
   const int rows = count[0];
   double s = 0.;
+#pragma unroll 8
   for (int i = threadIdx.x; i < rows; i += 1024) s += rowloss[i];
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -1244,11 +1247,13 @@ __global__ __launch_bounds__(1024) void k_factor(const float* __restrict__ grad,
   __shared__ float top[16];
   const int rows = count[0];
   float m = 0.f;
+#pragma unroll 8
   for (int i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(grad[rowmap[i] * ldg]));
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
   __syncthreads();
   for (int i = 0; i < 16; ++i) m = fmaxf(m, top[i]);
+#pragma unroll 8
   for (int i = threadIdx.x; i < rows; i += 1024) {
     const float g = grad[rowmap[i] * ldg];
     factor[i] = g == 0.f ? 0.f : g / m * span;
