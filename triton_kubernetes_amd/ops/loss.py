@@ -96,10 +96,10 @@ def small_products(n: int, d: int, v: int) -> int:
 
 def keeps(n: int, d: int, v: int) -> bool:
     """Whether the forward pass keeps the logits, in 16 bits, for the backward pass, which otherwise
-    computes them again (``keep_logits`` decides for a single call).  A short product is cheaper than two passes over its result.  A step at
-    bf16, kept and again, in us: 4096 x 4096 x 32768 2740 and 3430, 512 x 32768 561 and 586,
-    384 530 and 534, 256 478 and 458; few tokens read the weight once less (16 x 4096 x 131072 841
-    and 1006, 512 x 256 x 32000 105 both)."""
+    computes them again (``keep_logits`` decides for a single call).  A short product is cheaper
+    than two passes over its result.  A step at bf16, kept and again, in us: 4096 x 4096 x 32768
+    2740 and 3430, 512 x 32768 561 and 586, 384 530 and 534, 256 478 and 458; few tokens read the
+    weight once less (16 x 4096 x 131072 841 and 1006, 512 x 256 x 32000 105 both)."""
     return (d >= 384 or n <= 512) and 2 * n * v <= KEEP_BYTES
 
 
