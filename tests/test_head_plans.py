@@ -1,0 +1,39 @@
+"""What a call of the output head's operators plans before the GPU has anything to do: what is
+kept between the passes, how the vocabulary is cut, which settings are refused."""
+
+import inspect
+
+import pytest
+import torch
+
+from triton_kubernetes_amd.ops import loss
+
+CUDA = torch.device("cuda", 0)
+
+
+def plan(n, d, v, *, k=0, keep="default", temperature=1.0, dt=torch.bfloat16):
+    """The plan of a training step of these sizes; ``k`` entries of a teacher's lists."""
+    call = loss.linear_distill if k else loss.linear_cross_entropy
+    if keep == "default":
+        keep = inspect.signature(call).parameters["keep_logits"].default
+
+    def meta(*shape, dtype=dt):
+        return torch.Size(shape), dtype, CUDA
+
+    rules = (loss.small_products, loss.keeps, loss.pieces, loss.fill, loss.weight_parts, loss.DL_BYTES, loss.KEEP_BYTES)
+    return loss._plan(call.__name__, meta(n, d), meta(v, d), meta(*([n, k] if k else [n]), dtype=torch.int64),
+                      meta(n, k, dtype=torch.float32) if k else None, "mean", temperature, -100, keep, True, rules)
+
+
+@pytest.mark.parametrize("k", [0, 64])
+@pytest.mark.parametrize("n,d,v", [(48, 512, 1000), (512, 256, 32000), (4096, 4096, 32768), (8192, 4096, 131072)])
+def test_no_logits_are_kept_unless_the_caller_says_so(n, d, v, k):
+    usual = plan(n, d, v, k=k)
+    assert not usual.keep and usual.codes == 0
+    # x's packed rows, and a few numbers a token and listed entry
+    assert usual.kept <= 2 * n * (d + 63) + n * (40 + 8 * k) + 512
+    assert plan(n, d, v, k=k, keep=False).kept == usual.kept
+    kept = plan(n, d, v, k=k, keep=True)
+    assert kept.keep and kept.kept >= usual.kept + 2 * n * v
+    where_faster = plan(n, d, v, k=k, keep=None)
+    assert where_faster.keep == loss.keeps(n, d, v)

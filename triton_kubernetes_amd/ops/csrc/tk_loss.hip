@@ -1,5 +1,6 @@
 // Losses of a language model's output head on MI355X (gfx950): the logits z = X W^T of N tokens
-// over a vocabulary of V leave the kernel that multiplies only as sums, or in 16 bits.
+// over a vocabulary of V leave the kernel that multiplies only as sums, or, where the caller has
+// them kept between the passes, in 16 bits.
 //
 // Both losses compare the softmax q of a row's logits (at a temperature T) with K sparse
 // targets (id_k, p_k), sum_k p_k = 1:
@@ -13,8 +14,8 @@
 // Forward: one matrix product whose epilogue reduces every tile of the vocabulary to a maximum
 // and a sum per token (k_logits<LSE>), a dot product per target, and a join over the tiles
 // (k_loss, which also forms a cross entropy's dot products; k_dots those of a teacher's lists).
-// Backward, in pieces of the vocabulary: the logits' 16-bit derivative dl, from codes that the
-// forward pass kept (k_dl, struct Codes), or from the same product again (k_logits<DL>); a
+// Backward, in pieces of the vocabulary: the logits' 16-bit derivative dl, from the same product
+// again (k_logits<DL>), or from codes that the forward pass kept (k_dl, struct Codes); a
 // teacher's targets are put in by k_fix; then dX += dl W and dW = dl^T X.
 //
 // dl is rounded to 16 bits, which costs each product about as much as the rounding of its result.

@@ -2,10 +2,10 @@
 
 ``linear_cross_entropy(x, w, target)`` is the softmax cross entropy of the logits ``x @ w.T``,
 and ``linear_distill(x, w, ids, logits)`` their divergence from a teacher's top logits; both
-with their gradients (torch autograd).  The ``[tokens, vocabulary]`` logits are never stored in
-full: the forward pass keeps a few numbers a token and, up to ``KEEP_BYTES`` of them, the
-logits in 16 bits for the backward pass, which otherwise computes them again; the backward
-pass works on a piece of the vocabulary at a time.  Like ``gemm.gemm_bt`` they take torch
+with their gradients (torch autograd).  The ``[tokens, vocabulary]`` logits are not kept: the
+forward pass leaves a few numbers a token, and the backward pass computes the logits again, a
+piece of the vocabulary at a time.  A caller who has the memory may have them kept in 16 bits
+instead (``keep_logits``).  Like ``gemm.gemm_bt`` the losses take torch
 tensors on the GPU and queue their work on torch's current stream of that device; nothing
 waits for it here, and both directions can be captured into a graph.
 
@@ -27,7 +27,7 @@ from .native import NativeUnavailable, load
 TILE = 256  # vocabulary entries and tokens of a large tile
 SMALL_M, SMALL_N = 128, 64  # of a small one
 DL_BYTES = 512 << 20  # the backward pass' 16-bit derivative of the logits, per piece
-KEEP_BYTES = 4 << 30  # of logits in 16 bits, kept from the forward to the backward pass
+KEEP_BYTES = 4 << 30  # most logits in 16 bits that a call with keep_logits=None keeps for its backward pass
 MAX_TARGETS = 1024  # ids of a token's list
 MAX_TOKENS = 1 << 20
 MAX_WIDTH = 1 << 16
@@ -95,8 +95,8 @@ def small_products(n: int, d: int, v: int) -> int:
 
 
 def keeps(n: int, d: int, v: int) -> bool:
-    """Whether the forward pass keeps the logits, in 16 bits, for the backward pass, which otherwise
-    computes them again (``keep_logits`` decides for a single call).  A short product is cheaper
+    """Whether a call with ``keep_logits=None`` keeps the logits, in 16 bits, for its backward pass:
+    where that is faster than to compute them again.  A short product is cheaper
     than two passes over its result.  A step at bf16, kept and again, in us: 4096 x 4096 x 32768
     2740 and 3430, 512 x 32768 561 and 586, 384 530 and 534, 256 478 and 458; few tokens read the
     weight once less (16 x 4096 x 131072 841 and 1006, 512 x 256 x 32000 105 both)."""
@@ -365,7 +365,7 @@ def _autograd():
 
 
 def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: str = "mean",
-                         keep_logits: Optional[bool] = None):
+                         keep_logits: Optional[bool] = False):
     """Softmax cross entropy of the logits ``x @ w.T`` against ``target``, in fp32.
 
     ``x [..., D]`` and ``w [V, D]`` are both bf16 or both fp16, of any strides (rows that are
@@ -375,14 +375,17 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
     ``reduction`` is ``mean`` over the tokens that count (0 if none does), ``sum``, or
     ``none`` for a loss per token.  Gradients flow to ``x`` and ``w``, once.
 
-    Between the passes 2 bytes a logit are kept where :func:`keeps` finds that faster;
-    ``keep_logits=False`` saves that memory, ``True`` spends it whatever the size."""
+    Between the passes the logits are not kept.  ``keep_logits=True`` keeps them, 2 bytes each
+    for as long as the loss lives, instead of computing them again, and ``None`` does so up to
+    ``KEEP_BYTES`` where :func:`keeps` finds that faster.  Kept logits are rounded: a probability
+    is then off by up to 8.5e-5 of itself, 3.4e-4 below 2^-8 of its tile's largest and 2.7e-3
+    below 2^-24, which joins the rounding of the gradient's operands."""
     plan = _planned("linear_cross_entropy", x, w, target, None, reduction, 1.0, int(ignore_index), keep_logits)
     return _apply(x, w, _ids(target), None, plan)
 
 
 def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean",
-                   keep_logits: Optional[bool] = None):
+                   keep_logits: Optional[bool] = False):
     """Divergence of the softmax of ``x @ w.T / temperature`` from a teacher's, times
     ``temperature ** 2``, in fp32: per token ``sum_k p_k (log p_k - log q_k)`` over the listed
     entries, with ``p`` the softmax of ``logits / temperature`` over them.
