@@ -101,8 +101,8 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
     ``[N, K/group]`` has ``x``'s type, ``zeros`` (uint8, the same shape) may be left out for
     symmetric weights, whose zero is 8.  The weight's tensors are contiguous; ``group`` is a
     multiple of 32.  Sums are fp32 and rounded once; they are of ``(16 + code) * x``, so an
-    infinite ``x`` gives NaN.  The result (``out``, if given: contiguous, ``[..., N]``) has
-    ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that wants one is
+    infinite ``x`` gives NaN.  The result (``out``, if given: contiguous, ``[..., N]``, changed
+    in place as torch counts it) has ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that wants one is
     refused."""
     import torch
 
@@ -135,6 +135,8 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
         raise GemvError("out must not share memory with x or the weight")
     elif out.requires_grad and torch.is_grad_enabled():
         raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
+    elif not out.is_inference():
+        torch.autograd.graph.increment_version(out)  # the kernel writes it behind torch's back
     if m == 0 or n == 0:
         return out
     if not flat:
