@@ -94,6 +94,13 @@ def _overlap(a, b) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _tangents(*tensors) -> bool:
+    """Whether one of them carries a forward-mode derivative (no_grad says nothing of these)."""
+    from torch.autograd import forward_ad
+
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def gemv_w4(x, codes, scales, zeros=None, *, out=None):
     """``x @ w.T`` for ``x [..., K]`` of at most 64 rows, bf16 or fp16, of any strides.
 
@@ -102,8 +109,8 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
     symmetric weights, whose zero is 8.  The weight's tensors are contiguous; ``group`` is a
     multiple of 32.  Sums are fp32 and rounded once; they are of ``(16 + code) * x``, so an
     infinite ``x`` gives NaN.  The result (``out``, if given: contiguous, ``[..., N]``, changed
-    in place as torch counts it) has ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that wants one is
-    refused."""
+    in place as torch counts it) has ``x``'s type.  It is for serving: it has no gradient, and an ``x`` that wants one,
+    or that has a forward-mode tangent, is refused."""
     import torch
 
     dtype = x.dtype
@@ -123,6 +130,8 @@ def gemv_w4(x, codes, scales, zeros=None, *, out=None):
         raise GemvError("gemv_w4 wants a contiguous weight, its codes 16-byte aligned")
     if (x.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
         raise GemvError("gemv_w4 has no gradient: call it under torch.no_grad()")
+    if torch.autograd.forward_ad._current_level >= 0 and _tangents(x, scales, out):  # (0.1 us, 0.9 always)
+        raise GemvError("gemv_w4 has no gradient: a tensor with a tangent has to be unpacked first")
     flat = len(shape) == 2
     m = shape[0] if flat else x.numel() // k
     if m > MAX_ROWS:
