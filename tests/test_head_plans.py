@@ -37,3 +37,14 @@ def test_no_logits_are_kept_unless_the_caller_says_so(n, d, v, k):
     assert kept.keep and kept.kept >= usual.kept + 2 * n * v
     where_faster = plan(n, d, v, k=k, keep=None)
     assert where_faster.keep == loss.keeps(n, d, v)
+
+
+def test_the_backward_workspace_has_a_place_for_the_number_of_splits():
+    """What k_dx found and k_dx_out has to go by: 4 bytes between the factors and the residuals."""
+    from test_head_ops import _args
+
+    sizes = dict(n=3, d=64, piece=256, fill=1, small=0, want=1, distill=1)
+    want = 2 * 3 * 256 + 4 * 3 * 64 + 4 * (3 + 1) + 4 + 16 * 3  # dl, sums, factors, splits, residuals
+    want = -(-want // 16) * 16
+    assert loss._lib().tkl_room_bytes(_args(**sizes)) == want
+    assert loss.room_bytes(3, 64, 256, 1, 0, 1, 1) == want

@@ -724,7 +724,8 @@ __global__ __launch_bounds__(256) void k_dl(const unsigned short* __restrict__ c
 // Into how many parts the vocabulary is split for dX of `rows` packed rows, so that the last round
 // of tiles over the compute units is as full as the others: of the most parts that 1, 2 or 3 rounds
 // hold (`fill` workgroups at most, 512 entries of a piece or more each) those that cost least, a
-// round's products and a tile's fp32 sums, written and read once more.  Only the device knows `rows`.
+// round's products and a tile's fp32 sums, written and read once more.  Only the device knows `rows`;
+// k_dx leaves what it found to k_dx_out (`splits`), which has to read just as many sums.
 template <class Tile>
 __device__ __forceinline__ int splits_of(int rows, int d, int fill, int piece) {
   const int tiles = ((d + Tile::BM - 1) / Tile::BM) * ((rows + Tile::BN - 1) / Tile::BN);
@@ -748,11 +749,12 @@ template <class Tile, bool F16>
 __global__ __launch_bounds__(Tile::THREADS) void k_dx(const void* __restrict__ w, long long ldw,
                                                       const void* __restrict__ dl, long long lddl, int v0, int vn,
                                                       int d, int dp, const int* __restrict__ count, int fill,
-                                                      int first, float* __restrict__ out) {
+                                                      int first, float* __restrict__ out, int* __restrict__ chosen) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int rows = count[0], splits = splits_of<Tile>(rows, d, fill, (int)(lddl / 2));
   const int tiles_d = (d + Tile::BM - 1) / Tile::BM, tiles_n = (rows + Tile::BN - 1) / Tile::BN;
   const int tiles = tiles_d * tiles_n, nwg = tiles * splits;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *chosen = splits;
   if ((int)blockIdx.x >= nwg) return;
   const int place = run_of(blockIdx.x, nwg), split = place / tiles;
   int td, tn;
@@ -1320,8 +1322,7 @@ __global__ __launch_bounds__(256) void k_fix(const long long* __restrict__ ids, 
 // Joins the splits of dX, adds what dl's rounding took, scales, rounds once, and puts zeros into
 // the rows without a loss.
 template <bool F16>
-__global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, int small, int fill, int piece,
-                                                int dk, int d, int dp,
+__global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, const int* __restrict__ chosen, int d, int dp,
                                                 const int* __restrict__ posof, Upstream<F16> up,
                                                 const int* __restrict__ at, const float* __restrict__ lost,
                                                 int residuals, const void* __restrict__ w, long long ldw,
@@ -1333,8 +1334,7 @@ __global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, 
   if (c >= d) return;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (pos >= 0) {
-    const int rows = up.count[0];
-    const int splits = small ? splits_of<Small>(rows, dk, fill, piece) : splits_of<Big>(rows, dk, fill, piece);
+    const int rows = up.count[0], splits = *chosen;
     const float* from = part + (size_t)pos * dp + c;
     int i = 0;
     for (; i + 8 <= splits; i += 8) {  // 8 loads in flight, added in order
@@ -1405,6 +1405,7 @@ struct Room {
   void* dl;       // [n][piece] 16-bit
   float* sums;    // [splits][packed rows][dp] of dX: n dp, or what `fill` tiles hold
   float* factor;  // [n + 1]
+  int* splits;    // of dX, as k_dx found them
   float* lost;    // [packed row][residuals] what dl's rounding took
   float* parts;   // [parts][v][dp] of dW, where there are more than one
   void* xt;       // Xc^T [dp][n up to 64], for dW in large tiles
@@ -1420,6 +1421,8 @@ Room room_of(const tkl_args& a) {
   if (a.want & 1) at += 4 * std::max(once, std::min(a.piece / 512 * once, a.fill * tile));
   r.factor = reinterpret_cast<float*>(at);
   at += 4 * (a.n + 1);
+  r.splits = reinterpret_cast<int*>(at);
+  at += 4;
   r.lost = reinterpret_cast<float*>(at);
   at += 4 * a.n * residuals(a);
   at += -(at - static_cast<char*>(a.room)) & 15;
@@ -1569,7 +1572,7 @@ template <class Tile, bool F16>
 void dx(const tkl_args& a, const Kept& q, const Room& r, const Weight& w, int dp, long long v0, int vn, hipStream_t s) {
   const unsigned most = std::max<long long>((long long)blocks(w.dk, Tile::BM) * blocks(a.n, Tile::BN), a.fill);
   k_dx<Tile, F16><<<most, Tile::THREADS, Tile::LDS, s>>>(w.at, w.ldb, r.dl, a.piece * 2, (int)v0, vn, w.dk, dp, q.count,
-                                                         (int)a.fill, v0 == 0, r.sums);
+                                                         (int)a.fill, v0 == 0, r.sums, r.splits);
 }
 
 template <class Tile, bool F16>
@@ -1615,9 +1618,8 @@ hipError_t backward(const tkl_args& a) {
     }
   }
   if (a.want & 1)
-    k_dx_out<F16><<<blocks(d, 1024) * (unsigned)n, 256, 0, s>>>(r.sums, a.small & 2, (int)a.fill, (int)a.piece, w.dk, d,
-                                                                dp, q.posof, up, q.at,
-                                                                r.lost, residuals(a), w.at, w.ldb / 2, a.dx);
+    k_dx_out<F16><<<blocks(d, 1024) * (unsigned)n, 256, 0, s>>>(r.sums, r.splits, d, dp, q.posof, up, q.at, r.lost,
+                                                                residuals(a), w.at, w.ldb / 2, a.dx);
   return hipGetLastError();
 }
 

@@ -135,12 +135,12 @@ def room_bytes(n: int, d: int, piece: int, groups: int, small: int, want: int, l
                weight: int = 0) -> int:
     """Of the backward pass' workspace: the derivative of a piece's logits, fp32 sums of x's
     gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors,
-    residuals, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``,
+    the number of splits, residuals, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``,
     unless ``small & 4``)."""
     once = n * _up(d, 64)
     tiles = groups * (SMALL_M * SMALL_N if small & 2 else TILE * TILE)
     sums = max(once, min(piece // 512 * once, tiles)) if want & 1 else 0
-    return _up(2 * n * piece + 4 * sums + 4 * (n + 1) + (16 * n if lists else 4 * n), 16) \
+    return _up(2 * n * piece + 4 * sums + 4 * (n + 2) + (16 * n if lists else 4 * n), 16) \
         + 4 * weight * _up(d, 64) + (2 * _up(d, 64) * _up(n, 64) if want & 2 and not small & 4 else 0)
 
 
