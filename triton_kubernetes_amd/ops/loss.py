@@ -10,10 +10,13 @@ tensors on the GPU and queue their work on torch's current stream of that device
 waits for it here, and both directions can be captured into a graph.
 
 A captured backward pass needs everything that it goes through to be made on the capture's
-stream.  torch keeps a leaf's gradient node, and its stream, for as long as any graph of that
-leaf lives; captured then, the pass would leave that stream behind in the capture, which ends
-the process.  A call that meets such a node of an earlier call is refused; drop the earlier loss
-first, or capture with leaves made in the capture (``x.detach().requires_grad_()``).
+stream.  torch keeps a leaf's gradient node, and its stream, for as long as anything holds that
+node: a loss that is alive, a data-parallel reducer, a gradient edge.  Captured then, the pass
+would leave that stream behind in the capture, which ends the process.  A call that meets a node
+that an earlier call on another stream went through is refused, whatever will be done with its
+result: drop what holds the node, or capture with leaves made in the capture
+(``x.detach().requires_grad_()``).  A node that only other operations went through before is not
+known here, and the same holds for it.
 """
 
 import ctypes
@@ -175,8 +178,9 @@ def _apply(x, w, ids, teacher, plan):
                 with torch.cuda.device(x.device):
                     if torch.cuda.is_current_stream_capturing():
                         del loss, made, node  # or the error's traceback keeps them
-                        raise LossError("captured while an eager graph of the same x or w lives: its gradient cannot be "
-                                        "captured (drop the earlier loss, or detach x and w in the capture)")
+                        raise LossError("captured while the gradient node of x or w from an eager graph on another stream "
+                                        "lives, through which no gradient can be captured: drop what holds it (an earlier "
+                                        "loss, a data-parallel reducer, a gradient edge), or detach x and w in the capture")
     return loss
 
 
