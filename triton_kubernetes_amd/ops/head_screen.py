@@ -8,6 +8,7 @@ pass (:func:`loss_screen`), and 4-bit codes unpacked and scaled on the way from 
 compared with 64-bit sums that torch forms.  Both need PyTorch-ROCm on the node.
 """
 
+from contextlib import contextmanager
 from dataclasses import asdict, dataclass
 from typing import Any, Dict
 
@@ -16,14 +17,26 @@ from .native import NativeUnavailable
 SAMPLE = 64  # tokens, and vocabulary entries, whose gradients are computed again in 64 bits
 
 
-def _torch():
+def _torch(dev: int):
     try:
         import torch
     except ImportError as exc:
         raise NativeUnavailable("this screen needs PyTorch-ROCm") from exc
     if not torch.cuda.is_available():
         raise NativeUnavailable("no GPU")
+    if not 0 <= dev < torch.cuda.device_count():
+        raise NativeUnavailable(f"no GPU {dev} (there are {torch.cuda.device_count()})")
     return torch
+
+
+@contextmanager
+def _on(torch, dev: int):
+    """``dev`` as the current device; what it has no memory for is a refusal."""
+    try:
+        with torch.cuda.device(dev):
+            yield
+    except torch.OutOfMemoryError as exc:
+        raise NativeUnavailable("the GPU's memory does not hold a screen of these sizes") from exc
 
 
 @dataclass
@@ -100,11 +113,11 @@ def loss_screen(dev: int = 0, tokens: int = 4096, vocab: int = 32768, hidden: in
                 dtype: str = "bf16", inject: int = -1) -> LossScreen:
     """``reps`` training steps of the head (loss and both gradients) on random operands.
     ``inject`` changes one value of the last pass' weight gradient, which has to show."""
-    torch = _torch()
+    torch = _torch(dev)
     from .loss import linear_cross_entropy
 
     dt = _dtype(torch, dtype)
-    with torch.cuda.device(dev):
+    with _on(torch, dev):
         gen = torch.Generator(device="cuda").manual_seed(0x5eed)
         w = (torch.randn((vocab, hidden), device="cuda", generator=gen) * hidden ** -0.5).to(dt).requires_grad_()
         target = torch.randint(0, vocab, (tokens,), device="cuda", generator=gen)
@@ -164,13 +177,13 @@ def gemv_screen(dev: int = 0, rows: int = 1, out: int = 16384, inp: int = 16384,
                 dtype: str = "bf16", inject: int = -1) -> GemvScreen:
     """``reps`` products of ``rows`` tokens with one 4-bit weight of random codes, each result
     compared with the 64-bit one.  ``inject`` changes one value of the last result."""
-    torch = _torch()
+    torch = _torch(dev)
     from .gemv import dequantize_w4, gemv_w4
 
     dt = _dtype(torch, dtype)
     if group < 32 or group % 32 or inp < group or inp % group:
         raise ValueError(f"a group of {group} must be a multiple of 32 that divides {inp} columns")
-    with torch.cuda.device(dev), torch.no_grad():
+    with _on(torch, dev), torch.no_grad():
         gen = torch.Generator(device="cuda").manual_seed(0x5eed)
         codes = torch.randint(0, 256, (out, inp // 2), device="cuda", generator=gen, dtype=torch.uint8)
         scales = (torch.rand((out, inp // group), device="cuda", generator=gen) + 0.5).to(dt)
