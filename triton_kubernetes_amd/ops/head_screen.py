@@ -103,10 +103,106 @@ def _timed(torch, call, reps: int) -> float:
     return best
 
 
-def _over(torch, got, want, tol):
-    """(elements off by more than ``tol`` or not finite, the worst error / tolerance)."""
-    ratio = ((got.double() - want).abs() / tol).nan_to_num(nan=float("inf"))
-    return int((ratio > 1).sum()), float(ratio.max())
+STEP = 2.0 ** -23  # of an fp32 sum, relative to it, at most
+
+
+class _Verdict:
+    """Counts of what was off by more than its tolerance, and the worst error / tolerance of all."""
+
+    def __init__(self):
+        self.worst = 0.0
+
+    def over(self, got, want, tol) -> int:
+        ratio = ((got.double() - want).abs() / tol).nan_to_num(nan=float("inf"))
+        self.worst = max(self.worst, float(ratio.max()))
+        return int((ratio > 1).sum())
+
+
+def head_data(torch, tokens: int, vocab: int, hidden: int, dt, gen):
+    """``(x, w, target)`` of a head whose logits have a standard deviation of 3, so that a token's
+    probabilities are neither one entry nor all alike, and its softmax is a large part of its
+    gradient (0.9 % of it at a deviation of 1 and 32768 entries)."""
+    dev = gen.device
+    w = (torch.randn((vocab, hidden), device=dev, generator=gen) * hidden ** -0.5).to(dt)
+    target = torch.randint(0, vocab, (tokens,), device=dev, generator=gen)
+    x = 3 * torch.randn((tokens, hidden), device=dev, generator=gen)
+    return (x + 8 * torch.rand((tokens, 1), device=dev, generator=gen) * w[target].float()).to(dt), w, target
+
+
+def judge_step(torch, x, w, ids, p, t, loss, dx, dw, rows, at):
+    """``(bad losses, bad in dx, bad in dw, worst error / tolerance)`` of the sum over all tokens of
+    ``t^2 sum_k p_k (log p_k - log q_{id_k})``, ``q`` the softmax of ``x @ w.T / t``: every token's
+    loss, ``dx`` of the tokens ``rows`` and ``dw`` of the entries ``at``, against 64 bits.  On any device.
+
+    Tolerances.  A logit is a sum of D products whose partial sums grow as a random walk to |x||w|
+    / sqrt(D) and as a line to z: rounding each costs about STEP (|x||w| + sqrt(D) |z|) at most,
+    here times 8 (``far``).  The sum of exponentials is of at most 80 + V/8192 additions in a row, all
+    positive; with 2^-20 for the exponential and logarithm that is the row's ``off``, common to all of
+    its probabilities.  The derivative of a logit is rounded to 16 bits, half a step u each; these
+    roundings are independent, so a gradient's element is off by 6 standard deviations at most, 6 u
+    sqrt(sum (dl b)^2), and half a step of its own.  A row of a gradient as a whole is off by u times
+    its terms' root mean square and u times itself, more than twice what roundings that are spread
+    evenly give; this finds what is wrong a little everywhere."""
+    n, d = x.shape
+    v, u, c = w.shape[0], torch.finfo(x.dtype).eps / 2, 2048
+    verdict, inf = _Verdict(), float("inf")
+    used = torch.where(ids >= 0, p.double(), 0.0)
+    at_ids = ids.clamp_min(0)
+    # 64-bit logits of all tokens, a block at a time: their logsumexp, the largest, and the targets'
+    lse, top, zk = (torch.empty(s, dtype=torch.float64, device=x.device) for s in ((n,), (n,), tuple(ids.shape)))
+    for n0 in range(0, n, 4096):
+        part = slice(n0, n0 + 4096)
+        xs = x[part].double()
+        m, s, big = xs.new_full((len(xs),), -inf), xs.new_zeros(len(xs)), xs.new_zeros(len(xs))
+        for v0 in range(0, v, c):
+            z = xs @ w[v0:v0 + c].double().T / t
+            m2 = torch.maximum(m, z.amax(1))
+            s, m = s * torch.exp(m - m2) + torch.exp(z - m2[:, None]).sum(1), m2
+            big = torch.maximum(big, z.abs().amax(1))
+        lse[part], top[part] = m + torch.log(s), big
+        for k in range(ids.shape[1]):
+            zk[part, k] = (xs * w[at_ids[part, k]].double()).sum(1) / t
+    far = 8 * STEP * (x.double().norm(dim=1) * float(w.float().norm(dim=1).max()) / t + (d ** 0.5 + 2) * top)
+    off = far + (80 + v / 8192) * STEP + 2.0 ** -20 + 4 * STEP * lse.abs()
+    terms = torch.special.xlogy(used, used)
+    true = t * t * (terms - used * (zk - lse[:, None])).sum(1)
+    size = (terms.abs() + used * (zk.abs() + lse.abs()[:, None])).sum(1)
+    bad_losses = verdict.over(loss, true, t * t * (2 * off + (8 + ids.shape[1]) * STEP * size))
+
+    delta = far + 2.0 ** -20 + v ** 0.5 * STEP
+    xr, lse_r, off_r, delta_r = x[rows].double(), lse[rows, None], off[rows, None], delta[rows, None]
+    true, square, drift = (torch.zeros((len(rows), d), dtype=torch.float64, device=x.device) for _ in range(3))
+    for v0 in range(0, v, c):
+        ws = w[v0:v0 + c].double()
+        q = torch.exp(xr @ ws.T / t - lse_r)
+        here = (ids[rows] >= v0) & (ids[rows] < v0 + c)
+        dl = q.scatter_add(1, torch.where(here, ids[rows] - v0, 0).clamp(0, len(ws) - 1), -torch.where(here, used[rows], 0.0)) * t
+        true += dl @ ws
+        square += dl.square() @ ws.square()
+        drift += t * (q @ ws)
+
+    def compare(got, true, spread, common):
+        tol = 6 * spread + common + u * true.abs() + 1e-7
+        rowwise = spread.norm(dim=1) + common.norm(dim=1) + u * true.norm(dim=1) + 1e-7 * d ** 0.5
+        return verdict.over(got, true, tol) + verdict.over((got.double() - true).norm(dim=1), 0 * rowwise, rowwise)
+
+    bad_dx = compare(dx[rows], true, square.sqrt() * (u + delta_r), off_r * drift.abs())
+
+    true, square, drift = (torch.zeros((len(at), d), dtype=torch.float64, device=x.device) for _ in range(3))
+    wa = w[at].double()
+    for n0 in range(0, n, 4096):
+        part = slice(n0, n0 + 4096)
+        xs = x[part].double()
+        q = torch.exp(xs @ wa.T / t - lse[part, None])
+        dl = q.clone()
+        for k in range(ids.shape[1]):
+            dl -= (ids[part, k, None] == at[None]) * used[part, k, None]
+        true += t * (dl.T @ xs)
+        each = (u * dl).square() + (q * (delta + off)[part, None]).square() + n * STEP ** 2 * dl.square()
+        square += t * t * (each.T @ xs.square())
+        drift += t * (q.T @ xs)
+    bad_dw = compare(dw[at], true, square.sqrt(), float(off.max()) * drift.abs())
+    return bad_losses, bad_dx, bad_dw, verdict.worst
 
 
 def loss_screen(dev: int = 0, tokens: int = 4096, vocab: int = 32768, hidden: int = 4096, reps: int = 3,
@@ -119,11 +215,9 @@ def loss_screen(dev: int = 0, tokens: int = 4096, vocab: int = 32768, hidden: in
     dt = _dtype(torch, dtype)
     with _on(torch, dev):
         gen = torch.Generator(device="cuda").manual_seed(0x5eed)
-        w = (torch.randn((vocab, hidden), device="cuda", generator=gen) * hidden ** -0.5).to(dt).requires_grad_()
-        target = torch.randint(0, vocab, (tokens,), device="cuda", generator=gen)
-        x = torch.randn((tokens, hidden), device="cuda", generator=gen)
-        x = (x + 8 * torch.rand((tokens, 1), device="cuda", generator=gen) * w.detach()[target].float()).to(dt)
+        x, w, target = head_data(torch, tokens, vocab, hidden, dt, gen)
         x.requires_grad_()
+        w.requires_grad_()
         ones = torch.ones(tokens, device="cuda")
 
         def step():
@@ -140,35 +234,12 @@ def loss_screen(dev: int = 0, tokens: int = 4096, vocab: int = 32768, hidden: in
                 got[2].view(-1)[inject] += 1
             # the bits, so that a NaN that repeats is no difference here (the comparison below finds it)
             differing += sum(int((a.view(bits) != b.view(bits)).sum()) for a, b in zip(got, first))
-        loss, dx, dw = first[0].double(), first[1], first[2]
-
-        u, step32 = torch.finfo(dt).eps / 2, 2.0 ** -23
-        xs, ws = x.detach().double(), w.detach()
         rows = torch.randperm(tokens, device="cuda", generator=gen)[:SAMPLE]
-        z = xs[rows] @ ws.double().T
-        lse = torch.logsumexp(z, 1)
-        true = lse - z.gather(1, target[rows, None])[:, 0]
-        # a logit is a sum of `hidden` fp32 products, the sum of exponentials one of `vocab`
-        far = (hidden + 8) * step32 * (xs[rows].norm(dim=1) * float(ws.float().norm(dim=1).max())) + vocab * step32
-        bad_losses, worst = _over(torch, loss[rows], true, 2 * far + 32 * step32 * (1 + true.abs() + lse.abs()))
-        dl = torch.exp(z - lse[:, None]).scatter_add_(1, target[rows, None], -torch.ones_like(lse)[:, None])
-        size = dl.abs() @ ws.double().abs()
-        bad_dx, more = _over(torch, dx[rows], dl @ ws.double(),
-                             (u + 4 * far[:, None] + vocab * step32) * size + u * (dl @ ws.double()).abs() + 1e-7)
-        worst = max(worst, more)
-        # entries of the weight's gradient: the softmax there follows from the tokens' losses
         at = torch.randperm(vocab, device="cuda", generator=gen)[:SAMPLE]
-        at[: SAMPLE // 2] = target[torch.randint(0, tokens, (len(at[: SAMPLE // 2]),), device="cuda", generator=gen)]
-        z_own = (xs * ws[target].double()).sum(1)
-        hit = (target[:, None] == at[None]).double()
-        q = torch.exp(xs @ ws[at].double().T - (loss + z_own)[:, None])
-        err = 4 * ((hidden + 8) * step32 * xs.norm(dim=1) * float(ws.float().norm(dim=1).max()) + vocab * step32)
-        dl = q - hit
-        size = dl.abs().T @ xs.abs()
-        true = dl.T @ xs
-        bad_dw, more = _over(torch, dw[at], true, (u + tokens * step32) * size + (q * err[:, None]).T @ xs.abs()
-                             + u * true.abs() + 1e-7)
-        worst = max(worst, more)
+        hits = len(at) // 2  # half of them are some token's target
+        at[:hits] = target[torch.randint(0, tokens, (hits,), device="cuda", generator=gen)]
+        bad_losses, bad_dx, bad_dw, worst = judge_step(torch, x.detach(), w.detach(), target[:, None],
+                                                       torch.ones((tokens, 1), device="cuda"), 1.0, *first, rows, at)
     return LossScreen(tokens, vocab, hidden, dtype, seconds * 1e3, 6e-12 * tokens * vocab * hidden / seconds, differing,
                       bad_losses, bad_dx, bad_dw, worst)
 
