@@ -71,3 +71,27 @@ def test_one_wrong_value_of_each_is_found():
         where = (rows[3],) if place == 0 else (rows[3], 5) if place == 1 else (at[3], 5)
         got[place][where] += 0.02 if place == 0 else 0.25
         assert [bool(b) for b in _judged(x, w, target, *got, rows, at)[:3]] == [place == i for i in range(3)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_a_teachers_lists_are_judged(dt):
+    """Lists with an entry twice, with none, and with probabilities of 0, at a temperature of 2."""
+    t, (x, w, target, _, _, _, rows, at) = 2.0, _step(*SIZES[0], dt)
+    n, v = SIZES[0][:2]
+    gen = torch.Generator().manual_seed(9)
+    ids = torch.randint(-300, v, (n, 20), generator=gen)
+    ids[:, 0] = ids[:, 5] = target
+    p = torch.softmax(torch.randn((n, 20), generator=gen).double().masked_fill(ids < 0, -float("inf")), 1)
+    z = x.double() @ w.double().T / t
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    loss = t * t * (torch.special.xlogy(p, p) - p * (z.gather(1, ids.clamp_min(0)) - lse)).sum(1)
+    dl = t * torch.exp(z - lse).scatter_add(1, ids.clamp_min(0), -p)
+    once = t * torch.exp(z - lse).scatter(1, ids.clamp_min(0), 0)
+    dx, dw = _gradients(x, w, dl)
+
+    def judged(loss, dx, dw):
+        return head_screen.judge_step(torch, x, w, ids, p, t, loss.float(), dx, dw, rows, at)
+
+    assert judged(loss, dx, dw)[:3] == (0, 0, 0)
+    wrong = _gradients(x, w, once)
+    assert judged(loss, wrong[0], dw)[1] and judged(loss, dx, wrong[1])[2] and judged(loss / t, dx, dw)[0]

@@ -10,7 +10,7 @@
     python -m triton_kubernetes_amd.ops.cli hbm|mfma [...] [--clock]
     python -m triton_kubernetes_amd.ops.cli rccl-slim [--source DIR] [--root DIR] [--no-verify]
     python -m triton_kubernetes_amd.ops.cli gemm [--size N] [--reps R] [--schedule staggered|single-barrier] [--dtype bf16|fp8]
-    python -m triton_kubernetes_amd.ops.cli loss [--tokens N] [--vocab V] [--hidden D] [--reps R] [--dtype bf16|fp16]
+    python -m triton_kubernetes_amd.ops.cli loss [--tokens N] [--vocab V] [--hidden D] [--entries K] [--reps R] [--dtype bf16|fp16]
     python -m triton_kubernetes_amd.ops.cli gemv [--rows M] [--out N] [--inp K] [--group G] [--reps R] [--dtype bf16|fp16]
 
 Every command prints one JSON document (``metrics``: Prometheus text); the exit status is
@@ -117,11 +117,12 @@ def _main(argv: Sequence[str]) -> int:
                    help="GEMM main loop (single-barrier: the earlier loop, for A/B; bf16 only)")
     g.add_argument("--dtype", default="bf16", choices=["bf16", "fp8"],
                    help="operands: bf16, or fp8 e4m3 through the block-scaled MFMA")
-    ls = sub.add_parser("loss", help="a training step's output head (loss and gradients), checked (needs PyTorch)")
+    ls = sub.add_parser("loss", help="steps of an output head (cross entropy, distillation, their gradients), checked (needs PyTorch)")
     ls.add_argument("--device", type=_num(0), default=0)
     ls.add_argument("--tokens", type=_num(1), default=4096)
     ls.add_argument("--vocab", type=_num(1), default=32768)
     ls.add_argument("--hidden", type=_num(1), default=4096)
+    ls.add_argument("--entries", type=_num(0), default=64, help="a teacher's logits a token, at most 1024 (0: no distillation)")
     ls.add_argument("--reps", type=_num(1), default=3)
     ls.add_argument("--dtype", default="bf16", choices=["bf16", "fp16"])
     gv = sub.add_parser("gemv", help="a token's product with a 4-bit weight, checked (needs PyTorch)")
@@ -225,7 +226,8 @@ def _main(argv: Sequence[str]) -> int:
         from . import head_screen
 
         if args.cmd == "loss":
-            res = head_screen.loss_screen(args.device, args.tokens, args.vocab, args.hidden, args.reps, args.dtype)
+            res = head_screen.loss_screen(args.device, args.tokens, args.vocab, args.hidden, args.reps, args.dtype,
+                                          entries=args.entries)
         else:
             res = head_screen.gemv_screen(args.device, args.rows, args.out, args.inp, args.group, args.reps, args.dtype)
         print(json.dumps(res.to_json()))

@@ -3,7 +3,7 @@
 The GEMM screen (``gemm.screen``) proves the matrix cores and the LDS.  These run what a
 training step and a token server run on such a node, and check the answers: the exponential
 and logarithm, sums across lanes, transposing LDS reads and the three products of a backward
-pass (:func:`loss_screen`), and 4-bit codes unpacked and scaled on the way from HBM
+pass, for a cross entropy and a distillation (:func:`loss_screen`), and 4-bit codes unpacked and scaled on the way from HBM
 (:func:`gemv_screen`).  Every pass has to give the bits of the first one, and the first is
 compared with 64-bit sums that torch forms.  Both need PyTorch-ROCm on the node.
 """
@@ -45,8 +45,10 @@ class LossScreen:
     vocab: int
     hidden: int
     dtype: str
-    ms: float
-    tflops: float  # of the 6 N V D that a step cannot do without
+    entries: int  # of a teacher's list, 0: no distillation
+    ms: float  # a step of the cross entropy
+    distill_ms: float
+    tflops: float  # of the 6 N V D that a step of the cross entropy cannot do without
     differing: int  # values that were not the first pass' bits, over all passes
     bad_losses: int
     bad_dx: int
@@ -206,42 +208,63 @@ def judge_step(torch, x, w, ids, p, t, loss, dx, dw, rows, at):
 
 
 def loss_screen(dev: int = 0, tokens: int = 4096, vocab: int = 32768, hidden: int = 4096, reps: int = 3,
-                dtype: str = "bf16", inject: int = -1) -> LossScreen:
-    """``reps`` training steps of the head (loss and both gradients) on random operands.
-    ``inject`` changes one value of the last pass' weight gradient, which has to show."""
+                dtype: str = "bf16", inject: int = -1, entries: int = 64) -> LossScreen:
+    """``reps`` training steps of the head (loss and both gradients) on random operands, and as
+    many distillation steps from lists of ``entries`` logits (0: none).  ``inject`` changes one
+    value of the last cross entropy's weight gradient, which has to show."""
     torch = _torch(dev)
-    from .loss import linear_cross_entropy
+    from .loss import linear_cross_entropy, linear_distill
 
-    dt = _dtype(torch, dtype)
+    dt, temperature, entries = _dtype(torch, dtype), 2.0, min(entries, vocab)
     with _on(torch, dev):
         gen = torch.Generator(device="cuda").manual_seed(0x5eed)
         x, w, target = head_data(torch, tokens, vocab, hidden, dt, gen)
         x.requires_grad_()
         w.requires_grad_()
         ones = torch.ones(tokens, device="cuda")
-
-        def step():
-            loss = linear_cross_entropy(x, w, target, reduction="none")
-            return (loss.detach(), *torch.autograd.grad(loss, (x, w), ones))
-
-        bits = torch.int16
-        first = step()
-        seconds, differing = float("inf"), 0
-        for turn in range(max(1, reps)):
-            got = []
-            seconds = min(seconds, _timed(torch, lambda: got.extend(step()), 1))
-            if inject >= 0 and turn == max(1, reps) - 1:
-                got[2].view(-1)[inject] += 1
-            # the bits, so that a NaN that repeats is no difference here (the comparison below finds it)
-            differing += sum(int((a.view(bits) != b.view(bits)).sum()) for a, b in zip(got, first))
         rows = torch.randperm(tokens, device="cuda", generator=gen)[:SAMPLE]
         at = torch.randperm(vocab, device="cuda", generator=gen)[:SAMPLE]
         hits = len(at) // 2  # half of them are some token's target
         at[:hits] = target[torch.randint(0, tokens, (hits,), device="cuda", generator=gen)]
-        bad_losses, bad_dx, bad_dw, worst = judge_step(torch, x.detach(), w.detach(), target[:, None],
-                                                       torch.ones((tokens, 1), device="cuda"), 1.0, *first, rows, at)
-    return LossScreen(tokens, vocab, hidden, dtype, seconds * 1e3, 6e-12 * tokens * vocab * hidden / seconds, differing,
-                      bad_losses, bad_dx, bad_dw, worst)
+
+        def passes(call, changed):
+            """(seconds, values that differ from the first pass', the first pass)"""
+
+            def step():
+                loss = call()
+                return (loss.detach(), *torch.autograd.grad(loss, (x, w), ones))
+
+            bits = torch.int16
+            first = step()
+            seconds, differing = float("inf"), 0
+            for turn in range(max(1, reps)):
+                got = []
+                seconds = min(seconds, _timed(torch, lambda: got.extend(step()), 1))
+                if changed >= 0 and turn == max(1, reps) - 1:
+                    got[2].view(-1)[changed] += 1
+                # the bits, so that a NaN that repeats is no difference here (the comparison below finds it)
+                differing += sum(int((a.view(bits) != b.view(bits)).sum()) for a, b in zip(got, first))
+            return seconds, differing, first
+
+        def judged(ids, p, t, first):
+            return judge_step(torch, x.detach(), w.detach(), ids, p, t, *first, rows, at)
+
+        seconds, differing, first = passes(lambda: linear_cross_entropy(x, w, target, reduction="none"), inject)
+        found = [judged(target[:, None], torch.ones((tokens, 1), device="cuda"), 1.0, first)]
+        distill = 0.0
+        if entries:  # the target and entries that may occur twice, some of them none
+            ids = torch.randint(-vocab // 8, vocab, (tokens, entries), device="cuda", generator=gen)
+            ids[:, 0] = target
+            logits = 2 * torch.randn((tokens, entries), device="cuda", generator=gen)
+            distill, more, first = passes(lambda: linear_distill(x, w, ids, logits, temperature=temperature,
+                                                                 reduction="none"), -1)
+            differing += more
+            p = torch.softmax(logits.double().masked_fill(ids < 0, -float("inf")) / temperature, 1)
+            found.append(judged(ids, p, temperature, first))
+        bad_losses, bad_dx, bad_dw = (sum(f[i] for f in found) for i in range(3))
+    return LossScreen(tokens, vocab, hidden, dtype, entries, seconds * 1e3, distill * 1e3,
+                      6e-12 * tokens * vocab * hidden / seconds, differing, bad_losses, bad_dx, bad_dw,
+                      max(f[3] for f in found))
 
 
 def gemv_screen(dev: int = 0, rows: int = 1, out: int = 16384, inp: int = 16384, group: int = 128, reps: int = 20,
