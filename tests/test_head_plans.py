@@ -48,3 +48,13 @@ def test_the_backward_workspace_has_a_place_for_the_number_of_splits():
     want = -(-want // 16) * 16
     assert loss._lib().tkl_room_bytes(_args(**sizes)) == want
     assert loss.room_bytes(3, 64, 256, 1, 0, 1, 1) == want
+
+
+@pytest.mark.parametrize("n", [1, 300, 48_211, 524_288, 700_001, 1_040_000, 1 << 20])
+@pytest.mark.parametrize("v", [1, 257, 51_400, 262_144, 1 << 24])
+def test_a_piece_of_the_vocabulary_stays_within_its_memory(n, v):
+    if -(-v // loss.TILE) * -(-n // loss.TILE) >= 1 << 23:
+        return  # refused
+    piece = loss.pieces(n, v)
+    assert piece % loss.TILE == 0 and 2 * n * piece <= 1.5 * loss.DL_BYTES
+    assert (-(-v // piece) - 1) * piece < v  # none is empty

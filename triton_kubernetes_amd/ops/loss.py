@@ -76,7 +76,8 @@ def pieces(n: int, v: int) -> int:
     ``n`` tokens' logits near ``DL_BYTES``, at most half as much again (a second piece for a little
     more costs 2 %: 5000 x 2048 x 60000 in one 3262 us, in two 3327), spread evenly, in whole tiles."""
     count = max(1, min((4 * n * v // DL_BYTES + 1) // 2, -(-v // TILE)))
-    return _up(-(-v // count), TILE)
+    # (of a great many tokens a whole tile more can be past that)
+    return min(_up(-(-v // count), TILE), max(TILE, 3 * DL_BYTES // (4 * n) // TILE * TILE))
 
 
 def small_products(n: int, d: int, v: int) -> int:
