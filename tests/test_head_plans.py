@@ -58,3 +58,20 @@ def test_a_piece_of_the_vocabulary_stays_within_its_memory(n, v):
     piece = loss.pieces(n, v)
     assert piece % loss.TILE == 0 and 2 * n * piece <= 1.5 * loss.DL_BYTES
     assert (-(-v // piece) - 1) * piece < v  # none is empty
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), float("inf"), 1e300, 1e20, 2.0 ** 33, 2.0 ** -33, 1e-20, 5e-324])
+def test_temperatures_whose_square_or_quotient_fp32_does_not_hold_are_refused(temperature):
+    from test_head_ops import _args
+
+    with pytest.raises(loss.LossError, match="temperature"):
+        plan(4, 64, 300, k=3, temperature=temperature)
+    if temperature < 1e38 or temperature != temperature:
+        for call in (loss._lib().tkl_forward, loss._lib().tkl_backward):
+            assert call(_args(temperature=temperature)) == -1
+            assert b"temperature" in loss._lib().tkl_last_error()
+
+
+@pytest.mark.parametrize("temperature", [2.0 ** -32, 0.7, 1, 2.0 ** 32])
+def test_temperatures_that_are_taken(temperature):
+    assert plan(4, 64, 300, k=3, temperature=float(temperature)).temperature == temperature

@@ -1459,7 +1459,7 @@ int check(const tkl_args& a) {
   else if ((a.v + 255) / 256 * ((a.n + 255) / 256) >= 1 << 23) bad = "tokens x vocabulary must be below 2^39";
   else if ((a.d + 1023) / 1024 * a.n >= 1 << 24) bad = "tokens x width must be below 2^34";
   else if (a.reduction < 0 || a.reduction > 2) bad = "reduction must be 0 to 2";
-  else if (!(a.temperature > 0.f)) bad = "the temperature must be above 0";
+  else if (!(a.temperature >= 0x1p-32f && a.temperature <= 0x1p32f)) bad = "the temperature must be 2^-32 to 2^32";
   if (bad) {
     snprintf(g_err, sizeof(g_err), "%s", bad);
     return -1;

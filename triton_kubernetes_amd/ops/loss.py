@@ -21,7 +21,6 @@ known here, and the same holds for it.
 
 import ctypes
 import functools
-import math
 import struct
 from typing import Optional
 
@@ -35,6 +34,7 @@ MAX_TARGETS = 1024  # ids of a token's list
 MAX_TOKENS = 1 << 20
 MAX_WIDTH = 1 << 16
 MAX_VOCAB = 1 << 24
+MAX_TEMPERATURE_BITS = 32  # the temperature's square, and logits over it, are fp32 numbers
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
@@ -231,8 +231,9 @@ def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, 
         p.k, p.distill = id_shape[-1], 1
         if p.k > MAX_TARGETS:
             raise LossError(f"{what}: {p.k} entries a token (at most {MAX_TARGETS})")
-        if not (math.isfinite(temperature) and temperature > 0):
-            raise LossError(f"{what}: the temperature must be above 0, not {temperature}")
+        if not 2.0 ** -MAX_TEMPERATURE_BITS <= temperature <= 2.0 ** MAX_TEMPERATURE_BITS:  # (not if it is NaN)
+            raise LossError(f"{what}: the temperature must be 2^-{MAX_TEMPERATURE_BITS} to 2^{MAX_TEMPERATURE_BITS}, "
+                            f"not {temperature}")
     if not -(1 << 63) <= ignore < 1 << 63:
         raise LossError(f"{what}: no target can be {ignore}")
     p.reduction, p.temperature, p.ignore = REDUCTIONS[reduction], temperature, ignore
@@ -399,7 +400,8 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     (fp32, bf16 or fp16; no gradient).  An id below 0 is no entry, so lists may differ in
     length; a token without any entry (or with logits of -inf alone) has loss 0 and takes part
     in no sum.  An entry listed twice counts twice.  An id past the vocabulary makes the
-    token's loss NaN.  ``x``, ``w``, ``reduction`` and ``keep_logits`` are those of
+    token's loss NaN.  The temperature is 2^-32 to 2^32; the loss has the rounding of fp32
+    logarithms times its square.  ``x``, ``w``, ``reduction`` and ``keep_logits`` are those of
     :func:`linear_cross_entropy`."""
     import torch
 
