@@ -408,4 +408,6 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     plan = _planned("linear_distill", x, w, ids, logits, reduction, float(temperature), 0, keep_logits)
     if logits.requires_grad and torch.is_grad_enabled():
         raise LossError("linear_distill gives the teacher's logits no gradient: detach them")
+    if torch.autograd.forward_ad._current_level >= 0 and torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
+        raise LossError("linear_distill gives the teacher's logits no gradient: detach them")
     return _apply(x, w, _ids(ids), logits.detach().float().contiguous(), plan)
