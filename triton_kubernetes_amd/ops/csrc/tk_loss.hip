@@ -1243,7 +1243,8 @@ __global__ __launch_bounds__(1024) void k_reduce(const float* __restrict__ rowlo
   }
 }
 
-// fp16 without a reduction: factor[pos] = span g / max|g|, factor[n] = max|g| T / span.
+// fp16 without a reduction: factor[pos] = span g / max|g|, factor[n] = max|g| T / span, with the largest
+// finite |g|, so that an infinite one (a loss scale that was too high) leaves the other tokens theirs.
 __global__ __launch_bounds__(1024) void k_factor(const float* __restrict__ grad, long long ldg,
                                                  const int* __restrict__ rowmap, const int* __restrict__ count, int n,
                                                  float t, float span, float* __restrict__ factor) {
@@ -1251,11 +1252,15 @@ __global__ __launch_bounds__(1024) void k_factor(const float* __restrict__ grad,
   const int rows = count[0];
   float m = 0.f;
 #pragma unroll 8
-  for (int i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(grad[rowmap[i] * ldg]));
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float g = fabsf(grad[rowmap[i] * ldg]);
+    m = g < INFINITY ? fmaxf(m, g) : m;
+  }
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
   __syncthreads();
   for (int i = 0; i < 16; ++i) m = fmaxf(m, top[i]);
+  if (m == 0.f) m = 1.f;
 #pragma unroll 8
   for (int i = threadIdx.x; i < rows; i += 1024) {
     const float g = grad[rowmap[i] * ldg];
