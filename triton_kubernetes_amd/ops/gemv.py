@@ -197,6 +197,8 @@ def quantize_w4(w, group: int = 128, symmetric: bool = True) -> Tuple[Any, Any, 
         zeros = None
     else:
         lo, hi = v.amin(2).clamp_max(0), v.amax(2).clamp_min(0)
+        if not bool(torch.isfinite(hi - lo).all()):
+            raise GemvError("quantize_w4 wants groups whose span is an fp32 number")
         scales = ((hi - lo) / 15).to(w.dtype)
     # codes go by the rounded scale; a scale of 0 (a group of zeros, or too small for the type) has code = zero
     step = scales.float()
