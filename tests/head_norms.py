@@ -37,8 +37,9 @@ def exact(x, w, ids, p, t, g):
     return loss, dl @ b, dl.T @ a, dict(x=a, w=b, z=z, lse=lse[:, 0], q=q, dl=dl, g=g, at=at, listed=ids >= 0, size=size, t=t)
 
 
-def wrong(dt, true, got, kept=False):
-    """The names of what is further from ``true`` (of :func:`exact`) than it may be."""
+def wrong(dt, true, got, kept=False, precise=False):
+    """The names of what is further from ``true`` (of :func:`exact`) than it may be.  ``precise``: the
+    derivative is multiplied in two 16-bit parts, so that u^2 is what its rounding costs."""
     (loss, dx, dw, m), u = true, U[dt]
     (n, d), v, t = m["x"].shape, m["w"].shape[0], m["t"]
     far = 8 * STEP * (m["x"].norm(dim=1) * m["w"].norm(dim=1).max() / t + (d ** 0.5 + 2) * m["z"].abs().amax(1))
@@ -51,7 +52,7 @@ def wrong(dt, true, got, kept=False):
 
     over("loss", (got[0].double() - loss).abs(), t * t * (2 * off + (8 + m["at"].shape[1]) * STEP * m["size"]))
     span = m["g"].abs() * t * m["q"]
-    each = (u * m["dl"]).square() + (span * (far + 2.0 ** -20)[:, None]).square()
+    each = ((u * u if precise else u) * m["dl"]).square() + (span * (far + 2.0 ** -20)[:, None]).square()
     if dt == torch.float16:
         each += (float(m["g"].abs().max()) * t * 2.0 ** -40) ** 2
     if kept:

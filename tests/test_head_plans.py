@@ -75,3 +75,26 @@ def test_temperatures_whose_square_or_quotient_fp32_does_not_hold_are_refused(te
 @pytest.mark.parametrize("temperature", [2.0 ** -32, 0.7, 1, 2.0 ** 32])
 def test_temperatures_that_are_taken(temperature):
     assert plan(4, 64, 300, k=3, temperature=float(temperature)).temperature == temperature
+
+
+def test_a_precise_gradient_has_two_parts_in_the_memory_of_one():
+    from test_head_ops import _args
+
+    def precise(n, d, v, keep=False):
+        def meta(*shape, dtype=torch.bfloat16):
+            return torch.Size(shape), dtype, CUDA
+
+        return loss._plan("linear_cross_entropy", meta(n, d), meta(v, d), meta(n, dtype=torch.int64), None, "mean", 1.0, -100,
+                          keep, True, (), True)
+
+    for n, d, v in ((1, 8, 1), (48, 512, 1000), (4096, 4096, 32768), (8192, 4096, 131072), (1 << 20, 8, 40)):
+        p, usual = precise(n, d, v), plan(n, d, v)
+        assert p.small == usual.small | 8 and not p.keep and p.kept == usual.kept
+        assert 4 * n * p.piece <= max(1.5 * loss.DL_BYTES, 4 * n * loss.TILE) and p.piece <= usual.piece
+        args = _args(n=n, d=d, v=v, want=3, piece=p.piece, fill=p.groups, small=p.small, parts=p.parts[3])
+        assert loss._lib().tkl_room_bytes(args) == p.room[3]
+    assert not precise(48, 512, 1000, None).keep
+    with pytest.raises(loss.LossError, match="kept logits"):
+        precise(48, 512, 1000, True)
+    assert loss._lib().tkl_backward(_args(small=8, codes=4096)) == -1
+    assert b"kept logits" in loss._lib().tkl_last_error()

@@ -18,8 +18,12 @@
 // again (k_logits<DL>), or from codes that the forward pass kept (k_dl, struct Codes); a
 // teacher's targets are put in by k_fix; then dX += dl W and dW = dl^T X.
 //
-// dl is rounded to 16 bits, which costs each product about as much as the rounding of its result.
-// Most of a row's derivative is at its target, though, and few numbers' roundings do not average
+// dl is rounded to 16 bits, which costs each product about as much as the rounding of its result, so
+// that the gradients are off by up to sqrt(2) times that (2048 tokens, 64 entries of a teacher: 1.41).
+// A caller who wants less has dl in two parts (k_logits<TWO>): what its rounding took is rounded to 16
+// bits too and multiplied in its turn, which leaves 2^-16 of dl in bf16, 2^-22 in fp16 (errors 1.000
+// times; 4096 x 4096 x 32768 5.3 ms for 3.5, 8192 x 4096 x 131072 41.8 for 26.7).
+// In one part, most of a row's derivative is at its target, though, and few numbers' roundings do not average
 // out: up to FEW_ROWS packed rows, what the largest ones lose (`lost`, RESIDUALS a row) is added
 // to dX and dW in fp32.  (48 tokens, bf16: error 1.0 instead of 1.25 times that of rounding the
 // exact gradients; one token alone can have twice as much.  For 4096 tokens it would be 1.0
@@ -70,7 +74,7 @@ struct tkl_args {
   int dev, f16, distill, reduction;  // reduction 0 none, 1 sum, 2 mean
   float temperature;
   int want;                    // backward: 1 dX, 2 dW, 3 both
-  int small;                   // products in small tiles: 1 the logits, 2 dX, 4 dW
+  int small;                   // products in small tiles: 1 the logits, 2 dX, 4 dW; 8: dl in two parts
   int parts;                   // backward: of the tokens for dW; more than 1 only where there is one piece
   const void *x, *w, *ids, *teacher, *grad;
   void *loss, *kept;           // kept: from forward to backward (struct Kept)
@@ -306,7 +310,6 @@ template <bool F16, bool AA, bool BA>
 __device__ __forceinline__ void product_small(f32x4 (&acc)[2][4], char* smem, const Panel<AA, 128, 256>& pa,
                                               const Panel<BA, 64, 256>& pb, int nk, int tid) {
   using Tile = Small;
-  clear<Tile>(acc);
   if (nk <= 0) return;
   constexpr int BYTES = (Tile::BM + Tile::BN) * KT * 2, AB = Tile::BM * KT * 2, DEPTH = Tile::STEPS;
   constexpr int COPIES = Panel<AA, 128, 256>::COPIES + Panel<BA, 64, 256>::COPIES;
@@ -358,7 +361,6 @@ __device__ __forceinline__ void product_big(Acc<Big>& acc, char* smem, const Pan
                                         const PanelB<Big, BA>& pb, int nk, int tid) {
   constexpr int HBYTES = 128 * KT * 2;
   const int lane = tid & 63, wid = tid >> 6, wr = wid >> 2, wc = wid & 3;
-  clear<Big>(acc);
   if (nk <= 0) return;
 
   const unsigned lds0 = lds_of(smem) + __builtin_amdgcn_readfirstlane(wid) * 64 * 16;
@@ -465,9 +467,12 @@ __device__ __forceinline__ void product_big(Acc<Big>& acc, char* smem, const Pan
   if (wr == 0) barrier();  // the other group's extra barrier
 }
 
-template <class Tile, bool F16, bool AA, bool BA, bool FLIP = false>
+// (MORE: added to what acc holds, after a barrier, for LDS still holds the product before)
+template <class Tile, bool F16, bool AA, bool BA, bool FLIP = false, bool MORE = false>
 __device__ __forceinline__ void multiply(Acc<Tile>& acc, char* smem, const PanelA<Tile, AA>& pa,
                                          const PanelB<Tile, BA>& pb, int nk, int tid) {
+  if constexpr (MORE) __syncthreads();
+  else clear<Tile>(acc);
   if constexpr (Tile::BM == 256) product_big<F16, AA, BA, FLIP>(acc, smem, pa, pb, nk, tid);
   else product_small<F16, AA, BA>(acc, smem, pa, pb, nk, tid);
 }
@@ -569,8 +574,8 @@ struct Codes {
 // many entries of few tokens and the softmax's sums need two shuffles a token.
 // LSE: writes part[tile][token] = (max, sum); KEEP: and the logits' codes to `out`.  DL: writes
 // f (q - p) in 16 bits to `out`, with a cross entropy's p; `targets` is null for a teacher's
-// lists.  sc = log2(e) / T.
-enum Mode { LSE, KEEP, DL };
+// lists.  TWO: the same, and what that rounding took, in 16 bits, to `low`.  sc = log2(e) / T.
+enum Mode { LSE, KEEP, DL, TWO };
 template <class Tile, bool F16, Mode MODE>
 __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict__ w, long long ldw,
                                                           const void* __restrict__ xc, long long ldxc, int v0,
@@ -578,7 +583,8 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
                                                           float sc, float2* __restrict__ part,
                                                           const float* __restrict__ lse, Upstream<F16> up,
                                                           const int* __restrict__ targets, void* __restrict__ out,
-                                                          long long ldout, float* __restrict__ lost) {
+                                                          long long ldout, float* __restrict__ lost,
+                                                          void* __restrict__ low) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
   const int rows = count[0];
@@ -597,7 +603,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
   const int vn = vend - v0;
   const bool whole = (tv + 1) * Tile::BM <= vn;
   const int first = tn * Tile::BN, here = min(Tile::BN, rows - first);
-  if constexpr (MODE != DL) {
+  if constexpr (MODE == LSE || MODE == KEEP) {
     barrier();  // LDS has been read
     float2* sums = reinterpret_cast<float2*>(smem + Outgoing<Tile, T>::BYTES);  // [WAVES_M][BN]
 #pragma unroll
@@ -678,10 +684,25 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
             if (vb + at + e >= vn) g[e] = 0.f;  // zeros pad the piece
         }
         Outgoing<Tile, T>::put(smem, Tile::col(j, wid) + fr, at + fq * 4, g[0], g[1], g[2], g[3]);
+        if constexpr (MODE == TWO) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = g[e] - (float)(T)g[e];
+        }
       }
     }
     __syncthreads();
     Outgoing<Tile, T>::store(smem, static_cast<T*>(out), ldout, first, here, tv * Tile::BM, Tile::BM, tid);
+    if constexpr (MODE == TWO) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < Tile::NF; ++j)
+#pragma unroll
+        for (int i = 0; i < Tile::MF; ++i)
+          Outgoing<Tile, T>::put(smem, Tile::col(j, wid) + fr, Tile::row(i, wid) + fq * 4, acc[i][j][0], acc[i][j][1],
+                                 acc[i][j][2], acc[i][j][3]);
+      __syncthreads();
+      Outgoing<Tile, T>::store(smem, static_cast<T*>(low), ldout, first, here, tv * Tile::BM, Tile::BM, tid);
+    }
   }
 }
 
@@ -820,13 +841,13 @@ __global__ __launch_bounds__(256) void k_transpose(const T* __restrict__ xc, int
 // launch: 21 us both ways at 8192 x 512 x 1000.)  Where dW has few tiles the tokens are split over
 // blockIdx.y, and each part writes its fp32 sums [v][dp], which k_dw_out adds in order (8192 x 512 x
 // 1000, 128 tiles: 86 us whole, 26 in 4 parts).
-template <class Tile, bool F16>
+template <class Tile, bool F16, bool TWICE>
 __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ xt, long long ldxt,
                                                       const void* __restrict__ xc, int dp, const void* __restrict__ dl,
                                                       long long lddl, int v0, int vn, int d, const int* __restrict__ count, Upstream<F16> up,
                                                       const int* __restrict__ at, const float* __restrict__ lost,
                                                       int residuals, void* __restrict__ dw, int lddw,
-                                                      float* __restrict__ sums) {
+                                                      float* __restrict__ sums, const void* __restrict__ low) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
   const int rows = count[0], per = ((rows + KT - 1) / KT + gridDim.y - 1) / gridDim.y * KT;
@@ -836,19 +857,24 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
   tile_of(run_of(blockIdx.x, tiles_d * tiles_v), tiles_d, tiles_v, &td, &tv);
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const PanelB<Tile, false> pb(dl, lddl, tv * Tile::BN, (int)(lddl / 2), k0, k, tid);
+  auto of_low = [&] { return PanelB<Tile, false>(low, lddl, tv * Tile::BN, (int)(lddl / 2), k0, k, tid); };
   Acc<Tile> acc;
   if constexpr (Tile::BM == Tile::BN) {
     const PanelA<Tile, true> pa(xt, ldxt, td * Tile::BM, dp, k0, (k + 7) & ~7, tid);
     multiply<Tile, F16, true, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+    if constexpr (TWICE)
+      multiply<Tile, F16, true, false, false, true>(acc, smem, pa, of_low(), (k + KT - 1) / KT, tid);
   } else {
     const PanelA<Tile, false> pa(xc, 2 * dp, td * Tile::BM, dp, k0, k, tid);
     multiply<Tile, F16, false, false>(acc, smem, pa, pb, (k + KT - 1) / KT, tid);
+    if constexpr (TWICE)
+      multiply<Tile, F16, false, false, false, true>(acc, smem, pa, of_low(), (k + KT - 1) / KT, tid);
   }
 
   // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
-  // share of the packed rows, in order; beyond ROOM of them a sum has so many targets that their
-  // roundings average out.  Their rows of Xc come through LDS, 64 at a time.
-  if (rows <= FEW_ROWS && blockIdx.y == 0) {
+  // share of the packed rows, in order; beyond ROOM of them the rounding stays, as it does past
+  // FEW_ROWS.  Their rows of Xc come through LDS, 64 at a time.
+  if (!TWICE && rows <= FEW_ROWS && blockIdx.y == 0) {
     constexpr int WAVES = Tile::THREADS / 64, ROOM = 32, PER = Tile::BM / 8;
     struct Hit {
       int pos, col;
@@ -1277,7 +1303,7 @@ __global__ __launch_bounds__(256) void k_fix(const long long* __restrict__ ids, 
                                              long long v, const float* __restrict__ zk, const float* __restrict__ lse,
                                              Upstream<F16> up, float sc, long long v0, long long vn,
                                              void* __restrict__ dl, long long lddl, int* __restrict__ at,
-                                             float* __restrict__ lost) {
+                                             float* __restrict__ lost, void* __restrict__ low) {
   using T = typename Type<F16>::T;
   __shared__ __attribute__((aligned(16))) int list[4][MAX_TARGETS];  // vocabulary entries, -1: none
   __shared__ __attribute__((aligned(16))) float prob[4][MAX_TARGETS];
@@ -1316,6 +1342,7 @@ __global__ __launch_bounds__(256) void k_fix(const long long* __restrict__ ids, 
     const bool here = id >= v0 && id < v0 + vn;
     const T r = (T)(f * g);
     if (here) static_cast<T*>(dl)[(size_t)pos * lddl + (id - v0)] = r;
+    if (here && low) static_cast<T*>(low)[(size_t)pos * lddl + (id - v0)] = (T)(f * g - (float)r);
     if (fabsf(g) >= LARGE && slot < RESIDUALS) {
       if (v0 == 0) at[pos * RESIDUALS + slot] = id;
       if (here) lost[pos * RESIDUALS + slot] = f * g - (float)r;
@@ -1372,6 +1399,7 @@ __global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, 
 int padded(long long d) { return (int)((d + 63) / 64 * 64); }
 
 int residuals(const tkl_args& a) { return a.distill ? RESIDUALS : 1; }
+int halves(const tkl_args& a) { return a.small & 8 ? 2 : 1; }  // parts of dl
 
 // What the forward pass keeps, in one buffer.  Without a teacher p and flag are not there.
 struct Kept {
@@ -1408,6 +1436,7 @@ Kept kept_of(const tkl_args& a) {
 // The backward pass' workspace, in one buffer.
 struct Room {
   void* dl;       // [n][piece] 16-bit
+  void* low;      // the same, what dl's rounding took, or null
   float* sums;    // [splits][packed rows][dp] of dX: n dp, or what `fill` tiles hold
   float* factor;  // [n + 1]
   int* splits;    // of dX, as k_dx found them
@@ -1420,7 +1449,8 @@ Room room_of(const tkl_args& a) {
   Room r;
   char* at = static_cast<char*>(a.room);
   r.dl = at;
-  at += 2 * a.n * a.piece;
+  r.low = halves(a) > 1 ? at + 2 * a.n * a.piece : nullptr;
+  at += 2 * a.n * a.piece * halves(a);
   r.sums = reinterpret_cast<float*>(at);
   const long long once = a.n * padded(a.d), tile = a.small & 2 ? Small::BM * Small::BN : Big::BM * Big::BN;
   if (a.want & 1) at += 4 * std::max(once, std::min(a.piece / 512 * once, a.fill * tile));
@@ -1481,9 +1511,11 @@ template <class Tile, bool F16>
 hipError_t allow_all() {
   hipError_t e = allow(&k_logits<Tile, F16, LSE>, Tile::LDS);
   if (e == hipSuccess) e = allow(&k_logits<Tile, F16, DL>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_logits<Tile, F16, TWO>, Tile::LDS);
   if (e == hipSuccess) e = allow(&k_logits<Tile, F16, KEEP>, Tile::LDS);
   if (e == hipSuccess) e = allow(&k_dx<Tile, F16>, Tile::LDS);
-  if (e == hipSuccess) e = allow(&k_dw<Tile, F16>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_dw<Tile, F16, false>, Tile::LDS);
+  if (e == hipSuccess) e = allow(&k_dw<Tile, F16, true>, Tile::LDS);
   return e;
 }
 hipError_t set_lds_limit() {
@@ -1519,16 +1551,16 @@ float2* part_of(const tkl_args& a) {
 
 template <class Tile, bool F16, Mode MODE>
 void logits_as(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
-               void* out, long long ldout, float* lost, hipStream_t s) {
+               void* out, long long ldout, float* lost, void* low, hipStream_t s) {
   k_logits<Tile, F16, MODE><<<blocks(vn, Tile::BM) * blocks(a.n, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
       w.at, w.ldb, kept.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, kept.count, (int)a.n, LOG2E / a.temperature,
-      part_of(a), kept.lse, up, a.distill ? nullptr : kept.at, out, ldout, lost);
+      part_of(a), kept.lse, up, a.distill ? nullptr : kept.at, out, ldout, lost, low);
 }
 
 template <class Tile, bool F16>
 void all_logits(const tkl_args& a, const Kept& q, const Weight& w, int dp, hipStream_t s) {
-  if (a.codes) logits_as<Tile, F16, KEEP>(a, q, w, dp, 0, (int)a.v, {}, a.codes, Codes::stride(a.v), nullptr, s);
-  else logits_as<Tile, F16, LSE>(a, q, w, dp, 0, (int)a.v, {}, nullptr, 0, nullptr, s);
+  if (a.codes) logits_as<Tile, F16, KEEP>(a, q, w, dp, 0, (int)a.v, {}, a.codes, Codes::stride(a.v), nullptr, nullptr, s);
+  else logits_as<Tile, F16, LSE>(a, q, w, dp, 0, (int)a.v, {}, nullptr, 0, nullptr, nullptr, s);
 }
 
 // dl of a piece, out of the kept logits or by computing them again
@@ -1539,8 +1571,10 @@ void derivative(const tkl_args& a, const Kept& q, const Weight& w, int dp, long 
     k_dl<Tile, F16><<<blocks(a.piece, 2048) * (unsigned)a.n, 256, 0, s>>>(
         static_cast<const unsigned short*>(a.codes), Codes::stride(a.v), part_of(a), (int)a.n, (int)v0, vn,
         LOG2E / a.temperature, q.lse, up, a.distill ? nullptr : q.at, q.zk, r.dl, a.piece, r.lost);
+  else if (r.low)
+    logits_as<Tile, F16, TWO>(a, q, w, dp, v0, vn, up, r.dl, a.piece, r.lost, r.low, s);
   else
-    logits_as<Tile, F16, DL>(a, q, w, dp, v0, vn, up, r.dl, a.piece, r.lost, s);
+    logits_as<Tile, F16, DL>(a, q, w, dp, v0, vn, up, r.dl, a.piece, r.lost, nullptr, s);
 }
 
 template <bool F16>
@@ -1578,15 +1612,18 @@ void dx(const tkl_args& a, const Kept& q, const Room& r, const Weight& w, int dp
   const unsigned most = std::max<long long>((long long)blocks(w.dk, Tile::BM) * blocks(a.n, Tile::BN), a.fill);
   k_dx<Tile, F16><<<most, Tile::THREADS, Tile::LDS, s>>>(w.at, w.ldb, r.dl, a.piece * 2, (int)v0, vn, w.dk, dp, q.count,
                                                          (int)a.fill, v0 == 0, r.sums, r.splits);
+  if (r.low)
+    k_dx<Tile, F16><<<most, Tile::THREADS, Tile::LDS, s>>>(w.at, w.ldb, r.low, a.piece * 2, (int)v0, vn, w.dk, dp,
+                                                           q.count, (int)a.fill, 0, r.sums, r.splits);
 }
 
 template <class Tile, bool F16>
 void dw(const tkl_args& a, const Kept& q, const Room& r, int dp, long long v0, int vn, const Upstream<F16>& up,
         hipStream_t s) {
   const dim3 grid(blocks(a.d, Tile::BM) * blocks(vn, Tile::BN), std::max(1, a.parts));
-  k_dw<Tile, F16><<<grid, Tile::THREADS, Tile::LDS, s>>>(r.xt, 2 * padded(a.n), q.xc, dp, r.dl, a.piece * 2, (int)v0, vn,
-                                                         (int)a.d, q.count, up, q.at, r.lost, residuals(a), a.dw,
-                                                         (int)a.d, r.parts);
+  auto* kernel = r.low ? &k_dw<Tile, F16, true> : &k_dw<Tile, F16, false>;
+  kernel<<<grid, Tile::THREADS, Tile::LDS, s>>>(r.xt, 2 * padded(a.n), q.xc, dp, r.dl, a.piece * 2, (int)v0, vn, (int)a.d,
+                                                q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d, r.parts, r.low);
   if (a.parts > 1)
     k_dw_out<F16><<<blocks(a.v * (dp / 4), 256), 256, 0, s>>>(r.parts, a.parts, a.v, (int)a.d, dp, up, a.dw);
 }
@@ -1612,7 +1649,7 @@ hipError_t backward(const tkl_args& a) {
     else derivative<Big, F16>(a, q, w, dp, v0, vn, up, r, s);
     if (a.distill)
       k_fix<F16><<<blocks(n, 4), 256, 0, s>>>(static_cast<const long long*>(a.ids), q.p, k, a.v, q.zk, q.lse, up,
-                                              LOG2E / a.temperature, v0, vn, r.dl, a.piece, q.at, r.lost);
+                                              LOG2E / a.temperature, v0, vn, r.dl, a.piece, q.at, r.lost, r.low);
     if (a.want & 1) {
       if (a.small & 2) dx<Small, F16>(a, q, r, w, dp, v0, vn, s);
       else dx<Big, F16>(a, q, r, w, dp, v0, vn, s);
@@ -1624,7 +1661,7 @@ hipError_t backward(const tkl_args& a) {
   }
   if (a.want & 1)
     k_dx_out<F16><<<blocks(d, 1024) * (unsigned)n, 256, 0, s>>>(r.sums, r.splits, d, dp, q.posof, up, q.at, r.lost,
-                                                                residuals(a), w.at, w.ldb / 2, a.dx);
+                                                                r.low ? 0 : residuals(a), w.at, w.ldb / 2, a.dx);
   return hipGetLastError();
 }
 
@@ -1657,6 +1694,10 @@ extern "C" int tkl_forward(const tkl_args* a) { return on_device(a, a->f16 ? for
 extern "C" int tkl_backward(const tkl_args* a) {
   if (a->parts < 0 || a->parts > 64 || (a->parts > 1 && a->piece < a->v)) {
     snprintf(g_err, sizeof(g_err), "dW in %d parts: at most 64, of one piece", a->parts);
+    return -1;
+  }
+  if (halves(*a) > 1 && a->codes) {
+    snprintf(g_err, sizeof(g_err), "kept logits are rounded: their derivative has no second part");
     return -1;
   }
   // (a tile's rows of dl are addressed below FAR)

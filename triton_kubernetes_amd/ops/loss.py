@@ -137,14 +137,14 @@ def part_bytes(n: int, v: int, small: bool) -> int:
 
 def room_bytes(n: int, d: int, piece: int, groups: int, small: int, want: int, lists: int,
                weight: int = 0) -> int:
-    """Of the backward pass' workspace: the derivative of a piece's logits, fp32 sums of x's
+    """Of the backward pass' workspace: the derivative of a piece's logits (twice with ``small & 8``), fp32 sums of x's
     gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors,
     the number of splits, residuals, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``,
     unless ``small & 4``)."""
-    once = n * _up(d, 64)
+    once, halves = n * _up(d, 64), 2 if small & 8 else 1
     tiles = groups * (SMALL_M * SMALL_N if small & 2 else TILE * TILE)
     sums = max(once, min(piece // 512 * once, tiles)) if want & 1 else 0
-    return _up(2 * n * piece + 4 * sums + 4 * (n + 2) + (16 * n if lists else 4 * n), 16) \
+    return _up(2 * n * piece * halves + 4 * sums + 4 * (n + 2) + (16 * n if lists else 4 * n), 16) \
         + 4 * weight * _up(d, 64) + (2 * _up(d, 64) * _up(n, 64) if want & 2 and not small & 4 else 0)
 
 
@@ -196,7 +196,7 @@ _INTEGERS = ("torch.int64", "torch.int32", "torch.int16", "torch.uint8", "torch.
 
 
 @functools.lru_cache(maxsize=256)
-def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, rules) -> _Plan:
+def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, rules, precise=False) -> _Plan:
     """The plan of a call whose tensors have these ``(shape, dtype, device)``; calls alike share one
     (``rules``: what else the sizes come from)."""
     (shape, dtype, device), (by, w_type, w_device) = x, w
@@ -237,16 +237,20 @@ def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, 
     if not -(1 << 63) <= ignore < 1 << 63:
         raise LossError(f"{what}: no target can be {ignore}")
     p.reduction, p.temperature, p.ignore = REDUCTIONS[reduction], temperature, ignore
+    if precise and keep:
+        raise LossError(f"{what}: kept logits are rounded, so a precise gradient has to compute them again")
     p.f16, p.device = str(dtype) == "torch.float16", device.index
     if n and p.k:
-        p.small = small_products(n, d, v)
-        p.keep = grads and (keeps(n, d, v) if keep is None else bool(keep))
+        p.small = small_products(n, d, v) | (8 if precise else 0)
+        p.keep = grads and not precise and (keeps(n, d, v) if keep is None else bool(keep))
         p.kept = _up(kept_bytes(n, d, n * p.k if p.distill else 0), 256)
         p.codes = p.kept if p.keep else 0  # the logits lie behind the rest
         p.sums = part_bytes(n, v, bool(p.small & 1))
         if p.keep:
             p.kept += codes_bytes(n, v, bool(p.small & 1))
         p.piece = pieces(n, v)
+        if precise:  # half of the piece's memory for each part
+            p.piece = min(p.piece, pieces(2 * n, v))
         p.groups = fill(bool(p.small & 2))
         parts = weight_parts(n, d, v) if p.small & 4 and p.piece >= v else 1
         p.parts = (1, 1, parts, parts)  # by the gradients that are wanted
@@ -255,14 +259,14 @@ def _plan(what, x, w, ids, logits, reduction, temperature, ignore, keep, grads, 
     return p
 
 
-def _planned(what, x, w, ids, logits, reduction, temperature, ignore, keep):
+def _planned(what, x, w, ids, logits, reduction, temperature, ignore, keep, precise):
     import torch
 
     grads = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
     rules = (small_products, keeps, pieces, fill, weight_parts, DL_BYTES, KEEP_BYTES)
     return _plan(what, (x.shape, x.dtype, x.device), (w.shape, w.dtype, w.device), (ids.shape, ids.dtype, ids.device),
                  None if logits is None else (logits.shape, logits.dtype, logits.device), reduction, temperature, ignore,
-                 keep, grads, rules)
+                 keep, grads, rules, bool(precise))
 
 
 def _ids(ids):
@@ -371,7 +375,7 @@ def _autograd():
 
 
 def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: str = "mean",
-                         keep_logits: Optional[bool] = False):
+                         keep_logits: Optional[bool] = False, precise_grad: bool = False):
     """Softmax cross entropy of the logits ``x @ w.T`` against ``target``, in fp32.
 
     ``x [..., D]`` and ``w [V, D]`` are both bf16 or both fp16, of any strides (rows that are
@@ -385,13 +389,20 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
     for as long as the loss lives, instead of computing them again, and ``None`` does so up to
     ``KEEP_BYTES`` where :func:`keeps` finds that faster.  Kept logits are rounded: a probability
     is then off by up to 8.5e-5 of itself, 3.4e-4 below 2^-8 of its tile's largest and 2.7e-3
-    below 2^-24, which joins the rounding of the gradient's operands."""
-    plan = _planned("linear_cross_entropy", x, w, target, None, reduction, 1.0, int(ignore_index), keep_logits)
+    below 2^-24, which joins the rounding of the gradient's operands.
+
+    These are in 16 bits: ``x``, ``w``, and the derivative of the logits, rounded to their type.
+    The gradients are then off by up to 1.42 times what rounding them once costs (1.0 for a few
+    confident tokens, 1.18 for a training step of 4096 tokens, 1.41 where a teacher's lists spread the
+    derivative).  ``precise_grad=True`` multiplies the derivative in two 16-bit parts instead, so that
+    little but the result's own rounding is left (1.00 times), for about half as much time again."""
+    plan = _planned("linear_cross_entropy", x, w, target, None, reduction, 1.0, int(ignore_index), keep_logits,
+                    precise_grad)
     return _apply(x, w, _ids(target), None, plan)
 
 
 def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: str = "mean",
-                   keep_logits: Optional[bool] = False):
+                   keep_logits: Optional[bool] = False, precise_grad: bool = False):
     """Divergence of the softmax of ``x @ w.T / temperature`` from a teacher's, times
     ``temperature ** 2``, in fp32: per token ``sum_k p_k (log p_k - log q_k)`` over the listed
     entries, with ``p`` the softmax of ``logits / temperature`` over them.
@@ -401,11 +412,12 @@ def linear_distill(x, w, ids, logits, *, temperature: float = 1.0, reduction: st
     length; a token without any entry (or with logits of -inf alone) has loss 0 and takes part
     in no sum.  An entry listed twice counts twice.  An id past the vocabulary makes the
     token's loss NaN.  The temperature is 2^-32 to 2^32; the loss has the rounding of fp32
-    logarithms times its square.  ``x``, ``w``, ``reduction`` and ``keep_logits`` are those of
-    :func:`linear_cross_entropy`."""
+    logarithms times its square.  ``x``, ``w``, ``reduction``, ``keep_logits`` and ``precise_grad`` are
+    those of :func:`linear_cross_entropy`."""
     import torch
 
-    plan = _planned("linear_distill", x, w, ids, logits, reduction, float(temperature), 0, keep_logits)
+    plan = _planned("linear_distill", x, w, ids, logits, reduction, float(temperature), 0, keep_logits,
+                    precise_grad)
     if logits.requires_grad and torch.is_grad_enabled():
         raise LossError("linear_distill gives the teacher's logits no gradient: detach them")
     if torch.autograd.forward_ad._current_level >= 0 and torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
