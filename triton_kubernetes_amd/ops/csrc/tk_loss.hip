@@ -22,16 +22,16 @@
 // that the gradients are off by up to sqrt(2) times that (2048 tokens, 64 entries of a teacher: 1.41).
 // A caller who wants less has dl in two parts (k_logits<TWO>): what its rounding took is rounded to 16
 // bits too and multiplied in its turn, which leaves 2^-16 of dl in bf16, 2^-22 in fp16 (errors 1.000
-// times; 4096 x 4096 x 32768 5.3 ms for 3.5, 8192 x 4096 x 131072 41.8 for 26.7).
+// times; 4096 x 4096 x 32768 5.1 ms for 3.3, 8192 x 4096 x 131072 40.9 for 26.1).
 // In one part, most of a row's derivative is at its target, though, and few numbers' roundings do not average
 // out: up to FEW_ROWS packed rows, what the largest ones lose (`lost`, RESIDUALS a row) is added
 // to dX and dW in fp32.  (48 tokens, bf16: error 1.0 instead of 1.25 times that of rounding the
 // exact gradients; one token alone can have twice as much.  For 4096 tokens it would be 1.0
 // instead of 1.18 times, and cost k_dw a tenth.)
 //
-// Measured at bf16, 8192 tokens x 4096 x 131072: k_logits 6.5 ms, 1.35 PF (matrix pipe busy 67 % of
-// the time, at 1.9 GHz), k_dx 6.65 ms and k_dw 6.8 ms, 1.32 and 1.30 PF, k_dl 0.72 ms, 5.9 TB/s; the
-// rest 0.17 ms.  The products are bound by the matrix pipe and LDS together, about 2050 cycles of
+// Measured at bf16, 8192 tokens x 4096 x 131072: k_logits 6.25 ms forward and 6.55 backward, 1.41 and
+// 1.34 PF (matrix pipe busy 69 and 64 % of the time, at 1.9 GHz), k_dx 6.7 ms and k_dw 6.7 ms, 1.31 PF; the rest
+// 0.14 ms.  With the logits kept k_logits 6.5 ms and k_dl 0.72 ms, 5.9 TB/s, instead.  The products are bound by the matrix pipe and LDS together, about 2050 cycles of
 // each in a step of 64 that takes 2800 to 3100.
 //
 // Rows without a target (masked tokens) are left out before any product: k_gather packs the

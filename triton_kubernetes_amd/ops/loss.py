@@ -74,7 +74,7 @@ def _up(n: int, to: int) -> int:
 def pieces(n: int, v: int) -> int:
     """Vocabulary entries of a piece of the backward pass: as many as keep the derivative of
     ``n`` tokens' logits near ``DL_BYTES``, at most half as much again (a second piece for a little
-    more costs 2 %: 5000 x 2048 x 60000 in one 3262 us, in two 3327), spread evenly, in whole tiles."""
+    more costs 2 %: 5000 x 2048 x 60000 in one 4004 us, in two 4077), spread evenly, in whole tiles."""
     count = max(1, min((4 * n * v // DL_BYTES + 1) // 2, -(-v // TILE)))
     # (of a great many tokens a whole tile more can be past that)
     return min(_up(-(-v // count), TILE), max(TILE, 3 * DL_BYTES // (4 * n) // TILE * TILE))
@@ -85,10 +85,10 @@ def small_products(n: int, d: int, v: int) -> int:
 
     A large tile multiplies faster, a small one wastes less on few tokens and fills more
     compute units.  Measured gain of a small tile over a large one, in us of a whole step at
-    bf16 (n x d x v), where the rules turn: logits, 128 x 4096 x 32000 12 of 298, 192 -7, 256 -23;
-    4096 x 512 x 1000 10 of 87, 8192 2.  x's gradient, 64 x 4096 x 32000 9, 128 1, 192 -19, 128 x
-    4096 x 131072 -77; 2048 x 1024 x 4000 10, 512 x 1024 x 32000 0, 4096 x 512 x 8000 -7.  w's, 1024 x
-    512 x 8000 (64 large tiles) 11, 1024 x 1024 x 6000 (96) 3, 4096 x 1024 x 8000 (128) -13."""
+    bf16 (n x d x v), where the rules turn: logits, 128 x 4096 x 32000 35 of 388, 192 -11, 256 -41;
+    4096 x 512 x 1000 18 of 98, 8192 3.  x's gradient, 64 x 4096 x 32000 9, 128 6, 192 -12, 128 x
+    4096 x 131072 -58; 2048 x 1024 x 4000 8, 512 x 1024 x 32000 -1, 4096 x 512 x 8000 -3.  w's, 1024 x
+    512 x 8000 (64 large tiles) 14, 1024 x 1024 x 6000 (96) 5, 4096 x 1024 x 8000 (128) -11."""
 
     def tiles(a, b):
         return -(-a // TILE) * -(-b // TILE)
@@ -102,15 +102,15 @@ def keeps(n: int, d: int, v: int) -> bool:
     """Whether a call with ``keep_logits=None`` keeps the logits, in 16 bits, for its backward pass:
     where that is faster than to compute them again.  A short product is cheaper
     than two passes over its result.  A step at bf16, kept and again, in us: 4096 x 4096 x 32768
-    2740 and 3430, 512 x 32768 561 and 586, 384 530 and 534, 256 478 and 458; few tokens read the
-    weight once less (16 x 4096 x 131072 841 and 1006, 512 x 256 x 32000 105 both)."""
+    2650 and 3330, 4096 x 512 x 32768 598 both, of width 384 540 both, 256 495 and 456; few tokens read
+    the weight once less (16 x 4096 x 131072 807 and 975, 512 x 256 x 32000 100 and 98)."""
     return (d >= 384 or n <= 512) and 2 * n * v <= KEEP_BYTES
 
 
 def fill(small: bool) -> int:
     """Most workgroups for x's gradient, among which the vocabulary is split: 3 rounds of a large
-    tile for each of the 256 compute units (a step of 5000 x 4000 x 32768, 320 tiles: 3906 us with
-    one round, 3517 with 3, 3472 with 5), or one of two small ones."""
+    tile for each of the 256 compute units (a step of 5000 x 4000 x 32768, 320 tiles: 4690 us with
+    one round, 4278 with 3 and with 5), or one of two small ones."""
     return 512 if small else 768
 
 
