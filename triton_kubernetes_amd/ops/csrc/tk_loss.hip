@@ -30,9 +30,10 @@
 // instead of 1.18 times, and cost k_dw a tenth.)
 //
 // Measured at bf16, 8192 tokens x 4096 x 131072: k_logits 6.25 ms forward and 6.55 backward, 1.41 and
-// 1.34 PF (matrix pipe busy 69 and 64 % of the time, at 1.9 GHz), k_dx 6.7 ms and k_dw 6.7 ms, 1.31 PF; the rest
-// 0.14 ms.  With the logits kept k_logits 6.5 ms and k_dl 0.72 ms, 5.9 TB/s, instead.  The products are bound by the matrix pipe and LDS together, about 2050 cycles of
-// each in a step of 64 that takes 2800 to 3100.
+// 1.34 PF (matrix pipe busy 69 and 64 % of the time, at 1.9 GHz), k_dx and k_dw 6.7 ms each, 1.31
+// PF; the rest 0.14 ms.  With the logits kept k_logits 6.5 ms and k_dl 0.72 ms, 5.9 TB/s, instead.
+// The products are bound by the matrix pipe and LDS together, about 2050 cycles of each in a step
+// of 64 that takes 2800 to 3100.
 //
 // Rows without a target (masked tokens) are left out before any product: k_gather packs the
 // others into Xc, so that whatever the masked rows hold (infinities, NaN) reaches nothing and
