@@ -98,3 +98,24 @@ def test_a_precise_gradient_has_two_parts_in_the_memory_of_one():
         precise(48, 512, 1000, True)
     assert loss._lib().tkl_backward(_args(small=8, codes=4096)) == -1
     assert b"kept logits" in loss._lib().tkl_last_error()
+
+
+@pytest.mark.parametrize("n,piece", [(1, 1 << 24), (2, 10_000_128), (30, 8_000_000 // 256 * 256), (64, 8_388_352)])
+def test_rows_too_long_for_large_tiles_are_refused_by_the_c_entry(n, piece):
+    """193 - n rows behind the last one, of 2 ``piece`` bytes each, against 2^31: past that a copy of rows
+    that are not there would read them."""
+    from test_head_ops import _args
+
+    assert (193 - n) * 2 * piece >= 1 << 31 and n * piece < 1 << 29
+    for small in (0, 5, 8):
+        assert loss._lib().tkl_backward(_args(n=n, v=piece, piece=piece, want=1, small=small)) == -1
+        assert b"too long" in loss._lib().tkl_last_error()
+
+
+@pytest.mark.parametrize("v", [4_000_000, 5_000_000, 6_190_000, 6_200_000, 8_000_000, 1 << 24])
+def test_no_rule_asks_for_rows_that_long(v):
+    for n in [*range(1, 130), 192, 193, 256, 300]:
+        for d in (8, 64, 4096):
+            if not loss.small_products(n, d, v) & 2:
+                for piece in (loss.pieces(n, v), min(loss.pieces(n, v), loss.pieces(2 * n, v))):
+                    assert (193 - min(n, 193)) * 2 * piece < 1 << 31

@@ -207,7 +207,7 @@ struct Panel<true, ROWS, THREADS> {
   static constexpr int COPIES = ROWS * 8 / THREADS;
   const char* base;
   unsigned ld, kbytes;  // row stride, valid bytes of a row
-  unsigned bytes;       // from base to the end of the last valid row (at most 256 rows: below 2^31)
+  unsigned bytes;       // from base to the end of the last valid row (at most 256 rows: below 2^30)
   unsigned voff, chunk;
 
   __device__ __forceinline__ Panel(const void* m, long long ldb, int row0, int rows, int k0, int k, int tid) {
@@ -224,7 +224,7 @@ struct Panel<true, ROWS, THREADS> {
     const unsigned k = t * (KT * 2), v = k + chunk < kbytes ? voff : FAR;  // past the row's end: zeros
     auto buffer = [&](int i) {
       const unsigned at = (h * ROWS + i * (THREADS / 8)) * ld + k;
-      return buffer_of(base + at, max((int)bytes - (int)at, 0));
+      return buffer_of(base + at, max((int)(bytes - at), 0));  // (rows past the last one: at most 2^31 behind it)
     };
 #pragma unroll
     for (int i = 0; i < COPIES; i += 2)
@@ -1706,6 +1706,12 @@ extern "C" int tkl_backward(const tkl_args* a) {
       std::min<long long>(a->n, Big::BN) * a->piece >= (1 << 29)) {
     snprintf(g_err, sizeof(g_err), "piece %lld must be a multiple of %d, below 2^29 over 256 tokens; fill %lld 1 to 4096",
              a->piece, Big::BM, a->fill);
+    return -1;
+  }
+  // dX in large tiles: the copies of a tile start at its rows 0, 64, 128 and 192, which are known not to
+  // be there by how far behind the last one they lie, in 32 bits with a sign
+  if ((a->want & 1) && !(a->small & 2) && (193 - std::min<long long>(a->n, 193)) * 2 * a->piece >= (1ll << 31)) {
+    snprintf(g_err, sizeof(g_err), "rows of %lld entries are too long for %lld tokens in large tiles", a->piece, a->n);
     return -1;
   }
   return on_device(a, a->f16 ? backward<true> : backward<false>);
