@@ -277,6 +277,8 @@ def base_node_config(ctx: Context, module_path: str, cluster: str, state: State)
         count = int(str(count_input).strip())
     except ValueError as exc:
         raise ConfigError(f"node_count must be a valid number. Found '{count_input}'.") from exc
+    if count >= 1 << 63:  # past int64 Go's strconv.Atoi has no number either
+        raise ConfigError(f"node_count must be a valid number. Found '{count_input}'.")
     if count <= 0:
         raise ConfigError(f"node_count must be greater than 0. Found '{count}'.")
 
