@@ -12,10 +12,10 @@
 // Nothing is rounded to 16 bits on the way but the result.
 //
 // Measured (device time, weights in turn, so out of HBM): one row, 131072 x 4096 with groups of 64
-// and zeros, 60 us, 4.9 TB/s; 8192 x 8192 11.2 us; 64 rows, 16384 x 16384 58 us and 6 to join.  One row is bound by
-// the reads and the instructions that unpack and scale; many rows by the vector and the matrix
-// instructions, 23 and 14 us, which hardly overlap (42 us without loads, barriers and x's way
-// through LDS, 54 without the loads, 49 with nothing but loads).
+// and zeros, 60 us, 4.9 TB/s; 8192 x 8192 11.2 us; 64 rows, 16384 x 16384 58 us and 6 to join.
+// One row is bound by the reads and the instructions that unpack and scale; many rows by the vector
+// and the matrix instructions, 23 and 14 us, which hardly overlap (42 us without loads, barriers
+// and x's way through LDS, 54 without the loads, 49 with nothing but loads).
 //
 // C ABI for ctypes: triton_kubernetes_amd/ops/gemv.py.
 
