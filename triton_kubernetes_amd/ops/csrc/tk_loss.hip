@@ -12,8 +12,8 @@
 // Cross entropy is K = 1, p = 1, T = 1; distillation takes p from a teacher's top logits.
 //
 // Forward: one matrix product whose epilogue reduces every tile of the vocabulary to a maximum
-// and a sum per token (k_logits<LSE>), a dot product per target, and a join over the tiles
-// (k_loss, which also forms a cross entropy's dot products; k_dots those of a teacher's lists).
+// and a sum per token and leaves a cross entropy's targets' logits (k_logits<LSE>), a dot product
+// per entry of a teacher's lists (k_dots), and a join over the tiles (k_loss).
 // Backward, in pieces of the vocabulary: the logits' 16-bit derivative dl, from the same product
 // again (k_logits<DL>), or from codes that the forward pass kept (k_dl, struct Codes); a
 // teacher's targets are put in by k_fix; then dX += dl W and dW = dl^T X.
@@ -576,6 +576,8 @@ struct Codes {
 // LSE: writes part[tile][token] = (max, sum); KEEP: and the logits' codes to `out`.  DL: writes
 // f (q - p) in 16 bits to `out`, with a cross entropy's p; `targets` is null for a teacher's
 // lists.  TWO: the same, and what that rounding took, in 16 bits, to `low`.  sc = log2(e) / T.
+// `of_target` gets of a cross entropy's targets the logits (LSE, KEEP), out of the accumulators that
+// the sums are made from, or what their derivative's rounding took (DL, TWO).
 enum Mode { LSE, KEEP, DL, TWO };
 template <class Tile, bool F16, Mode MODE>
 __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict__ w, long long ldw,
@@ -584,7 +586,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
                                                           float sc, float2* __restrict__ part,
                                                           const float* __restrict__ lse, Upstream<F16> up,
                                                           const int* __restrict__ targets, void* __restrict__ out,
-                                                          long long ldout, float* __restrict__ lost,
+                                                          long long ldout, float* __restrict__ of_target,
                                                           void* __restrict__ low) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
@@ -605,6 +607,19 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
   const bool whole = (tv + 1) * Tile::BM <= vn;
   const int first = tn * Tile::BN, here = min(Tile::BN, rows - first);
   if constexpr (MODE == LSE || MODE == KEEP) {
+    if (targets) {
+#pragma unroll
+      for (int j = 0; j < Tile::NF; ++j) {
+        const int token = first + Tile::col(j, wid) + fr, target = token < rows ? targets[token] - v0 - vb : -Tile::BM;
+        if ((unsigned)(target + 12) < Tile::BM + 12u) {  // (vb is up to 12 past the tile's start)
+#pragma unroll
+          for (int i = 0; i < Tile::MF; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (Tile::row(i, wid) + e == target) of_target[token] = acc[i][j][e];
+        }
+      }
+    }
     barrier();  // LDS has been read
     float2* sums = reinterpret_cast<float2*>(smem + Outgoing<Tile, T>::BYTES);  // [WAVES_M][BN]
 #pragma unroll
@@ -676,7 +691,7 @@ __global__ __launch_bounds__(Tile::THREADS) void k_logits(const void* __restrict
           for (int e = 0; e < 4; ++e)
             if (at + e == target) {
               g[e] -= f;
-              lost[token] = g[e] - (float)(T)g[e];
+              of_target[token] = g[e] - (float)(T)g[e];
             }
         }
         if (!whole) {
@@ -1023,7 +1038,8 @@ __global__ __launch_bounds__(256) void k_teacher(const long long* __restrict__ i
   if (lane == 0) flag[row] = any;
 }
 
-// Packs the rows that have a loss into xc [rows][dp] (zeros behind d).  A wave takes `per` rows, and
+// Packs the rows that have a loss into xc [rows][dp] (zeros behind d), and of a cross entropy the
+// targets (`at`; one outside the vocabulary is -1, and its logit in `zk` NaN).  A wave takes `per` rows, and
 // its block counts the kept rows before them itself, which needs no second launch for a scan
 // (8192 tokens: 1024 blocks read at most 64 KiB of targets each, out of L2).
 constexpr int MOST_PER = 32;
@@ -1033,7 +1049,8 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
                                                 const long long* __restrict__ target, long long ignore,
                                                 const int* __restrict__ flag, T* __restrict__ xc,
                                                 int* __restrict__ rowmap, int* __restrict__ posof,
-                                                int* __restrict__ count, float* __restrict__ loss, int per) {
+                                                int* __restrict__ count, float* __restrict__ loss, int per,
+                                                long long v, int* __restrict__ at, float* __restrict__ zk) {
   __shared__ int total[4], kept[4 * MOST_PER];
   const int row0 = blockIdx.x * 4 * per, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c = 0;
@@ -1082,6 +1099,11 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x, long lo
     if (lane == 0) {
       rowmap[pos] = r;
       posof[r] = pos;
+      if (!flag) {
+        const bool there = target[r] >= 0 && target[r] < v;
+        at[pos] = there ? (int)target[r] : -1;
+        if (!there) zk[pos] = NAN;
+      }
     }
     ++pos;
   }
@@ -1111,123 +1133,101 @@ __global__ __launch_bounds__(256) void k_pad(const T* __restrict__ w, long long 
   }
 }
 
-// x . w[id] over `lanes` neighbouring lanes, the sum in all of them.  A target outside the
-// vocabulary gives NaN.
-template <typename T>
-__device__ __forceinline__ float dot(const T* x, const T* w, long long ldw, int dk, long long id, long long v, int lane,
-                                     int lanes) {
-  if (id < 0 || id >= v) return NAN;
-  const T* b = w + id * ldw;
-  float s = 0.f;
-#pragma unroll 4
-  for (int e = lane * 8; e < dk; e += lanes * 8) {
-    typedef __attribute__((ext_vector_type(8))) T t8;
-    const t8 p = *reinterpret_cast<const t8*>(x + e), q = *reinterpret_cast<const t8*>(b + e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += (float)p[i] * (float)q[i];
-  }
-  for (int o = lanes / 2; o; o >>= 1) s += __shfl_xor(s, o, 64);
-  return s;
-}
-
-// A teacher's lists: zk[pos][j] = x . w[id], one wave for 4 entries of a token, which share its x
-// (2048 tokens x 64 entries of 2048: 92 us one by one, 82 so, 6.5 TB/s).  An id below 0 is no entry.
-template <typename T>
-__global__ __launch_bounds__(256) void k_dots(const T* __restrict__ xc, int dp, const T* __restrict__ w,
+// A teacher's lists: zk[pos][j] = x . w[id], one wave for 16 entries of a token.  By matrix instructions
+// in the order of k_logits' steps, so that each is that kernel's logit to the bit: a loss is a
+// difference of the two (a student that is sure of the same entry as its teacher had 4 times the
+// plain form's error with sums of their own order).  An id below 0 is no entry.
+template <bool F16>
+__global__ __launch_bounds__(256) void k_dots(const void* __restrict__ xc, int dp, const void* __restrict__ w,
                                               long long ldw, int dk, const long long* __restrict__ ids, int k,
                                               long long v, const int* __restrict__ rowmap,
                                               const int* __restrict__ count, float* __restrict__ zk) {
-  constexpr int SHARE = 4;
-  typedef __attribute__((ext_vector_type(8))) T t8;
-  const int per_row = (k + SHARE - 1) / SHARE, lane = threadIdx.x & 63;
+  using T = typename Type<F16>::T;
+  constexpr int SHARE = 16, AHEAD = 8;
+  const int per_row = (k + SHARE - 1) / SHARE, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const long long items = (long long)count[0] * per_row;
   for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < items; i += (long long)gridDim.x * 4) {
     const int pos = (int)(i / per_row), j = (int)(i - (long long)pos * per_row) * SHARE;
     const long long* row = ids + (size_t)rowmap[pos] * k;
-    long long id[SHARE];
-    const T* from[SHARE];
-    float s[SHARE] = {};
+    const long long id = j + r < k ? row[j + r] : -1;
+    const bool there = id >= 0 && id < v;
+    const T* from = static_cast<const T*>(w) + (there ? id : 0) * ldw + q * 8;
+    const T* x = static_cast<const T*>(xc) + (size_t)pos * dp + q * 8;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < dk; e += 32 * AHEAD) {
+      u32x4 a[AHEAD], b[AHEAD];
 #pragma unroll
-    for (int o = 0; o < SHARE; ++o) {
-      id[o] = j + o < k ? row[j + o] : -1;
-      from[o] = w + (id[o] >= 0 && id[o] < v ? id[o] : 0) * ldw;
+      for (int o = 0; o < AHEAD; ++o) {
+        const bool in = e + o * 32 + q * 8 < dk;
+        a[o] = in && there ? *reinterpret_cast<const u32x4*>(from + e + o * 32) : u32x4{0, 0, 0, 0};
+        b[o] = in ? *reinterpret_cast<const u32x4*>(x + e + o * 32) : u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int o = 0; o < AHEAD; ++o) acc = Type<F16>::mfma(a[o], b[o], acc);
     }
-    const T* x = xc + (size_t)pos * dp;
-#pragma unroll 2
-    for (int e = lane * 8; e < dk; e += 512) {
-      const t8 p = *reinterpret_cast<const t8*>(x + e);
-      t8 q[SHARE];
-#pragma unroll
-      for (int o = 0; o < SHARE; ++o) q[o] = *reinterpret_cast<const t8*>(from[o] + e);
-#pragma unroll
-      for (int o = 0; o < SHARE; ++o)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) s[o] += (float)p[c] * (float)q[o][c];
-    }
-#pragma unroll
-    for (int o = 0; o < SHARE; ++o) {
-      s[o] = wave_sum(s[o]);
-      if (lane == 0 && j + o < k) zk[(size_t)pos * k + j + o] = id[o] < 0 ? 0.f : id[o] < v ? s[o] : NAN;
+    // every column has the 16 sums, 4 to a lane: column c of 4 writes its lanes' c-th
+    const int own = j + q * 4 + r;
+    if (r < 4 && own < k) {
+      const float z = r == 0 ? acc[0] : r == 1 ? acc[1] : r == 2 ? acc[2] : acc[3];
+      const long long of = row[own];
+      zk[(size_t)pos * k + own] = of < 0 ? 0.f : of < v ? z : NAN;
     }
   }
 }
 
-// Joins the tiles' (max, sum) of 8 rows, 32 threads a row, and forms the rows' losses; of a cross
-// entropy (p null) also the targets' logits.  lse is kept in the exponent's base 2.  With a
-// reduction the block that ends last adds the rows' losses, always in the same order (`done` not
+// Joins the tiles' (max, sum) of 8 rows, 32 threads a row, and forms the rows' losses.  lse is kept in the
+// exponent's base 2, but the losses take the targets' distance from the row's maximum m, exact but for
+// one rounding, where a difference of lse and logit would have theirs:
+//
+//     log q = ln 2 ((z sc - m) - log2 sum_v exp2(z_v sc - m))
+//
+// With a reduction the block that ends last adds the rows' losses, always in the same order (`done` not
 // null; the release that this takes of every block costs 60 us of 1024 blocks, so many rows have
 // k_reduce).  A batch without any loss has 0.
-template <typename T>
 __global__ __launch_bounds__(256) void k_loss(const float2* __restrict__ part, int parts, int n,
-                                              const T* __restrict__ xc, int dp, const T* __restrict__ w, long long ldw,
-                                              int dk, const long long* __restrict__ ids, long long v,
-                                              float* __restrict__ zk, const float* __restrict__ p, int k,
+                                              const float* __restrict__ zk, const float* __restrict__ p, int k,
                                               const int* __restrict__ rowmap, const int* __restrict__ count, float sc,
                                               float t2, float* __restrict__ lse, float* __restrict__ rowloss,
-                                              float* __restrict__ loss, int reduction, int* __restrict__ at_out,
-                                              int* __restrict__ done) {
-  __shared__ float sm[32][8], ss[32][8], sd[32][8], sz[8];
+                                              float* __restrict__ loss, int reduction, int* __restrict__ done) {
+  __shared__ float sm[32][8], ss[32][8], sd[32][8];
   const int r = threadIdx.x & 7, slice = threadIdx.x >> 3, pos = blockIdx.x * 8 + r, rows = count[0];
-  if (!p) {
-    const int own = threadIdx.x >> 5, at = blockIdx.x * 8 + own;
-    if (at < rows) {
-      const long long id = ids[rowmap[at]];
-      const float z = dot(xc + (size_t)at * dp, w, ldw, dk, id, v, threadIdx.x & 31, 32);
-      if ((threadIdx.x & 31) == 0) {
-        sz[own] = zk[at] = z;
-        at_out[at] = id >= 0 && id < v ? (int)id : -1;
-      }
-    }
-  }
-  float m = -INFINITY, s = 0.f, dot = 0.f;
+  float m = -INFINITY, s = 0.f;
   if (pos < rows) {
 #pragma unroll 4
     for (int i = slice; i < parts; i += 32) {
       const float2 c = part[(size_t)i * n + pos];
       merge(m, s, c.x, c.y);
     }
-    // sum_k p (ln p - ln 2 (z sc - lse)) = sum_k p (ln p - ln 2 z sc) + ln 2 lse
-    if (p) {
-      const size_t row = (size_t)rowmap[pos] * k;
-      for (int i = slice; i < k; i += 32) {
-        const float q = p[row + i], z = zk[(size_t)pos * k + i];
-        if (q > 0.f) dot += q * (logf(q) - LN2 * sc * z);
-        else if (q != q || z != z) dot = NAN;
-      }
-    }
   }
   sm[slice][r] = m;
   ss[slice][r] = s;
-  sd[slice][r] = dot;
   __syncthreads();
-  if (threadIdx.x < 8 && pos < rows) {
-    for (int i = 1; i < 32; ++i) {
-      merge(m, s, sm[i][r], ss[i][r]);
-      dot += sd[i][r];
+  m = sm[0][r];
+  s = ss[0][r];
+  for (int i = 1; i < 32; ++i) merge(m, s, sm[i][r], ss[i][r]);  // every thread of a row, in the same order
+  const float log_s = log2f(s);
+  if (p) {
+    float sum = 0.f;
+    if (pos < rows) {
+      const size_t row = (size_t)rowmap[pos] * k;
+      for (int i = slice; i < k; i += 32) {
+        const float q = p[row + i], z = zk[(size_t)pos * k + i];
+        if (q > 0.f) sum += q * (logf(q) - LN2 * (__builtin_fmaf(z, sc, -m) - log_s));
+        else if (q != q || z != z) sum = NAN;
+      }
     }
-    if (!p) dot = -LN2 * sc * sz[r];
-    const float l = m + log2f(s), out = t2 * (dot + LN2 * l);
-    lse[pos] = l;
+    sd[slice][r] = sum;
+    __syncthreads();
+  }
+  if (threadIdx.x < 8 && pos < rows) {
+    float sum = 0.f;
+    if (p) {
+      for (int i = 0; i < 32; ++i) sum += sd[i][r];
+    } else {
+      sum = LN2 * (log_s - __builtin_fmaf(zk[pos], sc, -m));
+    }
+    const float out = t2 * sum;
+    lse[pos] = m + log_s;
     __hip_atomic_store(rowloss + pos, out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!reduction) loss[rowmap[pos]] = out;
   }
@@ -1552,16 +1552,16 @@ float2* part_of(const tkl_args& a) {
 
 template <class Tile, bool F16, Mode MODE>
 void logits_as(const tkl_args& a, const Kept& kept, const Weight& w, int dp, long long v0, int vn, const Upstream<F16>& up,
-               void* out, long long ldout, float* lost, void* low, hipStream_t s) {
+               void* out, long long ldout, float* of_target, void* low, hipStream_t s) {
   k_logits<Tile, F16, MODE><<<blocks(vn, Tile::BM) * blocks(a.n, Tile::BN), Tile::THREADS, Tile::LDS, s>>>(
       w.at, w.ldb, kept.xc, (long long)dp * 2, (int)v0, (int)v0 + vn, w.dk, kept.count, (int)a.n, LOG2E / a.temperature,
-      part_of(a), kept.lse, up, a.distill ? nullptr : kept.at, out, ldout, lost, low);
+      part_of(a), kept.lse, up, a.distill ? nullptr : kept.at, out, ldout, of_target, low);
 }
 
 template <class Tile, bool F16>
 void all_logits(const tkl_args& a, const Kept& q, const Weight& w, int dp, hipStream_t s) {
-  if (a.codes) logits_as<Tile, F16, KEEP>(a, q, w, dp, 0, (int)a.v, {}, a.codes, Codes::stride(a.v), nullptr, nullptr, s);
-  else logits_as<Tile, F16, LSE>(a, q, w, dp, 0, (int)a.v, {}, nullptr, 0, nullptr, nullptr, s);
+  if (a.codes) logits_as<Tile, F16, KEEP>(a, q, w, dp, 0, (int)a.v, {}, a.codes, Codes::stride(a.v), q.zk, nullptr, s);
+  else logits_as<Tile, F16, LSE>(a, q, w, dp, 0, (int)a.v, {}, nullptr, 0, q.zk, nullptr, s);
 }
 
 // dl of a piece, out of the kept logits or by computing them again
@@ -1591,19 +1591,18 @@ hipError_t forward(const tkl_args& a) {
     k_teacher<<<blocks(n, 4), 256, 0, s>>>(ids, static_cast<const float*>(a.teacher), n, k, 1.f / t, q.p, q.flag);
   const int per = gather_rows(n);
   k_gather<T><<<blocks(n, 4 * per), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, dp, ids, a.ignore, q.flag, xc,
-                                                 q.rowmap, q.posof, q.count, a.reduction ? nullptr : loss, per);
+                                                 q.rowmap, q.posof, q.count, a.reduction ? nullptr : loss, per, a.v, q.at,
+                                                 q.zk);
   pad<T>(a, dp, s);
   const Weight w = weight_of(a, dp);
-  const T* wt = static_cast<const T*>(w.at);
   if (a.small & 1) all_logits<Small, F16>(a, q, w, dp, s);
   else all_logits<Big, F16>(a, q, w, dp, s);
   if (a.distill)
-    k_dots<T><<<(unsigned)std::min<long long>((n * ((k + 3ll) / 4) + 3) / 4, 1 << 22), 256, 0, s>>>(
-        xc, dp, wt, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count, q.zk);
-  k_loss<T><<<blocks(n, 8), 256, 0, s>>>(part_of(a),
-                                         (int)blocks(a.v, a.small & 1 ? Small::BM : Big::BM), n, xc, dp, wt, w.ldb / 2,
-                                         w.dk, ids, a.v, q.zk, q.p, k, q.rowmap, q.count, LOG2E / t, t * t, q.lse,
-                                         q.rowloss, loss, a.reduction, q.at, a.reduction && n <= 512 ? q.count + 1 : nullptr);
+    k_dots<F16><<<(unsigned)std::min<long long>((n * ((k + 15ll) / 16) + 3) / 4, 1 << 22), 256, 0, s>>>(
+        xc, dp, w.at, w.ldb / 2, w.dk, ids, k, a.v, q.rowmap, q.count, q.zk);
+  k_loss<<<blocks(n, 8), 256, 0, s>>>(part_of(a), (int)blocks(a.v, a.small & 1 ? Small::BM : Big::BM), n, q.zk, q.p, k,
+                                      q.rowmap, q.count, LOG2E / t, t * t, q.lse, q.rowloss, loss, a.reduction,
+                                      a.reduction && n <= 512 ? q.count + 1 : nullptr);
   if (a.reduction && n > 512) k_reduce<<<1, 1024, 0, s>>>(q.rowloss, q.count, a.reduction, loss);
   return hipGetLastError();
 }
