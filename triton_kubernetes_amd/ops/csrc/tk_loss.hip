@@ -1378,7 +1378,7 @@ __global__ __launch_bounds__(256) void k_dx_out(const float* __restrict__ part, 
       for (int o = 0; o < 8; ++o) s += v[o];
     }
     for (; i < splits; ++i) s += *reinterpret_cast<const f32x4*>(from + (size_t)i * rows * dp);
-    for (int r = 0; rows <= FEW_ROWS && r < residuals; ++r) {
+    for (int r = 0; r < residuals; ++r) {
       const int id = at[pos * residuals + r];
       if (id < 0) break;
       const t4 v = *reinterpret_cast<const t4*>(static_cast<const T*>(w) + id * ldw + c);
