@@ -18,16 +18,17 @@
 // again (k_logits<DL>), or from codes that the forward pass kept (k_dl, struct Codes); a
 // teacher's targets are put in by k_fix; then dX += dl W and dW = dl^T X.
 //
-// dl is rounded to 16 bits, which costs each product about as much as the rounding of its result, so
-// that the gradients are off by up to sqrt(2) times that (2048 tokens, 64 entries of a teacher: 1.41).
-// A caller who wants less has dl in two parts (k_logits<TWO>): what its rounding took is rounded to 16
-// bits too and multiplied in its turn, which leaves 2^-16 of dl in bf16, 2^-22 in fp16 (errors 1.000
-// times; 4096 x 4096 x 32768 5.1 ms for 3.3, 8192 x 4096 x 131072 40.9 for 26.1).
-// In one part, most of a row's derivative is at its target, though, and few numbers' roundings do not average
-// out: up to FEW_ROWS packed rows, what the largest ones lose (`lost`, RESIDUALS a row) is added
-// to dX and dW in fp32.  (48 tokens, bf16: error 1.0 instead of 1.25 times that of rounding the
-// exact gradients; one token alone can have twice as much.  For 4096 tokens it would be 1.0
-// instead of 1.18 times, and cost k_dw a tenth.)
+// dl is rounded to 16 bits, which costs each product about as much as the rounding of its result.
+// Most of a row's derivative is at its targets, though, and one number's rounding does not average
+// out: it is common to the row's whole part of a gradient, up to 1.57 times what rounding the result
+// once costs, all told.  So what the targets lose (`lost`: of a cross entropy each, of a teacher's list
+// RESIDUALS a row) is given back, to dX in fp32 (k_dx_out), to dW as steps more of its product (k_dw;
+// k_list finds each tile's).  Errors, as multiples of rounding the exact gradients once: a cross
+// entropy 1.00 (1.18 without, 4096 tokens), 64 entries of a teacher 1.16 (1.41), at most 1.35 seen.
+// It costs a step 1 % (4096 x 4096 x 32768), where many tokens meet a small vocabulary up to 12 %
+// (8192 x 512 x 1000).  A caller who wants less error has dl in two parts (k_logits<TWO>): what its
+// rounding took is rounded to 16 bits too and multiplied in its turn, which leaves 2^-16 of dl in
+// bf16, 2^-22 in fp16 (errors 1.000; 4096 x 4096 x 32768 1.55 times as long).
 //
 // Measured at bf16, 8192 tokens x 4096 x 131072: k_logits 6.25 ms forward and 6.55 backward, 1.41 and
 // 1.34 PF (matrix pipe busy 69 and 64 % of the time, at 1.9 GHz), k_dx and k_dw 6.7 ms each, 1.31
@@ -92,7 +93,7 @@ constexpr int KT = 64;  // K elements of a step (128 bytes of a row)
 constexpr int MAX_TARGETS = 1024;
 constexpr int RESIDUALS = 4;  // entries of a teacher's list whose rounding is made good; 1 of a cross entropy
 constexpr float LARGE = 0.125f;  // |q - p| from which it is: at most 16 of a row
-constexpr int FEW_ROWS = 512;
+constexpr int FEW_ROWS = 512;  // up to which each tile of dW looks for its targets among all (a launch less)
 
 // The two tilings of the matrix products.  A fragment is 16 x 16; a lane of a wave holds rows
 // row(mf) + (lane / 16) * 4 + 0..3 and column col(nf) + lane % 16 of fragment (mf, nf).
@@ -104,7 +105,6 @@ struct Big {  // 8 waves, the schedule of product_big
   static __device__ __forceinline__ int wave_m(int wid) { return wid >> 2; }
   static __device__ __forceinline__ int row(int mf, int wid) { return (mf >> 2) * 128 + (wid >> 2) * 64 + (mf & 3) * 16; }
   static __device__ __forceinline__ int col(int nf, int wid) { return (nf >> 1) * 128 + (wid & 3) * 32 + (nf & 1) * 16; }
-  static __device__ __forceinline__ bool owns(int col, int wid) { return (col >> 5 & 3) == (wid & 3); }
 };
 struct Small {  // 4 waves, STEPS steps in LDS, two workgroups to a compute unit: for few tokens
   static constexpr int BM = 128, BN = 64, THREADS = 256, MF = 2, NF = 4, WAVES_M = 4, STEPS = 3,
@@ -114,7 +114,6 @@ struct Small {  // 4 waves, STEPS steps in LDS, two workgroups to a compute unit
   static __device__ __forceinline__ int wave_m(int wid) { return wid; }
   static __device__ __forceinline__ int row(int mf, int wid) { return wid * 32 + mf * 16; }
   static __device__ __forceinline__ int col(int nf, int) { return nf * 16; }
-  static __device__ __forceinline__ bool owns(int, int) { return true; }
 };
 
 constexpr unsigned FAR = 0x40000000u;  // an offset past every descriptor's end: the copy writes zeros
@@ -851,6 +850,53 @@ __global__ __launch_bounds__(256) void k_transpose(const T* __restrict__ xc, int
   }
 }
 
+// The entries (of all packed rows' `at`) whose vocabulary entry is in the piece, by BUCKET entries of it:
+// those of bucket b are listed[starts[b] .. starts[b + 1]), in order.  A block finds those of its
+// bucket, and how many are in the buckets before it, by looking at all.
+constexpr int BUCKET = 256;
+__global__ __launch_bounds__(1024) void k_list(const int* __restrict__ at, int residuals, const int* __restrict__ count,
+                                               int v0, int vn, int* __restrict__ listed, int* __restrict__ starts) {
+  __shared__ int before[16], found[16];
+  const int rows = count[0];
+  if (rows <= FEW_ROWS) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, entries = rows * residuals;
+  const int lo = v0 + blockIdx.x * BUCKET, hi = min(lo + BUCKET, v0 + vn);
+  const int per = (entries + 1023) / 1024, i0 = min(entries, tid * per), i1 = min(entries, i0 + per);
+  int below = 0, mine = 0;
+#pragma unroll 8
+  for (int i = i0; i < i1; ++i) {
+    const int t = at[i];
+    below += t >= v0 && t < lo;
+    mine += t >= lo && t < hi;
+  }
+  int upto = mine;  // of this wave's lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int other = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += other;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) below += __shfl_xor(below, o, 64);
+  if (lane == 63) found[wave] = upto;
+  if (lane == 0) before[wave] = below;
+  __syncthreads();
+  int start = 0, to = upto - mine, total = 0;
+  for (int o = 0; o < 16; ++o) {
+    start += before[o];
+    if (o < wave) to += found[o];
+    total += found[o];
+  }
+  if (tid == 0) {
+    starts[blockIdx.x] = start;
+    if (blockIdx.x == gridDim.x - 1) starts[blockIdx.x + 1] = start + total;
+  }
+  if (!mine) return;
+  for (int i = i0; i < i1; ++i) {
+    const int t = at[i];
+    if (t >= lo && t < hi) listed[start + to++] = i;
+  }
+}
+
 // dW^T tile: A = Xc^T (K = tokens along the rows), B = dl (K = tokens, down the rows).  (With A down
 // the rows of Xc its fragments have to be transposed on their way out of LDS too, which takes twice
 // the time of a plain read: 1950 us for 1724 at 8192 x 4096 x 32768.  Small tiles do that, and save a
@@ -863,7 +909,8 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
                                                       long long lddl, int v0, int vn, int d, const int* __restrict__ count, Upstream<F16> up,
                                                       const int* __restrict__ at, const float* __restrict__ lost,
                                                       int residuals, void* __restrict__ dw, int lddw,
-                                                      float* __restrict__ sums, const void* __restrict__ low) {
+                                                      float* __restrict__ sums, const void* __restrict__ low,
+                                                      const int* __restrict__ listed, const int* __restrict__ starts) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using T = typename Type<F16>::T;
   const int rows = count[0], per = ((rows + KT - 1) / KT + gridDim.y - 1) / gridDim.y * KT;
@@ -887,68 +934,85 @@ __global__ __launch_bounds__(Tile::THREADS) void k_dw(const void* __restrict__ x
       multiply<Tile, F16, false, false, false, true>(acc, smem, pa, of_low(), (k + KT - 1) / KT, tid);
   }
 
-  // What dl's rounding took from the targets among this tile's rows.  Each wave lists those in its
-  // share of the packed rows, in order; beyond ROOM of them the rounding stays, as it does past
-  // FEW_ROWS.  Their rows of Xc come through LDS, 64 at a time.
-  if (!TWICE && rows <= FEW_ROWS && blockIdx.y == 0) {
-    constexpr int WAVES = Tile::THREADS / 64, ROOM = 32, PER = Tile::BM / 8;
-    struct Hit {
-      int pos, col;
-      float lost;
-    };
-    Hit* list = reinterpret_cast<Hit*>(smem);  // [WAVES][ROOM]
-    Hit* all = list + WAVES * ROOM;
-    int* lengths = reinterpret_cast<int*>(all + WAVES * ROOM);
-    u32x4* xrows = reinterpret_cast<u32x4*>(smem + 16384);  // [64][PER]
-    static_assert(2 * WAVES * ROOM * sizeof(Hit) + WAVES * 4 <= 16384, "the lists fit");
+  // What dl's rounding took from the targets among this tile's rows: a window of entries at a time, of all
+  // of them where they are few, else of those that k_list found for these 256 rows.  The hits of a window
+  // are put together in order; 64 of them are a step more of the product, of their rows of Xc with a
+  // matrix that has each one's rest at its column.  (By vector instructions, a hit at a time, 8192 x 4096 x
+  // 1536 with 1400 hits a tile took 770 us instead of 550 without any of this.)
+  if constexpr (!TWICE) {
+    constexpr int WAVES = Tile::THREADS / 64, PER = Tile::BM / 8;
+    using Image = Panel<false, 128, Tile::THREADS>;  // of the hits' rows of Xc, 128 columns each
+    int* hit_pos = reinterpret_cast<int*>(smem);  // [THREADS]
+    int* hit_col = hit_pos + Tile::THREADS;
+    float* hit_lost = reinterpret_cast<float*>(hit_col + Tile::THREADS);
+    int* lengths = reinterpret_cast<int*>(hit_lost + Tile::THREADS);
+    char* images = smem + 16384;
+    static_assert(3 * Tile::THREADS * 4 + WAVES * 4 <= 16384, "the hits fit");
     static_assert(16384 + 64 * PER * 16 <= Tile::LDS, "the rows fit");
-    __syncthreads();  // LDS has been read
-    const int entries = rows * residuals, share = (entries + Tile::THREADS - 1) / Tile::THREADS * 64;
-    const int end = min(entries, (wid + 1) * share);
+    const bool few = rows <= FEW_ROWS;
+    const int bucket = tv * Tile::BN / BUCKET, start = few ? 0 : starts[bucket];
+    const int entries = few ? rows * residuals : starts[bucket + 1] - start;
+    const int share = (entries + (int)gridDim.y - 1) / (int)gridDim.y, end = min(entries, ((int)blockIdx.y + 1) * share);
     const int first = v0 + tv * Tile::BN, width = min(Tile::BN, vn - tv * Tile::BN);
-    int found = 0;
-    for (int i = wid * share; i < end && found < ROOM; i += 64) {
-      const int e = i + lane, v = e < end ? at[e] - first : -1;
+    for (int i0 = blockIdx.y * share; i0 < end; i0 += Tile::THREADS) {
+      const int i = i0 + tid, e = i >= end ? -1 : few ? i : listed[start + i], v = e < 0 ? -1 : at[e] - first;
       const bool here = v >= 0 && v < width;
       const unsigned long long mask = __ballot(here);
-      const int slot = found + __popcll(mask & ((1ull << lane) - 1));
-      if (here && slot < ROOM) list[wid * ROOM + slot] = Hit{e / residuals, v, lost[e]};
-      found = min(ROOM, found + __popcll(mask));
-    }
-    if (lane == 0) lengths[wid] = found;
-    __syncthreads();
-    int total = 0;
-    for (int o = 0; o < WAVES; ++o) {
-      if (tid < lengths[o]) all[total + tid] = list[o * ROOM + tid];
-      total += lengths[o];
-    }
-    __syncthreads();
-    for (int b = 0; b < total; b += 64) {
-      const int here = min(64, total - b);
-      if (b) __syncthreads();
-      for (int i = tid; i < here * PER; i += Tile::THREADS) {
-        const int c = td * Tile::BM + i % PER * 8;
-        xrows[i] = c < dp ? *reinterpret_cast<const u32x4*>(static_cast<const T*>(xc) + (size_t)all[b + i / PER].pos * dp + c)
-                          : u32x4{0, 0, 0, 0};
-      }
+      __syncthreads();  // LDS has been read
+      if (lane == 0) lengths[wid] = __popcll(mask);
       __syncthreads();
-      const Hit own = lane < here ? all[b + lane] : Hit{0, 0, 0.f};
-      for (int i = 0; i < here; ++i) {
-        const int col = __builtin_amdgcn_readlane(own.col, i);
-        if (!Tile::owns(col, __builtin_amdgcn_readfirstlane(wid))) continue;
-        const float l = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own.lost), i));
-        typedef __attribute__((ext_vector_type(4))) T t4;
-        const t4* x = reinterpret_cast<const t4*>(xrows + i * PER);
+      int slot = __popcll(mask & ((1ull << lane) - 1)), total = 0;
+      for (int o = 0; o < WAVES; ++o) {
+        if (o < wid) slot += lengths[o];
+        total += lengths[o];
+      }
+      if (here) {
+        hit_pos[slot] = e / residuals;
+        hit_col[slot] = v;
+        hit_lost[slot] = lost[e];
+      }
+      if (tid >= total) hit_col[tid] = -1;  // none
+      __syncthreads();
+      for (int b = 0; b < total; b += 64) {
+        if (b) __syncthreads();
+        for (int x = tid; x < 64 * PER; x += Tile::THREADS) {
+          const int k = x / PER, c = x % PER, unit = c & 15;
+          u32x4 v8 = {0, 0, 0, 0};
+          if (b + k < total && td * Tile::BM + c * 8 < dp)
+            v8 = *reinterpret_cast<const u32x4*>(static_cast<const T*>(xc) + (size_t)hit_pos[b + k] * dp + td * Tile::BM + c * 8);
+          *reinterpret_cast<u32x4*>(images + (c >> 4) * 64 * Image::STRIDE + k * Image::STRIDE +
+                                    ((((unit >> 1) ^ Image::f(k)) << 1) | (unit & 1)) * 16) = v8;
+        }
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < Tile::NF; ++j)
-          if (Tile::col(j, wid) + (lane & 15) == col) {
+        for (int kk = 0; kk < 2; ++kk) {
+          u32x4 x[Tile::MF];
 #pragma unroll
-            for (int m = 0; m < Tile::MF; ++m) {
-              const t4 v4 = x[(Tile::row(m, wid) + (lane >> 4) * 4) / 4];
+          for (int m = 0; m < Tile::MF; ++m)
+            x[m] = Image::frag(images + (Tile::row(m, wid) >> 7) * 64 * Image::STRIDE, Tile::row(m, wid) & 127, kk, lane);
+          int cols[8];
+          float rest[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[m][j][e] += l * (float)v4[e];
-            }
+          for (int o = 0; o < 8; ++o) {
+            cols[o] = hit_col[b + kk * 32 + (lane >> 4) * 8 + o];
+            rest[o] = hit_lost[b + kk * 32 + (lane >> 4) * 8 + o];
           }
+#pragma unroll
+          for (int j = 0; j < Tile::NF; ++j) {
+            const int own = Tile::col(j, wid) + (lane & 15);
+            bool any = false;
+            u32x4 r;
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+              const bool p = cols[2 * o] == own, q = cols[2 * o + 1] == own;
+              any |= p || q;
+              r[o] = pack2<T>(p ? rest[2 * o] : 0.f, q ? rest[2 * o + 1] : 0.f);
+            }
+            if (!__any(any)) continue;
+#pragma unroll
+            for (int m = 0; m < Tile::MF; ++m) acc[m][j] = Type<F16>::mfma(x[m], r, acc[m][j]);
+          }
+        }
       }
     }
   }
@@ -1442,6 +1506,7 @@ struct Room {
   float* factor;  // [n + 1]
   int* splits;    // of dX, as k_dx found them
   float* lost;    // [packed row][residuals] what dl's rounding took
+  int *listed, *starts;  // k_list's, of more than FEW_ROWS tokens: [packed row][residuals], [piece / BUCKET + 1]
   float* parts;   // [parts][v][dp] of dW, where there are more than one
   void* xt;       // Xc^T [dp][n up to 64], for dW in large tiles
   long long bytes;
@@ -1461,6 +1526,13 @@ Room room_of(const tkl_args& a) {
   at += 4;
   r.lost = reinterpret_cast<float*>(at);
   at += 4 * a.n * residuals(a);
+  r.listed = r.starts = nullptr;
+  if ((a.want & 2) && halves(a) == 1 && a.n > FEW_ROWS) {
+    r.listed = reinterpret_cast<int*>(at);
+    at += 4 * a.n * residuals(a);
+    r.starts = reinterpret_cast<int*>(at);
+    at += 4 * (a.piece / BUCKET + 1);
+  }
   at += -(at - static_cast<char*>(a.room)) & 15;
   r.parts = reinterpret_cast<float*>(at);
   if (a.parts > 1) at += 4 * a.parts * a.v * padded(a.d);
@@ -1621,9 +1693,12 @@ template <class Tile, bool F16>
 void dw(const tkl_args& a, const Kept& q, const Room& r, int dp, long long v0, int vn, const Upstream<F16>& up,
         hipStream_t s) {
   const dim3 grid(blocks(a.d, Tile::BM) * blocks(vn, Tile::BN), std::max(1, a.parts));
+  if (r.listed)
+    k_list<<<blocks(vn, BUCKET), 1024, 0, s>>>(q.at, residuals(a), q.count, (int)v0, vn, r.listed, r.starts);
   auto* kernel = r.low ? &k_dw<Tile, F16, true> : &k_dw<Tile, F16, false>;
   kernel<<<grid, Tile::THREADS, Tile::LDS, s>>>(r.xt, 2 * padded(a.n), q.xc, dp, r.dl, a.piece * 2, (int)v0, vn, (int)a.d,
-                                                q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d, r.parts, r.low);
+                                                q.count, up, q.at, r.lost, residuals(a), a.dw, (int)a.d, r.parts, r.low, r.listed,
+                                                r.starts);
   if (a.parts > 1)
     k_dw_out<F16><<<blocks(a.v * (dp / 4), 256), 256, 0, s>>>(r.parts, a.parts, a.v, (int)a.d, dp, up, a.dw);
 }

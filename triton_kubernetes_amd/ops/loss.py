@@ -28,6 +28,7 @@ from .native import NativeUnavailable, load
 
 TILE = 256  # vocabulary entries and tokens of a large tile
 SMALL_M, SMALL_N = 128, 64  # of a small one
+FEW_ROWS = 512  # tokens whose targets every tile of w's gradient looks for itself
 DL_BYTES = 512 << 20  # the backward pass' 16-bit derivative of the logits, per piece
 KEEP_BYTES = 4 << 30  # most logits in 16 bits that a call with keep_logits=None keeps for its backward pass
 MAX_TARGETS = 1024  # ids of a token's list
@@ -139,12 +140,15 @@ def room_bytes(n: int, d: int, piece: int, groups: int, small: int, want: int, l
                weight: int = 0) -> int:
     """Of the backward pass' workspace: the derivative of a piece's logits (twice with ``small & 8``), fp32 sums of x's
     gradient (as many splits as the tiles of ``groups`` workgroups hold, ``want & 1``), factors,
-    the number of splits, residuals, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``,
+    the number of splits, residuals and (of more than ``FEW_ROWS`` tokens, ``want & 2``) their lists by
+    tile of the vocabulary, fp32 sums of w's gradient (``weight`` rows of them) and x transposed (``want & 2``,
     unless ``small & 4``)."""
     once, halves = n * _up(d, 64), 2 if small & 8 else 1
     tiles = groups * (SMALL_M * SMALL_N if small & 2 else TILE * TILE)
     sums = max(once, min(piece // 512 * once, tiles)) if want & 1 else 0
-    return _up(2 * n * piece * halves + 4 * sums + 4 * (n + 2) + (16 * n if lists else 4 * n), 16) \
+    rest = 16 * n if lists else 4 * n
+    listed = rest + 4 * (piece // TILE + 1) if want & 2 and halves == 1 and n > FEW_ROWS else 0
+    return _up(2 * n * piece * halves + 4 * sums + 4 * (n + 2) + rest + listed, 16) \
         + 4 * weight * _up(d, 64) + (2 * _up(d, 64) * _up(n, 64) if want & 2 and not small & 4 else 0)
 
 
@@ -391,11 +395,12 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, reduction: s
     is then off by up to 8.5e-5 of itself, 3.4e-4 below 2^-8 of its tile's largest and 2.7e-3
     below 2^-24, which joins the rounding of the gradient's operands.
 
-    These are in 16 bits: ``x``, ``w``, and the derivative of the logits, rounded to their type.
-    The gradients are then off by up to 1.42 times what rounding them once costs (1.0 for a few
-    confident tokens, 1.18 for a training step of 4096 tokens, 1.41 where a teacher's lists spread the
-    derivative).  ``precise_grad=True`` multiplies the derivative in two 16-bit parts instead, so that
-    little but the result's own rounding is left (1.00 times), for about half as much time again."""
+    These are in 16 bits: ``x``, ``w``, and the derivative of the logits, rounded to their type, of
+    which the targets get back what that took.  The gradients are off by 1.00 times what rounding
+    them once costs where the targets are most of the derivative, as in training; up to 1.35 times was
+    seen where a teacher's lists spread it.  ``precise_grad=True`` multiplies the derivative in two
+    16-bit parts instead, so that little but the result's own rounding is left (1.00 times in any
+    case), for about half as much time again."""
     plan = _planned("linear_cross_entropy", x, w, target, None, reduction, 1.0, int(ignore_index), keep_logits,
                     precise_grad)
     return _apply(x, w, _ids(target), None, plan)
