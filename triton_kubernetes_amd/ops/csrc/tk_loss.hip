@@ -30,9 +30,9 @@
 // rounding took is rounded to 16 bits too and multiplied in its turn, which leaves 2^-16 of dl in
 // bf16, 2^-22 in fp16 (errors 1.000; 4096 x 4096 x 32768 1.55 times as long).
 //
-// Measured at bf16, 8192 tokens x 4096 x 131072: k_logits 6.25 ms forward and 6.55 backward, 1.41 and
-// 1.34 PF (matrix pipe busy 69 and 64 % of the time, at 1.9 GHz), k_dx and k_dw 6.7 ms each, 1.31
-// PF; the rest 0.14 ms.  With the logits kept k_logits 6.5 ms and k_dl 0.72 ms, 5.9 TB/s, instead.
+// Measured at bf16, 8192 tokens x 4096 x 131072: k_logits 6.4 ms forward and 6.6 backward, 1.38 and
+// 1.33 PF (matrix pipe busy 69 and 64 % of the time, at 1.9 GHz), k_dx 6.75 ms and k_dw 7.0, 1.30 and
+// 1.26 PF; the rest 0.16 ms.  With the logits kept k_logits 6.5 ms and k_dl 0.72 ms, 5.9 TB/s, instead.
 // The products are bound by the matrix pipe and LDS together, about 2050 cycles of each in a step
 // of 64 that takes 2800 to 3100.
 //
@@ -1200,7 +1200,8 @@ __global__ __launch_bounds__(256) void k_pad(const T* __restrict__ w, long long 
 // A teacher's lists: zk[pos][j] = x . w[id], one wave for 16 entries of a token.  By matrix instructions
 // in the order of k_logits' steps, so that each is that kernel's logit to the bit: a loss is a
 // difference of the two (a student that is sure of the same entry as its teacher had 4 times the
-// plain form's error with sums of their own order).  An id below 0 is no entry.
+// plain form's error with sums of their own order).  An id below 0 is no entry.  (2048 tokens x 64
+// entries of 2048: 81 to 87 us, 6.4 TB/s.)
 template <bool F16>
 __global__ __launch_bounds__(256) void k_dots(const void* __restrict__ xc, int dp, const void* __restrict__ w,
                                               long long ldw, int dk, const long long* __restrict__ ids, int k,

@@ -75,7 +75,7 @@ def _up(n: int, to: int) -> int:
 def pieces(n: int, v: int) -> int:
     """Vocabulary entries of a piece of the backward pass: as many as keep the derivative of
     ``n`` tokens' logits near ``DL_BYTES``, at most half as much again (a second piece for a little
-    more costs 2 %: 5000 x 2048 x 60000 in one 4004 us, in two 4077), spread evenly, in whole tiles."""
+    more costs 2 %: 5000 x 2048 x 60000 in one 4160 us, in two 4228), spread evenly, in whole tiles."""
     count = max(1, min((4 * n * v // DL_BYTES + 1) // 2, -(-v // TILE)))
     # (of a great many tokens a whole tile more can be past that)
     return min(_up(-(-v // count), TILE), max(TILE, 3 * DL_BYTES // (4 * n) // TILE * TILE))
@@ -86,10 +86,10 @@ def small_products(n: int, d: int, v: int) -> int:
 
     A large tile multiplies faster, a small one wastes less on few tokens and fills more
     compute units.  Measured gain of a small tile over a large one, in us of a whole step at
-    bf16 (n x d x v), where the rules turn: logits, 128 x 4096 x 32000 35 of 388, 192 -11, 256 -41;
-    4096 x 512 x 1000 18 of 98, 8192 3.  x's gradient, 64 x 4096 x 32000 9, 128 6, 192 -12, 128 x
-    4096 x 131072 -58; 2048 x 1024 x 4000 8, 512 x 1024 x 32000 -1, 4096 x 512 x 8000 -3.  w's, 1024 x
-    512 x 8000 (64 large tiles) 14, 1024 x 1024 x 6000 (96) 5, 4096 x 1024 x 8000 (128) -11."""
+    bf16 (n x d x v), where the rules turn: logits, 128 x 4096 x 32000 35 of 387, 192 -9, 256 -38;
+    4096 x 512 x 1000 21 of 111, 8192 4.  x's gradient, 64 x 4096 x 32000 11, 128 8, 192 -10, 128 x
+    4096 x 131072 -50; 2048 x 1024 x 4000 8, 512 x 1024 x 32000 -2, 4096 x 512 x 8000 -3.  w's, 1024 x
+    512 x 8000 (64 large tiles) 16, 1024 x 1024 x 6000 (96) 5, 4096 x 1024 x 8000 (128) -7."""
 
     def tiles(a, b):
         return -(-a // TILE) * -(-b // TILE)
@@ -103,15 +103,15 @@ def keeps(n: int, d: int, v: int) -> bool:
     """Whether a call with ``keep_logits=None`` keeps the logits, in 16 bits, for its backward pass:
     where that is faster than to compute them again.  A short product is cheaper
     than two passes over its result.  A step at bf16, kept and again, in us: 4096 x 4096 x 32768
-    2650 and 3330, 4096 x 512 x 32768 598 both, of width 384 540 both, 256 495 and 456; few tokens read
-    the weight once less (16 x 4096 x 131072 807 and 975, 512 x 256 x 32000 100 and 98)."""
+    2740 and 3440, 4096 x 512 x 32768 617 and 628, of width 384 558 and 566, 256 515 and 487; few tokens
+    read the weight once less (16 x 4096 x 131072 790 and 958, 512 x 256 x 32000 101 and 100)."""
     return (d >= 384 or n <= 512) and 2 * n * v <= KEEP_BYTES
 
 
 def fill(small: bool) -> int:
     """Most workgroups for x's gradient, among which the vocabulary is split: 3 rounds of a large
-    tile for each of the 256 compute units (a step of 5000 x 4000 x 32768, 320 tiles: 4690 us with
-    one round, 4278 with 3 and with 5), or one of two small ones."""
+    tile for each of the 256 compute units (a step of 5000 x 4000 x 32768, 320 tiles: 4820 us with
+    one round, 4370 with 3, 4410 with 5), or one of two small ones."""
     return 512 if small else 768
 
 
